@@ -206,6 +206,23 @@ extern "C" {
         batch_size: usize,
         stream: Stream,
     ) -> c_int;
+    pub fn ellm_attn_set_scores(
+        handle: *mut ellm_attn,
+        score_cap: f32,
+        distance_slopes: *const f32,
+        window: usize,
+        key_begin: *const u32,
+        key_end: *const u32,
+        bounds_pitch: usize,
+    ) -> c_int;
+    pub fn ellm_attn_set_shared_prefix(
+        handle: *mut ellm_attn,
+        k: *const c_void,
+        v: *const c_void,
+        head_stride: usize,
+        position_stride: usize,
+        length: usize,
+    ) -> c_int;
 
     pub fn ellm_kv_create(desc: *const ellm_kv_desc, out_cache: *mut *mut ellm_kv_cache) -> c_int;
     pub fn ellm_kv_create_ragged(desc: *const ellm_kv_ragged_desc, out_cache: *mut *mut ellm_kv_cache) -> c_int;
@@ -455,6 +472,33 @@ impl Attention<Half> {
         check(
             unsafe { ellm_attn_run_ragged(self.handle, positions, max_position, batch_size, self.stream) },
             "ellm_attn_run_ragged",
+        );
+    }
+
+    /// Shaped scores for the runs from here on: a cap (0: none), slopes over the distance (null: none), a window
+    /// (0: none) and a key range for each query position (null: every key up to the query's own).  Device arrays that
+    /// the handle reads in every run.
+    pub fn set_scores(
+        &mut self,
+        score_cap: f32,
+        distance_slopes: *const f32,
+        window: usize,
+        key_begin: *const u32,
+        key_end: *const u32,
+        bounds_pitch: usize,
+    ) {
+        check(
+            unsafe { ellm_attn_set_scores(self.handle, score_cap, distance_slopes, window, key_begin, key_end, bounds_pitch) },
+            "ellm_attn_set_scores",
+        );
+    }
+
+    /// `length` rows of keys and values that all sequences share, ahead of their own rows (0: none); runs count
+    /// positions from the prefix's end.
+    pub fn set_shared_prefix(&mut self, k: *const Half, v: *const Half, head_stride: usize, position_stride: usize, length: usize) {
+        check(
+            unsafe { ellm_attn_set_shared_prefix(self.handle, k.cast(), v.cast(), head_stride, position_stride, length) },
+            "ellm_attn_set_shared_prefix",
         );
     }
 }

@@ -132,6 +132,8 @@ ABI_SYMBOLS = {
     "ellm_attn_run_ragged": (ctypes.c_int, [_vp, _vp, _sz, _sz, _vp]),
     "ellm_attn_ragged_path": (ctypes.c_int, [_vp, _sz, _sz]),
     "ellm_attn_run_noalloc": (ctypes.c_int, [ctypes.POINTER(AttnDesc), _vp, _sz, _sz, _vp]),
+    "ellm_attn_set_scores": (ctypes.c_int, [_vp, ctypes.c_float, _vp, _sz, _vp, _vp, _sz]),
+    "ellm_attn_set_shared_prefix": (ctypes.c_int, [_vp, _vp, _vp, _sz, _sz, _sz]),
     "ellm_kv_create": (ctypes.c_int, [ctypes.POINTER(KvDesc), _pvp]),
     "ellm_kv_create_ragged": (ctypes.c_int, [ctypes.POINTER(KvRaggedDesc), _pvp]),
     "ellm_kv_layer_ragged": (ctypes.c_int, [_vp, _sz, _sz, _pvp, _pvp, ctypes.POINTER(_sz * 4),

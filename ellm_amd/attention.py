@@ -104,6 +104,7 @@ class Attention:
         d.sequence_capacity = cap
         d.max_position_interval = interval
         self.desc = d
+        self._scores = self._prefix = None   # tensors that the handle reads
         self._handle = ctypes.c_void_p()
         if seq_table is not None:
             check(self._lib.ellm_attn_create_ragged(ctypes.byref(d), ctypes.byref(seq_table.table),
@@ -114,6 +115,66 @@ class Attention:
     @classmethod
     def new(cls, *args, **kwargs):
         return cls(*args, **kwargs)
+
+    def set_scores(self, cap=0.0, slopes=None, window=0, key_begin=None, key_end=None):
+        """Shaped scores for the runs from here on (ellm_attn_set_scores): the scaled product x of the query at
+        position p and the key at position j becomes cap tanh(x / cap) - slopes[head] |p - j|, and the query sees the
+        keys key_begin[sequence, p] <= j < key_end[sequence, p] with p - j < window.  slopes: float32 device tensor, one
+        a query head; key_begin, key_end: uint32/int32 device tensors [batch, positions], positions at least the
+        capacity (None: 0 and p + 1).  Without arguments: the plain operator again."""
+        import torch
+
+        d = self.desc
+        if window < 0:
+            raise ValueError(f"a window of {window} positions")
+        if slopes is not None:
+            if not slopes.is_contiguous():
+                raise ValueError("slopes must be contiguous")
+            _device_buffer("slopes", slopes, d.attention_head_num, torch.float32)
+        pitch = 0
+        for name, bound in (("key_begin", key_begin), ("key_end", key_end)):
+            if bound is None:
+                continue
+            if bound.dtype not in (torch.int32, torch.uint32):
+                raise TypeError(f"{name} must hold 32-bit integers, got {bound.dtype}")
+            if bound.dim() != 2 or bound.shape[0] < d.batch_size or bound.shape[1] < d.sequence_capacity:
+                raise ValueError(f"{name} is {tuple(bound.shape)}; the operator reads [{d.batch_size}, {d.sequence_capacity}]")
+            if bound.stride(1) != 1 or bound.stride(0) < bound.shape[1]:
+                raise ValueError(f"{name} must be row-major")
+            if pitch and bound.stride(0) != pitch:
+                raise ValueError("key_begin and key_end must have the same row pitch")
+            pitch = bound.stride(0)
+            _device_buffer(name, bound, (d.batch_size - 1) * pitch + d.sequence_capacity)
+        ptr = [t.data_ptr() if t is not None else None for t in (slopes, key_begin, key_end)]
+        check(self._lib.ellm_attn_set_scores(self._handle, ctypes.c_float(cap), ptr[0], int(window), ptr[1], ptr[2], pitch))
+        self._scores = (slopes, key_begin, key_end)
+
+    def set_shared_prefix(self, k=None, v=None, length=None):
+        """A prefix that all sequences share, ahead of their own rows, for the runs from here on
+        (ellm_attn_set_shared_prefix).  k, v: device tensors [kv_head, position, 128] (any view whose last dimension is
+        contiguous), of which the first `length` positions count (None: all of them); runs count positions from the
+        prefix's end.  Without arguments: no prefix."""
+        if k is None and v is None:
+            check(self._lib.ellm_attn_set_shared_prefix(self._handle, None, None, 0, 0, 0))
+            self._prefix = None
+            return
+        d = self.desc
+        for name, t in (("k", k), ("v", v)):
+            if t is None or t.dim() != 3 or t.shape[0] != d.kv_head_num or t.shape[2] != d.head_size or t.stride(2) != 1:
+                raise ValueError(f"{name} of the prefix must be [{d.kv_head_num}, positions, {d.head_size}], rows contiguous")
+            if _dtype_code(t) != d.dtype:
+                raise TypeError(f"{name} of the prefix is {t.dtype}, not the operator's type")
+        if k.stride() != v.stride():
+            raise ValueError("k and v of the prefix must have the same strides")
+        length = int(min(k.shape[1], v.shape[1]) if length is None else length)
+        if length < 0 or length > min(k.shape[1], v.shape[1]):
+            raise ValueError(f"a prefix of {length} positions in tensors of {k.shape[1]} and {v.shape[1]}")
+        if length:
+            span = (d.kv_head_num - 1) * k.stride(0) + (length - 1) * k.stride(1) + d.head_size
+            _device_buffer("k", k, span)
+            _device_buffer("v", v, span)
+        check(self._lib.ellm_attn_set_shared_prefix(self._handle, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), length))
+        self._prefix = (k, v)
 
     def run(self, position_index, position_interval, batch_size, cpu_num=1, thread_id=0,
             stream=None):
@@ -129,7 +190,8 @@ class Attention:
 
     def ragged_path(self, max_position, batch_size):
         """Which kernel run_ragged takes for this call: 0 = every plane split alike, 1 = the keys
-        of all planes dealt evenly to the workgroups (ellm_attn_ragged_path)."""
+        of all planes dealt evenly to the workgroups, 2 = the kernels for shaped scores and shared prefixes
+        (ellm_attn_ragged_path)."""
         path = self._lib.ellm_attn_ragged_path(self._handle, int(max_position), batch_size)
         if path < 0:
             check(-path)

@@ -185,7 +185,8 @@ struct ellm_kv_cache {
 
 static hipError_t free_workspace(ellm_attn* h) {
   hipError_t first = hipSuccess;
-  void* ptrs[] = {h->ws_acc, h->ws_ml, h->ws2_acc, h->ws2_ml, h->counters, h->part_o, h->part_ml};
+  void* ptrs[] = {h->ws_acc, h->ws_ml, h->ws2_acc, h->ws2_ml, h->counters, h->part_o, h->part_ml,
+                  h->shaped.part_o, h->shaped.part_ml};
   for (void* p : ptrs) {
     if (!p) continue;
     hipError_t e = hipFree(p);
@@ -193,6 +194,7 @@ static hipError_t free_workspace(ellm_attn* h) {
   }
   h->ws_acc = h->ws_ml = h->ws2_acc = h->ws2_ml = h->part_o = h->part_ml = nullptr;
   h->counters = nullptr;
+  h->shaped = ellm::ShapedState{};
   return first;
 }
 
@@ -357,6 +359,7 @@ static bool takes_balanced(const ellm_attn* h, size_t batch, size_t max_position
 }
 
 int ellm::attn_run_single_token(ellm_attn* h, ellm::AttnArgs* a, uint32_t max_position, hipStream_t stream) {
+  if (h->shaped.active()) return ellm::attn_run_shaped(h, *a, stream);
   if (h->general) {
     const hipError_t e = ellm::launch_attn_general(*a, (uint32_t)h->desc.head_size, stream);
     if (e != hipSuccess) return fail_hip(e, "attention launch (general head size)");
@@ -408,6 +411,7 @@ int ellm_attn_run(ellm_attn* h, size_t position_index, size_t position_interval,
   a.position_interval = (uint32_t)position_interval;
   a.batch = (uint32_t)batch_size;
   if (position_interval == 1) return ellm::attn_run_single_token(h, &a, (uint32_t)position_index, (hipStream_t)stream);
+  if (h->shaped.active()) return ellm::attn_run_shaped(h, a, (hipStream_t)stream);
   hipError_t e = h->general ? ellm::launch_attn_general(a, (uint32_t)d.head_size, (hipStream_t)stream)
                             : ellm::launch_prefill(a, (hipStream_t)stream);
   if (e != hipSuccess) return fail_hip(e, "chunk attention launch");
@@ -442,6 +446,7 @@ int ellm_attn_ragged_path(const ellm_attn* h, size_t max_position, size_t batch_
     return -fail(ELLM_ERR_OUT_OF_RANGE, "batch_size %zu / max_position %zu outside the handle's %zu / %zu",
                  batch_size, max_position, h->desc.batch_size, h->desc.sequence_capacity);
   if (h->general) return 0;
+  if (h->shaped.active()) return 2;
   uint32_t wgs = 0;
   return takes_balanced(h, batch_size, max_position, &wgs) ? 1 : 0;
 }
@@ -727,6 +732,11 @@ static int kv_append_attn(ellm_kv_cache* c, size_t layer, ellm_attn* a, const vo
   args.position_interval = 1;
   args.batch = (uint32_t)batch_size;
   args.positions = positions;
+  if (a->shaped.active()) {   // the kernels for shaped scores read finished rows: the two calls one after the other
+    const int st = ellm_kv_append_norm_rope(c, layer, position_index, 1, batch_size, k_src, v_src, batch_size, rope,
+                                            rope_positions, eps, positions, max_position, stream);
+    return st != ELLM_OK ? st : ellm::attn_run_shaped(a, args, (hipStream_t)stream);
+  }
   args.pending.k_rows = k_src;
   args.pending.v_rows = v_src;
   args.pending.rope = rope;

@@ -7,6 +7,7 @@
 
 #include "../../include/ellm_attn.h"
 #include "kernels.hpp"
+#include "shaped.hpp"
 
 struct ellm_attn {
   ellm_attn_desc desc;
@@ -29,6 +30,8 @@ struct ellm_attn {
   std::vector<size_t> caps_host;
   // a head size other than 128 or binary32 storage: every call goes to attn_general.hip
   bool general;
+  // shaped scores and shared prefix (shaped_api.hip); inactive until one of them is set
+  ellm::ShapedState shaped{};
 };
 
 struct ellm_matmul3 {
@@ -50,6 +53,9 @@ void attn_fill_args(const ellm_attn* h, AttnArgs* a);
 // The single-token launch of a handle (a->batch, a->position_index, a->positions, a->pending set):
 // the kernel for sequences of different lengths when the call is large enough, else the split plan.
 int attn_run_single_token(ellm_attn* h, AttnArgs* a, uint32_t max_position, hipStream_t stream);
+
+// Either kind of call of a handle with shaped scores or a shared prefix (a->position_interval set as well).
+int attn_run_shaped(ellm_attn* h, const AttnArgs& a, hipStream_t stream);
 
 // The range checks of ellm_matmul3_run / _run_ragged and the launch arguments of a call
 // (ELLM_OK, or a status with the message recorded).

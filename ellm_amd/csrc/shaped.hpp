@@ -1,0 +1,46 @@
+// Attention with shaped scores (a cap, a slope over the distance, a window, one key range for each query position) and
+// over a prefix that a batch shares: what the host plans, the launches take and the kernels have in common.
+//
+// Keys are counted over both parts a query reads: 0 .. prefix - 1 are the shared prefix, prefix + r is row r of the
+// query's own sequence.  For the query at position p (own row p - prefix) and the key at position j
+//     x = scale q.k;   x <- cap tanh(x / cap)   (with a cap);   x <- x - slope[head] |p - j|   (with slopes)
+// and the row sees begin <= j < end with p - j < window; begin = 0 and end = p + 1 without a range of their own.
+// The kernels work in log2 units on an affine function of one value a score: y = a0 + a1 s - slope2 |p - j| with
+//     s = q.k,                                  a1 = scale log2(e), a0 = 0                     without a cap,
+//     s = 1 / (1 + 2^(q.k . 2 scale log2(e) / cap)),  a1 = -2 cap log2(e), a0 = cap log2(e)    with one
+// (tanh z = 1 - 2 / (1 + e^2z)): two transcendental instructions more a score.  The cap's absolute error is a rounding
+// or two of 2 cap log2(e), 2^-24 relative: 1e-5 of a binary order at a cap of 50, far below a 16-bit weight's 2^-9 or 2^-12.
+#pragma once
+
+#include "kernels.hpp"
+#include "shaped_plan.hpp"
+
+namespace ellm {
+
+// What ellm_attn_set_scores / ellm_attn_set_shared_prefix leave in a handle, and the room both work in.
+struct ShapedState {
+  float cap;                   // 0: none
+  const float* slopes;         // device, one a query head; null: none
+  uint32_t window;             // 0: none
+  const uint32_t* key_begin;   // device [sequence][bounds_pitch]; null: 0
+  const uint32_t* key_end;     // null: position + 1
+  size_t bounds_pitch;
+  const void* prefix_k;        // device; null: no prefix
+  const void* prefix_v;
+  size_t prefix_stride_head, prefix_stride_pos;   // elements
+  uint32_t prefix;             // rows of the prefix
+  float* part_o;               // partial rows [part_rows][128] and [part_rows][2], from the first set call to destroy
+  float* part_ml;
+  size_t part_rows;
+  bool scores() const { return cap != 0.0f || slopes || window || key_begin || key_end; }
+  bool active() const { return scores() || prefix; }
+};
+
+struct ShapedArgs {
+  AttnArgs a;   // description, tables and the run's own fields
+  ShapedState s;
+};
+
+hipError_t launch_shaped(const ShapedArgs& args, hipStream_t stream);
+
+}  // namespace ellm

@@ -40,7 +40,8 @@ const char* mismatch(const ellm_matmul3* m, const ellm_attn* a) {
   return nullptr;
 }
 
-bool fused_takes(const ellm_matmul3* m, size_t batch_size) {
+bool fused_takes(const ellm_matmul3* m, const ellm_attn* a, size_t batch_size) {
+  if (a->shaped.active()) return false;   // (those kernels read finished rows)
   const ellm_matmul3_desc& p = m->d;
   return ellm::project_raw_takes((uint32_t)batch_size, (uint32_t)(p.attention_head_num + 2 * p.kv_head_num),
                                  (uint32_t)p.hidden_size, m->ws && m->counters);
@@ -51,8 +52,8 @@ int run(ellm_matmul3* m, ellm_attn* a, size_t position_index, const uint32_t* po
   if (!m || !a) return ellm::set_error(ELLM_ERR_INVALID_ARGUMENT, "null handle");
   if (batch_size == 0) return ELLM_OK;
   if (const char* why = mismatch(m, a)) return ellm::set_error(ELLM_ERR_INVALID_ARGUMENT, "%s", why);
-  if (!fused_takes(m, batch_size)) {
-    // shapes the few-rows projection does not take: the two ordinary calls, same results
+  if (!fused_takes(m, a, batch_size)) {
+    // shapes the few-rows projection does not take, shaped scores: the two ordinary calls, same results
     const int st = positions ? ellm_matmul3_run_ragged(m, positions, max_position, batch_size, stream)
                              : ellm_matmul3_run(m, position_index, 1, batch_size, stream);
     if (st != ELLM_OK) return st;
@@ -108,7 +109,7 @@ int ellm_matmul3_attn_path(const ellm_matmul3* proj, const ellm_attn* attn, size
   if (batch_size == 0 || batch_size > proj->d.batch_size)
     return -ellm::set_error(ELLM_ERR_OUT_OF_RANGE, "batch_size %zu outside the handles' %zu", batch_size,
                             proj->d.batch_size);
-  return fused_takes(proj, batch_size) ? 1 : 0;
+  return fused_takes(proj, attn, batch_size) ? 1 : 0;
 }
 
 }  // extern "C"

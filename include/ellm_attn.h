@@ -172,7 +172,7 @@ int ellm_attn_run_ragged(ellm_attn* handle, const uint32_t* positions, size_t ma
  * on this handle: 0 = the single-token kernel of ellm_attn_run (every K/V plane split alike,
  * sized for max_position), 1 = the kernel that deals the keys of all planes to the workgroups
  * in equal shares, whatever the sequences' lengths (taken when the call is large enough for
- * the split to matter); negative: a status code (null handle, arguments out of range).  No
+ * the split to matter), 2 = the kernels for shaped scores and shared prefixes; negative: a status code (null handle, arguments out of range).  No
  * counterpart in the reference (its Attention::run has one code path); it lets a test or a
  * harness see which kernel its shapes reach.
  */
@@ -210,6 +210,50 @@ int ellm_attn_ragged_path(const ellm_attn* handle, size_t max_position, size_t b
  */
 int ellm_attn_run_noalloc(const ellm_attn_desc* desc, const uint32_t* positions, size_t position,
                           size_t batch_size, void* stream);
+
+/*
+ * Shaped scores.  From this call on, runs of the handle (ellm_attn_run, ellm_attn_run_ragged, and the calls that
+ * contain one: ellm_matmul3_attn_run*, ellm_kv_append_attn_run*) turn the product x = inverse_sqrt_head * q.k of the
+ * query at position p and the key at position j into
+ *     x <- score_cap * tanh(x / score_cap)                    with a score_cap,
+ *     x <- x - distance_slopes[query head] * |p - j|          with slopes, after the cap,
+ * and the query sees the keys with
+ *     key_begin[p] <= j < key_end[p]  and  p - j < window     only.
+ *   score_cap       : 0 (none) or 2^-10..256 (beyond, the rounding of the cap would show in binary16 weights).
+ *   distance_slopes : device float [attention_head_num], or NULL: no bias.
+ *   window          : 0: none; 1: a query sees no key before its own position.
+ *   key_begin, key_end : device uint32 [batch_size][bounds_pitch], one entry for each position a sequence can hold
+ *                     (bounds_pitch >= sequence_capacity), or NULL: 0 and p + 1.  They say which keys the query at that
+ *                     position sees, later ones too: documents packed into a sequence (begin of the document, p + 1), a
+ *                     prefix that all of its own positions see (0, max(p + 1, prefix length)), padding (0, 0).  key_end
+ *                     counts up to the sequence's capacity; keys it admits must have been written.
+ * A row that sees no key is 0, its lse -infinity.  Keys and values that a row does not see may hold anything, infinities
+ * and NaN included.  All arguments 0 / NULL: the plain operator again.  Takes handles with head_size 128 and 16-bit
+ * storage (else ELLM_ERR_UNSUPPORTED).  The arrays are read by every run, not copied.  Host-side: takes effect with the
+ * next run; a recorded graph keeps what its runs were recorded with.  The first of this call and
+ * ellm_attn_set_shared_prefix on a handle allocates room for the partial results of split walks (at most 68 MB, kept
+ * until destroy), so it belongs ahead of a recording.  The reference has no counterpart (its leaf knows the scaled
+ * product and the causal bound only, src/kernel/generic/flash_attention.rs:60-89).
+ */
+int ellm_attn_set_scores(ellm_attn* handle, float score_cap, const float* distance_slopes, size_t window,
+                         const uint32_t* key_begin, const uint32_t* key_end, size_t bounds_pitch);
+
+/*
+ * A prefix that all sequences of the handle share: `length` rows of keys and values a K/V head, ahead of every
+ * sequence's own rows.
+ *   k, v : device, the prefix's planes: head h's row j starts at k + h * head_stride + j * position_stride (elements,
+ *          multiples of 8, the handle's dtype), e.g. one sequence of a cache layer (ellm_kv_layer: strides [1], [2]).
+ * Runs count positions from the prefix's end, as the cache rows are counted: own row p of a sequence is position
+ * length + p of its text, and the query there sees the whole prefix and own rows 0..p.  ellm_kv_append* and
+ * ellm_matmul3_run* write the own rows at the same positions p, with the rotary table moved on by `length` rows
+ * (rope + length * 128).  Distances and windows of ellm_attn_set_scores count prefix rows too; key ranges do not go
+ * with a prefix (ELLM_ERR_UNSUPPORTED).  Calls with few rows a sequence (single tokens, short chunks) read the prefix
+ * once for all sequences of a K/V head.  length 0: no prefix (k, v and the strides are not looked at).  Limits, room and
+ * effect as for ellm_attn_set_scores; length + sequence_capacity < 2^31.  No counterpart in the reference (every
+ * sequence has rows of its own, src/memory/cache.rs:69-75).
+ */
+int ellm_attn_set_shared_prefix(ellm_attn* handle, const void* k, const void* v, size_t head_stride,
+                                size_t position_stride, size_t length);
 
 /* ------------------------------------------------------------------------ *
  * Key/value cache: one allocation, [layer][sequence][kv_head][position][128],
@@ -346,7 +390,7 @@ int ellm_kv_append_norm_rope(ellm_kv_cache* cache, size_t layer, size_t position
  * the corresponding call is ellm_matmul3_attn_run).
  * attn must have been created over this layer of this cache (k, v, kv_strides of ellm_kv_layer /
  * ellm_kv_layer_ragged from the cache's first sequence, the cache's dtype); else
- * ELLM_ERR_INVALID_ARGUMENT.  k_src, v_src: device, [batch_size][kv_head][128] rows of the new
+ * ELLM_ERR_INVALID_ARGUMENT.  (With shaped scores or a shared prefix: as two launches, the cache write and the run.)  k_src, v_src: device, [batch_size][kv_head][128] rows of the new
  * token; rope, rope_positions, eps, positions, max_position as in ellm_kv_append_norm_rope.
  * The query rows in the operator's q are final (normalised and rotated by the caller's
  * projection).  Results: the cache as ellm_kv_append_norm_rope leaves it, out / lse as
@@ -524,7 +568,8 @@ int ellm_matmul3_reset(ellm_matmul3* handle, void* stream);
  * The handles must describe the same step: proj's q_state / k_state / v_state are attn's
  * q / k / v, same dtype, head counts, batch_size, kv_strides, sequence_capacity and (for caches
  * with per-sequence capacities) the same sequence table; else ELLM_ERR_INVALID_ARGUMENT.
- * Shapes the fused form does not take (more than 64 sequences, hidden_size below 1024) run the two ordinary calls: same results.  ellm_matmul3_attn_path tells
+ * Shapes the fused form does not take (more than 64 sequences, hidden_size below 1024; an attention handle with shaped
+ * scores or a shared prefix) run the two ordinary calls: same results.  ellm_matmul3_attn_path tells
  * which (1 fused, 0 two ordinary calls, negative: a status).  Neither handle may have
  * another call in flight.
  */
