@@ -12,8 +12,18 @@
 // and fill each other's waits.
 //
 // Masks are one key range [lo, hi) a row: a step that all of a wave's rows see whole takes no mask, one that none of them
-// sees is passed over, and in between the range is two compares a score.  Value rows that only some rows of a step see
-// may hold infinities and NaN: such a step looks at its values first (values_odd) and multiplies odd ones apart.
+// sees is passed over, and in between the range is one compare a score.  Value rows that only some rows of a step see
+// may hold infinities and NaN: such a step looks at its values first (find_odd), multiplies odd ones apart and drops them.
+//
+// What bounds it (8192 tokens, 32 / 4 heads, binary16, 550 GFLOP): the board's power and the vector unit, 350 us with
+// constant operands and no weights, 555 without a cap, 645 with one (0.85 PFLOP/s; 69 us a plane's worth of transcendental
+// instructions), 560 with slopes.  Against a plain loop (Q.K, soft-max with a maximum every step, P.V) 740: references
+// that move only where a sum asks for it 8 %, addresses and descriptors in scalar registers that move on 5 %, priority 2 to
+// 9 %, walks from the last step where scores fall with the distance 24 % of those.  Tried and dropped: eight waves of two
+// groups half a step apart (256 rows; 5 % faster on long plain walks, 5 to 10 % slower on short ones), 64 rows a wave (scores land
+// in accumulation registers: twice the time), operands read 3, 6 or 8 ahead (the same).
+#include <type_traits>
+
 #include "common.hpp"
 #include "shaped.hpp"
 
@@ -23,11 +33,12 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kRows = (int)kShapedRows;
+static_assert(kRows == 32 * kWaves, "32 rows a wave");
+constexpr int kBuffers = 2;   // tiles of K, and of V, in LDS
+constexpr int kAhead = 4;     // LDS operand reads in flight ahead of their products
 constexpr int kKeys = (int)kShapedKeys;
 constexpr int kTileBytes = kKeys * kHeadDim * 2;
-constexpr int kAhead = 4;   // LDS operand reads in flight ahead of their product
 constexpr uint32_t kNoKey = 0xffffffffu;
-static_assert(kRows == 32 * kWaves, "32 rows a wave");
 
 typedef __attribute__((address_space(3))) uint16_t LdsHalf;
 typedef __attribute__((address_space(3))) u32x4 LdsU32x4;
@@ -82,41 +93,38 @@ __device__ __forceinline__ void load_to_lds(const u32x4& rsrc, uint32_t voff, ui
                :: "s"(lds_at), "v"(voff), "s"(rsrc) : "memory");
 }
 
-// Where a query row is: sequence, position of its own row, query head.
-struct Row {
-  uint32_t seq, token, head;
-};
-
+// Packed pairs of 16-bit values: which are infinities or NaN, without compares (masks of lanes are scarce registers).
 template <typename T>
-struct Odd;   // bits of infinities and NaN
+struct Odd;
 template <>
 struct Odd<F16> {
-  static constexpr uint32_t kInf = 0x7c00u, kOne = 0x3c00u;
+  static constexpr uint32_t kInf = 0x7c00u, kOne = 0x3c00u, kLast = 0x0400u;   // infinity, one, the exponent's last bit
 };
 template <>
 struct Odd<BF16> {
-  static constexpr uint32_t kInf = 0x7f80u, kOne = 0x3f80u;
+  static constexpr uint32_t kInf = 0x7f80u, kOne = 0x3f80u, kLast = 0x0080u;
 };
-
+constexpr uint32_t both(uint32_t half) { return half * 0x10001u; }
+// the top bit of every half that is odd (an exponent of ones carries into it)
+template <typename T>
+__device__ __forceinline__ uint32_t odd_bits(uint32_t x) {
+  return ((x & both(Odd<T>::kInf)) + both(Odd<T>::kLast)) & both(0x8000u);
+}
+__device__ __forceinline__ uint32_t whole_halves(uint32_t top) { return (top - (top >> 15)) | top; }
 // The operand's finite values, zeros where it has others.
 template <typename T>
 __device__ __forceinline__ u32x4 finite_values(u32x4 a) {
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const uint32_t lo = (a[w] & 0x7fffu) < Odd<T>::kInf ? 0xffffu : 0u, hi = ((a[w] >> 16) & 0x7fffu) < Odd<T>::kInf ? 0xffff0000u : 0u;
-    a[w] &= lo | hi;
-  }
+  for (int w = 0; w < 4; ++w) a[w] &= ~whole_halves(odd_bits<T>(a[w]));
   return a;
 }
-// Ones where the operand has infinities or NaN other than `but`.
+// Ones where the operand has infinities or NaN other than `but` (in both halves).
 template <typename T>
 __device__ __forceinline__ u32x4 odd_values(u32x4 a, uint32_t but) {
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    const uint32_t x = a[w] & 0xffffu, y = a[w] >> 16;
-    const uint32_t lo = ((x & 0x7fffu) >= Odd<T>::kInf) & (x != but) ? Odd<T>::kOne : 0u;
-    const uint32_t hi = ((y & 0x7fffu) >= Odd<T>::kInf) & (y != but) ? Odd<T>::kOne << 16 : 0u;
-    a[w] = lo | hi;
+    const uint32_t d = a[w] ^ but, differs = ((d & both(0x7fffu)) + both(0x7fffu)) | d;   // (top bits)
+    a[w] = whole_halves(odd_bits<T>(a[w]) & differs) & both(Odd<T>::kOne);
   }
   return a;
 }
@@ -124,9 +132,10 @@ __device__ __forceinline__ u32x4 odd_values(u32x4 a, uint32_t but) {
 template <typename T, bool CAP, bool SLOPES>
 __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelArgs p) {
   // K tiles [2][64][128] then V tiles [2][64][128]; of the sixteen 16-byte pieces of a row, piece x of K row r sits at
-  // x ^ (r & 15), of V row r at x ^ 2 (r & 7): reads meet few banks twice
-  __shared__ __attribute__((aligned(256))) uint16_t smem[4 * kKeys * kHeadDim];
-  __shared__ uint32_t s_lo[kWaves], s_hi[kWaves];
+  // x ^ (r & 15), of V row r at x ^ 4 (r & 3): the lanes that a read serves at once (16 rows of a piece, 4 rows of 64
+  // bytes) meet no bank twice
+  __shared__ __attribute__((aligned(256))) uint16_t smem[2 * kBuffers * kKeys * kHeadDim];
+  __shared__ uint32_t s_lo[kWaves], s_hi[kWaves], s_all_lo[kWaves], s_all_hi[kWaves], s_odd[kBuffers];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = (int)uniform((uint32_t)tid >> 6);
@@ -152,51 +161,77 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
     tile = p.tiles_plane - 1 - id / n_split;
   }
   const uint32_t n_rows = on_prefix ? p.prefix_rows : p.rows_plane;
-  const uint32_t at_row = tile * kRows + 32 * wave + j;
-  const bool valid = at_row < n_rows;
+  struct Row {   // this lane's query row: where it is, what it sees
+    bool valid;
+    uint32_t seq, token, head, pos;
+    uint32_t lo, hi;   // (rows that are not stored see everything: they never ask for a mask)
+  };
   Row row;
+  uint32_t wlo = kNoKey, whi = 0;              // the keys that any row of the wave sees
+  uint32_t all_lo = 0, all_hi = kNoKey;        // the keys that every row of the wave sees
   {
-    const uint32_t r = min(at_row, n_rows - 1);
+    const uint32_t at_row = tile * kRows + 32 * wave + j, r = min(at_row, n_rows - 1);
+    row.valid = at_row < n_rows;
     row.seq = on_prefix ? r / p.rows_plane : seq0;
     const uint32_t in_plane = on_prefix ? r % p.rows_plane : r;
     row.token = in_plane / p.group;
     row.head = kvh * p.group + in_plane % p.group;
+    uint32_t own = p.position;   // the query's own row
+    if (p.positions) own = min(p.positions[row.seq], own);
+    const uint32_t cap_seq = p.seq_caps ? p.seq_caps[row.seq] : p.capacity;
+    own = min(own + row.token, cap_seq - 1);
+    row.pos = p.prefix + own;
+    uint32_t lo = 0, hi = row.pos + 1;
+    if (p.key_begin) lo = p.key_begin[row.seq * p.bounds_pitch + own];
+    if (p.key_end) hi = min(p.key_end[row.seq * p.bounds_pitch + own], cap_seq);
+    if (p.window && row.pos + 1 > p.window) lo = max(lo, row.pos + 1 - p.window);
+    // this workgroup's part of the keys: all, the prefix, or the sequence's own rows
+    if (on_prefix) hi = min(hi, p.prefix);
+    if (!on_prefix && p.prefix_tiles) lo = max(lo, p.prefix);
+    if (lo >= hi) lo = hi = 0;   // sees nothing
+    if (row.valid && lo < hi) {
+      wlo = min(wlo, lo);
+      whi = max(whi, hi);
+    }
+    row.lo = row.valid ? lo : 0u;
+    row.hi = row.valid ? hi : kNoKey;
+    all_lo = max(all_lo, row.lo);
+    all_hi = min(all_hi, row.hi);
   }
-  uint32_t own = p.position;   // the query's own row
-  if (p.positions) own = min(p.positions[row.seq], own);
-  const uint32_t cap_seq = p.seq_caps ? p.seq_caps[row.seq] : p.capacity;
-  own = min(own + row.token, cap_seq - 1);
-  const uint32_t pos = p.prefix + own;
-  uint32_t lo = 0, hi = pos + 1;
-  if (p.key_begin) lo = p.key_begin[row.seq * p.bounds_pitch + own];
-  if (p.key_end) hi = min(p.key_end[row.seq * p.bounds_pitch + own], cap_seq);
-  if (p.window && pos + 1 > p.window) lo = max(lo, pos + 1 - p.window);
-  // this workgroup's part of the keys: all, the prefix, or the sequence's own rows
-  if (on_prefix) hi = min(hi, p.prefix);
-  if (!on_prefix && p.prefix_tiles) lo = max(lo, p.prefix);
-  if (lo >= hi) lo = hi = 0;   // sees nothing
-  const bool live = valid && lo < hi;
 
   // ---- the steps from the first to the last key that any row sees, this split's share of them -----
-  uint32_t wlo = live ? lo : kNoKey, whi = live ? hi : 0u;
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) {
     wlo = min(wlo, (uint32_t)__shfl_xor((int)wlo, x));
     whi = max(whi, (uint32_t)__shfl_xor((int)whi, x));
+    all_lo = max(all_lo, (uint32_t)__shfl_xor((int)all_lo, x));
+    all_hi = min(all_hi, (uint32_t)__shfl_xor((int)all_hi, x));
   }
   if (lane == 0) {
     s_lo[wave] = wlo;
     s_hi[wave] = whi;
+    s_all_lo[wave] = all_lo;
+    s_all_hi[wave] = all_hi;
   }
+  if (tid < kBuffers) s_odd[tid] = 0;
   __syncthreads();
-  uint32_t hull_lo = kNoKey, hull_hi = 0;
+  // over the workgroup: the keys that any row sees, those that every row sees
+  uint32_t hull_lo = kNoKey, hull_hi = 0, wg_lo = 0, wg_hi = kNoKey;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
     hull_lo = min(hull_lo, uniform(s_lo[w]));
     hull_hi = max(hull_hi, uniform(s_hi[w]));
+    wg_lo = max(wg_lo, uniform(s_all_lo[w]));
+    wg_hi = min(wg_hi, uniform(s_all_hi[w]));
   }
   wlo = uniform(wlo);
   whi = uniform(whi);
+  all_lo = uniform(all_lo);
+  all_hi = uniform(all_hi);
+  hull_lo = uniform(hull_lo);
+  hull_hi = uniform(hull_hi);
+  wg_lo = uniform(wg_lo);
+  wg_hi = uniform(wg_hi);
   const uint32_t prefix_steps = (p.prefix + kKeys - 1) / kKeys;
   auto step_of = [&](uint32_t key) { return key < p.prefix ? key / kKeys : prefix_steps + (key - p.prefix) / kKeys; };
   uint32_t step = 0, end = 0;
@@ -205,6 +240,27 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
     step = first + (uint32_t)((uint64_t)n * split / n_split);
     end = first + (uint32_t)((uint64_t)n * (split + 1) / n_split);
   }
+  // Scores that fall with the distance are walked from the last step to the first: their references are then found in
+  // the first step instead of moving in every one.  Step s of the walk is step place(s) of the keys.
+  const uint32_t mirror = step + end - 1;
+  auto place = [&](uint32_t s) { return SLOPES ? mirror - s : s; };
+  auto first_key = [&](uint32_t s) {
+    const uint32_t at = place(s);
+    return at < prefix_steps ? at * kKeys : p.prefix + (at - prefix_steps) * kKeys;
+  };
+  auto keys_end = [&](uint32_t s) { return place(s) < prefix_steps ? min(p.prefix, first_key(s) + kKeys) : first_key(s) + kKeys; };
+  // the walk's first step in the other of prefix and own rows than the one it starts in
+  const uint32_t other_part = SLOPES ? mirror + 1 - prefix_steps : prefix_steps;
+  // the steps in which any row of this wave sees keys
+  uint32_t w_begin = end, w_end = end;
+  if (wlo < whi) {
+    const uint32_t from = max(step, step_of(wlo)), to = min(end, step_of(whi - 1) + 1);   // (places; from >= to: none of this split's)
+    w_begin = SLOPES ? mirror + 1 - to : from;
+    w_end = SLOPES ? mirror + 1 - from : to;
+    if (from >= to) w_begin = w_end = end;
+  }
+  w_begin = uniform(w_begin);
+  w_end = uniform(w_end);
 
   u32x4 qreg[8];
   {
@@ -212,51 +268,50 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
 #pragma unroll
     for (int s = 0; s < 8; ++s) qreg[s] = load16(qrow + 16 * s + 8 * g);
   }
-  float slope2 = 0.0f;
-  if constexpr (SLOPES) slope2 = p.slopes[row.head] * kLog2e;
-
-  // rows that are not stored see what the wave's others see, so that they never ask for a mask
-  const uint32_t mlo = valid ? lo : 0u, mhi = valid ? hi : kNoKey;
-  uint32_t all_lo = mlo, all_hi = mhi;   // the keys that every row of the wave sees
-#pragma unroll
-  for (int x = 1; x < 32; x <<= 1) {
-    all_lo = max(all_lo, (uint32_t)__shfl_xor((int)all_lo, x));
-    all_hi = min(all_hi, (uint32_t)__shfl_xor((int)all_hi, x));
-  }
-  all_lo = uniform(all_lo);
-  all_hi = uniform(all_hi);
+  const float slope2 = SLOPES ? p.slopes[row.head] * kLog2e : 0.0f;
 
   // ---- staging ------------------------------------------------------------------------------------
   const size_t plane_at = seq_plane_offset(p.seq_offsets, p.kv_stride_seq, seq0) + kvh * p.kv_stride_head;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(LdsHalf*)smem;
-  const int ld_r = 16 * wave + (lane >> 4), ld_x = lane & 15;   // this lane's piece of each of the wave's four loads: row ld_r + 4 i
+  // four waves move a tile, four loads each; this lane's piece is piece ld_x of row ld_r + 4 i
+  const int ld_r = 16 * wave + (lane >> 4), ld_x = lane & 15;
   const uint32_t wave_lds = lds0 + (uint32_t)wave * 16 * kHeadDim * 2;
-  auto stage = [&](uint32_t s, uint32_t buf) __attribute__((always_inline)) {
-    const bool ahead = s < prefix_steps;   // (uniform)
-    const uint32_t first = (ahead ? s : s - prefix_steps) * kKeys, rows = ahead ? p.prefix : hull_hi - p.prefix;
-    const size_t stride = ahead ? p.prefix_stride_pos : p.kv_stride_pos;
-    const size_t at = (size_t)first * stride + (ahead ? kvh * p.prefix_stride_head : plane_at);
-    // rows past the last one read as zeros
-    const uint64_t span = ((uint64_t)(rows - 1 - first) * stride + kHeadDim) * 2;
-    const uint32_t left = uniform(span > 0xffffffffull ? 0xffffffffu : (uint32_t)span);
-    const uint64_t kat = uniform64((uint64_t)((ahead ? p.prefix_k : p.k) + at)),
-                   vat = uniform64((uint64_t)((ahead ? p.prefix_v : p.v) + at));
-    const u32x4 krsrc = {(uint32_t)kat, (uint32_t)(kat >> 32) & 0xffffu, left, (uint32_t)kBufferFlags};
-    const u32x4 vrsrc = {(uint32_t)vat, (uint32_t)(vat >> 32) & 0xffffu, left, (uint32_t)kBufferFlags};
+  // byte offsets of this lane's pieces: row ld_r + 4 i, of K and of V; they change with the rows' distance only
+  uint32_t off_k[4], off_v[4];
+  auto aim = [&](uint32_t s) __attribute__((always_inline)) {
+    const uint32_t pitch = 2 * (uint32_t)(place(s) < prefix_steps ? p.prefix_stride_pos : p.kv_stride_pos);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t r = ld_r + 4 * i;
+      off_k[i] = r * pitch + 16 * (ld_x ^ (r & 15));
+      off_v[i] = r * pitch + 16 * (ld_x ^ (4 * (r & 3)));
+    }
+  };
+  // Where the next step of K and of V comes from: address, bytes up to the end of its last row that is read (rows past it
+  // read as zeros), bytes from step to step; scalar registers that move on from call to call.
+  struct Source {
+    uint64_t at, left, pace;
+  };
+  auto source = [&](const uint16_t* own_rows, const uint16_t* prefix_rows, uint32_t s) __attribute__((always_inline)) {
+    const bool ahead = place(s) < prefix_steps;   // (uniform)
+    const uint32_t skip = (ahead ? place(s) : place(s) - prefix_steps) * kKeys, n = ahead ? p.prefix : hull_hi - p.prefix;
+    const uint64_t pitch = 2 * (ahead ? p.prefix_stride_pos : p.kv_stride_pos);
+    const uint16_t* plane = ahead ? prefix_rows + kvh * p.prefix_stride_head : own_rows + plane_at;
+    return Source{uniform64((uint64_t)plane + skip * pitch), uniform64((n - 1 - skip) * pitch + 2 * kHeadDim),
+                  uniform64(SLOPES ? 0 - kKeys * pitch : kKeys * pitch)};
+  };
+  // the source's next step on its way into buffer `buf`, pieces at `off`
+  auto send = [&](Source& from, const uint32_t (&off)[4], uint32_t buf) __attribute__((always_inline)) {
+    const uint64_t at = uniform64(from.at);
+    const u32x4 rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu,
+                        uniform(from.left >> 32 ? 0xffffffffu : (uint32_t)from.left), (uint32_t)kBufferFlags};
     const uint32_t to = uniform(wave_lds + buf * kTileBytes);
-    const uint32_t pitch = 2 * (uint32_t)stride;
     // a scalar register that the vector unit wrote (readfirstlane) is a load's to read five wait states later
-    asm volatile("s_nop 4" :: "s"(krsrc), "s"(vrsrc), "s"(to));
+    asm volatile("s_nop 4" :: "s"(rsrc), "s"(to));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t r = ld_r + 4 * i;
-      load_to_lds(krsrc, r * pitch + 16 * (ld_x ^ (r & 15)), to + 4 * i * kHeadDim * 2);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t r = ld_r + 4 * i;
-      load_to_lds(vrsrc, r * pitch + 16 * (ld_x ^ (2 * (r & 7))), to + 2 * kTileBytes + 4 * i * kHeadDim * 2);
-    }
+    for (int i = 0; i < 4; ++i) load_to_lds(rsrc, off[i], to + 4 * i * kHeadDim * 2);
+    from.at += from.pace;
+    from.left -= from.pace;
   };
 
   // A operand of Q.K: keys 32 mb + j, dims 16 s + 8 g ..
@@ -268,7 +323,7 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
   // in two transposing reads (keys +0 and +8).  A 16-lane block of such a read hands lane t element t & 3 of what its lanes
   // 4 e + (t >> 2), e = 0..3, address: lane s of a block points at key s >> 2, dims 4 (s & 3) .. of the block's sixteen.
   const int v_row = 4 * g + ((lane & 15) >> 2), v_piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-  const uint32_t v_read = lds0 + 2 * kTileBytes + v_row * kHeadDim * 2 + 16 * (v_piece ^ (2 * (v_row & 7))) + 8 * (lane & 1);
+  const uint32_t v_read = lds0 + kBuffers * kTileBytes + v_row * kHeadDim * 2 + 16 * (v_piece ^ (4 * (v_row & 3))) + 8 * (lane & 1);
   auto v_operand = [&](uint32_t base, int cc, int db) {   // base: v_read in the step's buffer
     u32x4 a;
 #pragma unroll
@@ -281,166 +336,250 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
     return a;
   };
 
+  Source ksrc = source(p.k, p.prefix_k, step), vsrc = source(p.v, p.prefix_v, step);
+
+  aim(step);
   // ---- walk ---------------------------------------------------------------------------------------
-  float m_run = -INFINITY, l_run = 0.0f;   // reference of the row (log2 units), this lane's share of the sum
+  // minus the row's reference (log2 units; +inf: no key seen yet; rows that will see none need none), this lane's share of its sum
+  float neg_m = row.lo < row.hi ? INFINITY : 0.0f, l_run = 0.0f;
   f32x16 oacc[4];
 #pragma unroll
   for (int db = 0; db < 4; ++db)
 #pragma unroll
     for (int r = 0; r < 16; ++r) oacc[db][r] = 0.0f;
-  const float hidden = p.a1 < 0.0f ? INFINITY : -INFINITY;   // a score that comes out as y = -inf
+  // a score's value once it is finished: y = a1 s + a0 without slopes, y itself with them; one that comes out as -inf
+  const float a0 = SLOPES ? 0.0f : p.a0, a1 = SLOPES ? 1.0f : p.a1;
+  const float hidden = a1 < 0.0f ? INFINITY : -INFINITY;
 
-  if (step < end) stage(step, 0);
-  for (uint32_t buf = 0; step < end; ++step, buf ^= 1) {
-    // this wave's loads have arrived and its reads of the other buffers are done; behind the barrier so have all
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (step + 1 < end) stage(step + 1, buf ^ 1);
-    const bool ahead = step < prefix_steps;
-    const uint32_t kb = ahead ? step * kKeys : p.prefix + (step - prefix_steps) * kKeys;
-    const uint32_t keys_end = ahead ? min(p.prefix, kb + kKeys) : kb + kKeys;
-    if (whi <= kb || wlo >= keys_end) continue;   // no row of this wave sees any of them
-    const bool partly = all_lo > kb || all_hi < kb + kKeys || keys_end < kb + kKeys;
-
-    // operands are read kAhead instructions ahead of the product that takes them; the scheduling barriers keep it so
-    u32x4 ring[kAhead];
-    const uint32_t ks = opaque(k_read + buf * kTileBytes), vs = opaque(v_read + buf * kTileBytes);
-    f32x16 st[2];
+  // keys of the lane: first key + 4 g + off, off = 32 mb + 8 (r >> 2) + (r & 3) for register r of block mb
+  auto off_of = [](int mb, int r) { return 32 * mb + 8 * (r >> 2) + (r & 3); };
+  // what the scores of a step become between the product and the weights, pair n of the eight of a block
+  auto finish = [&](f32x16& st, int mb, int n, float dist) __attribute__((always_inline)) {
 #pragma unroll
-    for (int mb = 0; mb < 2; ++mb)
+    for (int h = 0; h < 2; ++h) {
+      const int r = 2 * n + h;
+      float x = st[r];
+      if constexpr (CAP) x = __builtin_amdgcn_rcpf(fast_exp2(x * p.c_in) + 1.0f);
+      if constexpr (SLOPES) x = __builtin_fmaf(x, p.a1, __builtin_fmaf(-slope2, fabsf(dist - (float)off_of(mb, r)), p.a0));
+      st[r] = x;
+    }
+  };
+  struct Seen {   // which keys of a step a row sees: off - from < width, unsigned
+    int32_t from;
+    uint32_t width;
+  };
+  auto seen_of = [&](uint32_t s) {
+    const uint32_t last = min(row.hi, keys_end(s));
+    return Seen{(int32_t)(row.lo - first_key(s)) - 4 * g, last > row.lo ? last - row.lo : 0u};
+  };
+  auto partly = [&](uint32_t lo, uint32_t hi, uint32_t s) {   // not every one of the rows behind (lo, hi) sees all keys
+    const uint32_t kb = first_key(s);
+    return uniform(lo > kb || hi < kb + kKeys || keys_end(s) < kb + kKeys) != 0;
+  };
+  // st = the finished scores of step s.  (ring: operands are read kAhead ahead of the products that take them; the
+  // scheduling barriers keep the order as it is written.)
+  auto scores = [&](f32x16 (&st)[2], u32x4 (&ring)[kAhead], uint32_t ks, uint32_t s) __attribute__((always_inline)) {
+    const float dist = SLOPES ? (float)((int32_t)(row.pos - first_key(s)) - 4 * g) : 0.0f;
+    f32x16 none;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) st[mb][r] = 0.0f;
+    for (int r = 0; r < 16; ++r) none[r] = 0.0f;
 #pragma unroll
-    for (int n = 0; n < kAhead; ++n) ring[n] = k_operand(ks, n & 1, n >> 1);
+    for (int n = 0; n < kAhead; ++n) ring[n] = k_operand(ks, n >> 3, n & 7);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int n = 0; n < 16; ++n) {
-      st[n & 1] = Mfma<T>::m32x32x16(ring[n % kAhead], qreg[n >> 1], st[n & 1]);
-      if (n + kAhead < 16) ring[n % kAhead] = k_operand(ks, (n + kAhead) & 1, (n + kAhead) >> 1);
+      st[n >> 3] = Mfma<T>::m32x32x16(ring[n % kAhead], qreg[n & 7], (n & 7) == 0 ? none : st[n >> 3]);
+      if constexpr (CAP || SLOPES) {   // (the first half beside the products of the second)
+        if (n >= 8) finish(st[0], 0, n - 8, dist);
+      }
+      if (n + kAhead < 16) ring[n % kAhead] = k_operand(ks, (n + kAhead) >> 3, (n + kAhead) & 7);
       __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (CAP) {
+    if constexpr (CAP || SLOPES) {
+#pragma unroll
+      for (int n = 0; n < 8; ++n) finish(st[1], 1, n, dist);
+    }
+    if (partly(all_lo, all_hi, s)) {
+      const Seen see = seen_of(s);
 #pragma unroll
       for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) st[mb][r] = __builtin_amdgcn_rcpf(fast_exp2(st[mb][r] * p.c_in) + 1.0f);
+        for (int r = 0; r < 16; ++r) st[mb][r] = (uint32_t)(off_of(mb, r) - see.from) < see.width ? st[mb][r] : hidden;
     }
-    // keys of the lane: kb + 4 g + off, off = 32 mb + 8 (r >> 2) + (r & 3)
-    const int32_t from = (int32_t)(mlo - kb) - 4 * g, until = (int32_t)(min(mhi, keys_end) - kb) - 4 * g;
-    if (partly) {
+  };
+  // weights n of the sixteen pairs of st
+  auto weights = [&](const f32x16 (&st)[2], u32x4 (&pk)[4], int n, float shift, float& sum) __attribute__((always_inline)) {
+    const int cc = n >> 2, w = n & 3, mb = cc >> 1, r = 8 * (cc & 1) + 2 * w;
+    const float p0 = fast_exp2(__builtin_fmaf(st[mb][r], a1, shift)), p1 = fast_exp2(__builtin_fmaf(st[mb][r + 1], a1, shift));
+    pk[cc][w] = Mfma<T>::pack2(p0, p1);
+    sum += p0 + p1;
+  };
+  // Where the weights of a step passed what they may add up to, rows move to their maximum and have them computed again.
+  auto settle = [&](const f32x16 (&st)[2], u32x4 (&pk)[4], float sum) __attribute__((always_inline)) {
+    const uint64_t over = __ballot(!(sum <= Mfma<T>::kMaxSum));
+    if (over) {
+      float top = -INFINITY;
 #pragma unroll
       for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int32_t off = 32 * mb + 8 * (r >> 2) + (r & 3);
-          st[mb][r] = off >= from && off < until ? st[mb][r] : hidden;
-        }
-    }
-    // y of the step's scores, with `shift` added
-    const float dist = (float)((int32_t)(pos - kb) - 4 * g);
-    auto y_of = [&](int mb, int r, float shift) __attribute__((always_inline)) {
-      if constexpr (SLOPES) shift = __builtin_fmaf(-slope2, fabsf(dist - (float)(32 * mb + 8 * (r >> 2) + (r & 3))), shift);
-      return __builtin_fmaf(st[mb][r], p.a1, shift);
-    };
-    float top = -INFINITY;
-#pragma unroll
-    for (int mb = 0; mb < 2; ++mb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, y_of(mb, r, p.a0));
-    top = max_with_partner_half(top);
-    if (__any(top > m_run)) {
-      const float m_new = fmaxf(m_run, top);
-      const float alpha = m_new == -INFINITY ? 1.0f : fast_exp2(m_run - m_new);
-      m_run = m_new;
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, __builtin_fmaf(st[mb][r], a1, a0));
+      top = max_with_partner_half(top);
+      // (a row moves by what its own two lanes saw: its bits do not depend on its neighbours)
+      const bool moves = (((over >> j) | (over >> (j + 32))) & 1) != 0;
+      const float neg_new = moves ? fminf(neg_m, -top) : neg_m;   // (+inf while the row has seen no key)
+      const float safe = neg_new == INFINITY ? 0.0f : neg_new;
+      const float alpha = neg_m == INFINITY ? 1.0f : fast_exp2(safe - neg_m);   // (nothing to rescale ahead of a first reference)
+      neg_m = neg_new;
       l_run *= alpha;
 #pragma unroll
       for (int db = 0; db < 4; ++db) oacc[db] *= alpha;
+      sum = 0.0f;
+#pragma unroll
+      for (int n = 0; n < 16; ++n) weights(st, pk, n, a0 + safe, sum);
     }
-    const float shift = p.a0 - (m_run == -INFINITY ? 0.0f : m_run);
-    u32x4 pk[4];
-    float sum = 0.0f;
+    l_run += sum;
+  };
+  // Value rows of which some rows of the workgroup see a part only: infinities and NaN among them (a wave looks at a quarter)
+  const uint32_t v_quarter = lds0 + kBuffers * kTileBytes + wave * (kTileBytes / 4) + 16 * lane;
+  auto find_odd = [&](uint32_t vbuf) __attribute__((always_inline)) {
+    uint32_t found = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const u32x4 x = *(const LdsU32x4*)(v_quarter + vbuf * kTileBytes + i * 1024);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) found |= odd_bits<T>(x[w]);
+    }
+    if (__any(found != 0) && lane == 0) s_odd[vbuf] = 1;
+  };
+  // are multiplied apart: how many a row sees of those that lead to +inf and to -inf (a NaN is one of each) ...
+  auto add_odd = [&](uint32_t vs, uint32_t s) __attribute__((always_inline)) {
+    const Seen see = seen_of(s);
+    const int32_t from = (int32_t)opaque((uint32_t)see.from);
+    const uint32_t width = opaque(see.width);
+    u32x4 ones[4];   // for the keys the row sees
 #pragma unroll
     for (int cc = 0; cc < 4; ++cc)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const int mb = cc >> 1, r = 8 * (cc & 1) + 2 * w;
-        const float p0 = fast_exp2(y_of(mb, r, shift)), p1 = fast_exp2(y_of(mb, r + 1, shift));
-        pk[cc][w] = Mfma<T>::pack2(p0, p1);
-        sum += p0 + p1;
-      }
-    l_run += sum;
-
-    bool odd = false;
-    if (partly) {   // infinities or NaN among the step's values?
-      uint32_t most = 0;
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll 4
-      for (int i = 0; i < 16; ++i) {
-        const u32x4 x = *(const LdsU32x4*)(lds0 + (2 + buf) * kTileBytes + i * 1024 + 16 * lane);
+        ones[cc][w] = 0;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          most = max(most, x[w] & 0x7fff0000u);
-          most = max(most, (x[w] & 0x7fffu) << 16);
+        for (int h = 0; h < 2; ++h) {
+          const int32_t off = off_of(cc >> 1, 8 * (cc & 1) + 2 * w + h);
+          ones[cc][w] |= (uint32_t)(off - from) < width ? Odd<T>::kOne << (16 * h) : 0u;
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      odd = __any((most >> 16) >= Odd<T>::kInf);
+#pragma unroll 1
+    for (int sign = 0; sign < 2; ++sign) {
+      const uint32_t at = opaque(vs), but = both(Odd<T>::kInf | (sign ? 0u : 0x8000u));
+      const float as = sign ? -INFINITY : INFINITY;
+#pragma unroll
+      for (int db = 0; db < 4; ++db) {
+        f32x16 n;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) n[r] = 0.0f;
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+          n = Mfma<T>::m32x32x16(odd_values<T>(v_operand(at, cc, db), but), ones[cc], n);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) oacc[db][r] += n[r] > 0.0f ? as : 0.0f;
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-    __builtin_amdgcn_sched_barrier(0);
-    if (!odd) {
+  };
+  // ... and then taken out of the tile
+  auto drop_odd = [&](uint32_t vbuf) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+      LdsU32x4* at = (LdsU32x4*)(v_quarter + vbuf * kTileBytes + i * 1024);
+      *at = finite_values<T>(*at);
+    }
+  };
+  auto meet = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+
+  // Turn s multiplies K of step s + 1 and V of step s and sends for K of step s + 2 and V of step s + 1: P.V of a step runs
+  // beside the weights of the next, whose vector instructions so find their place between the wave's own matrix
+  // instructions.  Buffers and weights swap from turn to turn; the first turn has no V, the last no K.
+  auto turn = [&](auto kbuf, auto vbuf, u32x4 (&pk)[4], u32x4 (&next)[4], uint32_t s) __attribute__((always_inline)) {
+    // this wave's loads have arrived and its reads of the other buffers are done; behind the barrier so have all
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // (V goes one step behind K: it is sent for first where K is to leave a part)
+    if (s + 1 < end) {
+      if (s + 1 == other_part) vsrc = source(p.v, p.prefix_v, other_part);
+      send(vsrc, off_v, kBuffers + 1 - vbuf);
+    }
+    if (s + 2 < end) {
+      if (s + 2 == other_part) {
+        aim(other_part);
+        ksrc = source(p.k, p.prefix_k, other_part);
+      }
+      send(ksrc, off_k, 1 - kbuf);
+    }
+    const bool has_k = uniform(s + 1 >= w_begin && s + 1 < w_end) != 0, has_v = uniform(s + 1 > w_begin && s < w_end) != 0;
+    const uint32_t vs = opaque(v_read + vbuf * kTileBytes);
+    const bool look = s + 1 != step && partly(wg_lo, wg_hi, s);   // (the first turn has no V; the same for all waves)
+    if (look) find_odd(vbuf);
+    // Weights against the reference that each row already has: while no lane's sum of them passes kMaxSum the step's
+    // maximum is not looked for.  A row without a reference (neg_m = +inf) makes its sums infinite or NaN and so asks for
+    // one; so does a score that is not finite.
+    float sum = 0.0f;
+    const float shift = a0 + neg_m;
+    f32x16 st[2];
+    u32x4 ring[kAhead];
+    __builtin_amdgcn_s_setprio(0);
+    if (has_k) {
+      scores(st, ring, opaque(k_read + kbuf * kTileBytes), s + 1);
+    } else {
+      asm volatile("" : "=v"(st[0]), "=v"(st[1]));   // (whatever the registers hold: nothing comes of it)
+    }
+    __builtin_amdgcn_s_setprio(1);   // (P.V and the weights ahead of the other workgroup's Q.K: 1 to 9 %)
+    if (look) {
+      meet();
+      if (uniform(s_odd[vbuf])) {
+        if (has_v) add_odd(vs, s);
+        meet();
+        drop_odd(vbuf);
+        if (tid == 0) s_odd[vbuf] = 0;
+        meet();
+      }
+    }
+    if (has_v) {
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) ring[n] = v_operand(vs, n >> 2, n & 3);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int n = 0; n < 16; ++n) {
+      for (int n = 0; n < 16; ++n) {   // (the last turn has no scores: its weights go nowhere)
         oacc[n & 3] = Mfma<T>::m32x32x16(ring[n % kAhead], pk[n >> 2], oacc[n & 3]);
+        weights(st, next, n, shift, sum);
         if (n + kAhead < 16) ring[n % kAhead] = v_operand(vs, (n + kAhead) >> 2, (n + kAhead) & 3);
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
-      // finite values as ever; then how many a row sees of those that lead to +inf and to -inf (a NaN is one of each)
-#pragma unroll
-      for (int n = 0; n < 16; ++n) {
-        oacc[n & 3] = Mfma<T>::m32x32x16(finite_values<T>(v_operand(vs, n >> 2, n & 3)), pk[n >> 2], oacc[n & 3]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      const int32_t from2 = (int32_t)opaque((uint32_t)from), until2 = (int32_t)opaque((uint32_t)until);
-#pragma unroll
-      for (int cc = 0; cc < 4; ++cc)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          pk[cc][w] = 0;   // ones for the keys a row sees
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int r = 8 * (cc & 1) + 2 * w + h;
-            const int32_t off = 32 * (cc >> 1) + 8 * (r >> 2) + (r & 3);
-            pk[cc][w] |= (off >= from2) & (off < until2) ? Odd<T>::kOne << (16 * h) : 0u;
-          }
-        }
-#pragma unroll 1
-      for (int sign = 0; sign < 2; ++sign) {
-        const uint32_t at = opaque(vs), but = Odd<T>::kInf | (sign ? 0u : 0x8000u);
-        const float as = sign ? -INFINITY : INFINITY;
-#pragma unroll
-        for (int db = 0; db < 4; ++db) {
-          f32x16 n;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) n[r] = 0.0f;
-#pragma unroll
-          for (int cc = 0; cc < 4; ++cc) {
-            n = Mfma<T>::m32x32x16(odd_values<T>(v_operand(at, cc, db), but), pk[cc], n);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) oacc[db][r] += n[r] > 0.0f ? as : 0.0f;
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      }
+      sum = INFINITY;   // a wave's first step: no row has a reference yet
+    }
+    if (!has_k) return;
+    settle(st, next, sum);
+  };
+  constexpr std::integral_constant<uint32_t, 0> kZero;
+  constexpr std::integral_constant<uint32_t, 1> kOne;
+  if (step < end) {
+    u32x4 even[4], odd[4];
+    send(ksrc, off_k, 0);
+    uint32_t s = step - 1;   // (step 0: one below zero, whose successor is 0 again)
+    for (;;) {
+      turn(kZero, kOne, odd, even, s);
+      if (++s == end) break;
+      turn(kOne, kZero, even, odd, s);
+      if (++s == end) break;
     }
   }
 
   // ---- results ------------------------------------------------------------------------------------
   const float l = sum_with_partner_half(l_run);
-  if (!valid) return;
-  const size_t at = (size_t)row.token * p.batch_pitch + row.seq;
+  const float m = l == 0.0f ? -INFINITY : -neg_m;
+  if (!row.valid) return;
   if (p.n_part == 1) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // (a row that sees no key is 0)
     uint16_t* orow = p.out + row.token * p.q_token_stride + ((size_t)row.seq * p.n_q_heads + row.head) * kHeadDim;
@@ -453,7 +592,8 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
         w[1] = Mfma<T>::pack2(oacc[db][4 * b + 2] * inv, oacc[db][4 * b + 3] * inv);
         *(u32x2*)(orow + 32 * db + 8 * b + 4 * g) = w;
       }
-    if (p.lse && g == 0) p.lse[at * p.n_q_heads + row.head] = (m_run + fast_log2(l)) * kLn2;
+    if (p.lse && g == 0)
+      p.lse[((size_t)row.token * p.batch_pitch + row.seq) * p.n_q_heads + row.head] = (m + fast_log2(l)) * kLn2;
     return;
   }
   const size_t part = (((size_t)row.token * p.batch + row.seq) * p.n_q_heads + row.head) * p.n_part + split + (on_prefix ? p.n_split : 0);
@@ -463,7 +603,7 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
 #pragma unroll
     for (int b = 0; b < 4; ++b)
       *(f32x4*)(prow + 32 * db + 8 * b + 4 * g) = f32x4{oacc[db][4 * b], oacc[db][4 * b + 1], oacc[db][4 * b + 2], oacc[db][4 * b + 3]};
-  if (g == 0) *(f32x2*)(p.part_ml + part * 2) = f32x2{m_run, l};
+  if (g == 0) *(f32x2*)(p.part_ml + part * 2) = f32x2{m, l};
 }
 
 // Joins the partial results of a row: G lanes share its four columns (fold_splits).
