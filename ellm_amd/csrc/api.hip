@@ -359,25 +359,33 @@ static bool takes_balanced(const ellm_attn* h, size_t batch, size_t max_position
 }
 
 int ellm::attn_run_single_token(ellm_attn* h, ellm::AttnArgs* a, uint32_t max_position, hipStream_t stream) {
-  if (h->shaped.active()) return ellm::attn_run_shaped(h, *a, stream);
+  const ellm::ShapedState* shape = h->shaped.active() ? &h->shaped : nullptr;
+  if (shape && shape->prefix) return ellm::attn_run_shaped(h, *a, stream);
   if (h->general) {
     const hipError_t e = ellm::launch_attn_general(*a, (uint32_t)h->desc.head_size, stream);
     if (e != hipSuccess) return fail_hip(e, "attention launch (general head size)");
     return ELLM_OK;
   }
-  uint32_t wgs = 0;
-  if (a->positions && takes_balanced(h, a->batch, max_position, &wgs)) {
-    const hipError_t e = ellm::launch_decode_balanced(*a, wgs, stream);
+  uint32_t wgs = 0, longest = max_position + 1;   // keys that a sequence may see
+  bool uneven = a->positions != nullptr;
+  if (shape) {
+    if (shape->key_end)
+      longest = a->capacity;
+    else if (shape->window && shape->window < longest)
+      longest = shape->window;
+    uneven = uneven || shape->key_begin || shape->key_end;
+  }
+  if (uneven && takes_balanced(h, a->batch, longest - 1, &wgs)) {
+    const hipError_t e = ellm::launch_decode_balanced(*a, wgs, stream, shape);
     if (e != hipSuccess) return fail_hip(e, "single-token attention launch");
     return ELLM_OK;
   }
-  const ellm::DecodePlan plan =
-      ellm::decode_plan(max_position + 1, a->batch, a->n_kv_heads, (uint32_t)h->n_cu);
+  const ellm::DecodePlan plan = ellm::decode_plan(longest, a->batch, a->n_kv_heads, (uint32_t)h->n_cu);
   a->split_len = plan.split_len;
   a->n_split = plan.n_split;
   if (!ellm::decode_plan_fits(h->ws, a->batch, a->n_q_heads, a->n_kv_heads, a->group, a->n_split))
     return fail(ELLM_ERR_OUT_OF_RANGE, "internal: split plan exceeds the workspace");
-  hipError_t e = ellm::launch_decode(*a, stream);
+  hipError_t e = ellm::launch_decode(*a, stream, shape);
   if (e != hipSuccess) return fail_hip(e, "single-token attention launch");
   return ELLM_OK;
 }
@@ -735,7 +743,7 @@ static int kv_append_attn(ellm_kv_cache* c, size_t layer, ellm_attn* a, const vo
   if (a->shaped.active()) {   // the kernels for shaped scores read finished rows: the two calls one after the other
     const int st = ellm_kv_append_norm_rope(c, layer, position_index, 1, batch_size, k_src, v_src, batch_size, rope,
                                             rope_positions, eps, positions, max_position, stream);
-    return st != ELLM_OK ? st : ellm::attn_run_shaped(a, args, (hipStream_t)stream);
+    return st != ELLM_OK ? st : ellm::attn_run_single_token(a, &args, (uint32_t)first, (hipStream_t)stream);
   }
   args.pending.k_rows = k_src;
   args.pending.v_rows = v_src;

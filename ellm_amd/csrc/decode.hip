@@ -32,7 +32,8 @@ namespace {
 // PENDING = kPendSums: the launch of a fused step (ellm_matmul3_attn_run): the query rows and the
 // new key / value row of every plane come as the projection's raw sums (p.pend) and are finished
 // here.  kPendRows (ellm_kv_append_attn_run): the new key / value rows come as stored 16-bit rows.
-template <typename T, int PENDING>
+// SHAPE: shaped scores (decode_common.hpp).
+template <typename T, int PENDING, int SHAPE = kShapeNone>
 __global__ __launch_bounds__(kDecThreads, PENDING ? 2 : 4) void decode_split_kernel(DecodeKernelArgs p) {
   __shared__ __attribute__((aligned(16))) uint16_t smem[kDecWaves * kWaveLdsHalves];
   __shared__ uint32_t s_last;
@@ -48,20 +49,25 @@ __global__ __launch_bounds__(kDecThreads, PENDING ? 2 : 4) void decode_split_ker
   const uint32_t seq = blockIdx.z;
   const Lane t;
 
-  uint32_t pos = p.position;
-  if (p.positions) pos = min(p.positions[seq], p.position);
-  if (p.seq_caps) pos = min(pos, p.seq_caps[seq] - 1);
-  const uint32_t len = pos + 1;
+  const KeyRange range = key_range_of<SHAPE>(p, seq);
+  const uint32_t len = range.len, pos = len - 1;
   const uint32_t k_begin = split * p.split_len;
   const uint32_t k_end = min(len, k_begin + p.split_len);
   const uint32_t heads_here = min((uint32_t)kMaxHeadsPerGroup, p.group - hgrp * kMaxHeadsPerGroup);
   // A split that starts beyond this sequence's keys has nothing to add and is
   // not counted: the merge below derives the live split count from the length.
-  if (k_begin >= len) return;
-
-  const size_t plane = seq_plane_offset(p.seq_offsets, p.kv_stride_seq, seq) + kvh * p.kv_stride_head;
   const uint32_t head0 = kvh * p.group + hgrp * kMaxHeadsPerGroup;
   const uint32_t row0 = seq * p.n_q_heads + head0;  // output row of the group's first head
+  if (k_begin >= len) {
+    if constexpr (SHAPE != kShapeNone) {
+      if (len == 0 && split == 0) emit_empty(p.out, p.lse, row0, heads_here, t.tid);
+    }
+    return;
+  }
+
+  const size_t plane = seq_plane_offset(p.seq_offsets, p.kv_stride_seq, seq) + kvh * p.kv_stride_head +
+                       (SHAPE != kShapeNone ? (size_t)range.first * p.kv_stride_pos : 0);
+  const auto score = score_of<SHAPE>(p, head0 + min((uint32_t)t.c, heads_here - 1), range);
   u32x4 qreg[4];
   float m_run, l_run;
   f32x4 acc[8];
@@ -75,7 +81,7 @@ __global__ __launch_bounds__(kDecThreads, PENDING ? 2 : 4) void decode_split_ker
                                              k_end == len, hgrp == 0);
     if constexpr (PENDING == kPendRows) load_queries(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
     stream_keys<T, PENDING>(p.k + plane, p.v + plane, p.kv_stride_pos, k_begin, k_end, pos, qreg, smem, t,
-                            split * 7u + blockIdx.y * 3u + seq * 5u, p.scale_log2, m_run, l_run, acc, &fresh,
+                            split * 7u + blockIdx.y * 3u + seq * 5u, score, m_run, l_run, acc, &fresh,
                             PENDING == kPendSums ? &queries : nullptr, heads_here);
     // the finished query rows, once per group: by the workgroup that also wrote the new key
     if constexpr (PENDING == kPendSums) {
@@ -84,7 +90,7 @@ __global__ __launch_bounds__(kDecThreads, PENDING ? 2 : 4) void decode_split_ker
   } else {
     load_queries(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
     stream_keys<T>(p.k + plane, p.v + plane, p.kv_stride_pos, k_begin, k_end, pos, qreg, smem, t,
-                   split * 7u + blockIdx.y * 3u + seq * 5u, p.scale_log2, m_run, l_run, acc);
+                   split * 7u + blockIdx.y * 3u + seq * 5u, score, m_run, l_run, acc);
   }
 
   auto final_row = [&](uint32_t h, uint32_t dq, const f32x4& a, float l, float m) {
@@ -132,7 +138,27 @@ __global__ __launch_bounds__(kDecThreads, PENDING ? 2 : 4) void decode_split_ker
 
 }  // namespace
 
-hipError_t launch_decode(const AttnArgs& a, hipStream_t stream) {
+namespace {
+template <typename T>
+void launch_shaped_split(const DecodeKernelArgs& p, dim3 grid, int shape, hipStream_t stream) {
+  const dim3 block(kDecThreads);
+  switch (shape) {
+    case kShapeOn:
+      hipLaunchKernelGGL((decode_split_kernel<T, kPendNone, kShapeOn>), grid, block, 0, stream, p);
+      break;
+    case kShapeOn | kShapeCap:
+      hipLaunchKernelGGL((decode_split_kernel<T, kPendNone, kShapeOn | kShapeCap>), grid, block, 0, stream, p);
+      break;
+    case kShapeOn | kShapeSlopes:
+      hipLaunchKernelGGL((decode_split_kernel<T, kPendNone, kShapeOn | kShapeSlopes>), grid, block, 0, stream, p);
+      break;
+    default:
+      hipLaunchKernelGGL((decode_split_kernel<T, kPendNone, kShapeOn | kShapeCap | kShapeSlopes>), grid, block, 0, stream, p);
+  }
+}
+}  // namespace
+
+hipError_t launch_decode(const AttnArgs& a, hipStream_t stream, const ShapedState* shape) {
   DecodeKernelArgs p;
   p.q = (const uint16_t*)a.q;
   p.k = (const uint16_t*)a.k;
@@ -165,7 +191,13 @@ hipError_t launch_decode(const AttnArgs& a, hipStream_t stream) {
 
   dim3 grid(a.n_split, a.n_kv_heads * p.head_groups, a.batch);
   dim3 block(kDecThreads);
-  if (a.pending.raw) {
+  if (shape) {
+    const int kind = fill_shape(*shape, a, &p.shape);
+    if (a.dtype == 0)
+      launch_shaped_split<F16>(p, grid, kind, stream);
+    else
+      launch_shaped_split<BF16>(p, grid, kind, stream);
+  } else if (a.pending.raw) {
     if (a.dtype == 0)
       hipLaunchKernelGGL((decode_split_kernel<F16, kPendSums>), grid, block, 0, stream, p);
     else

@@ -37,8 +37,9 @@ __device__ __forceinline__ uint32_t uni(uint32_t v) { return (uint32_t)__builtin
 // clusters of 16 pieces take cluster slots p + slot0 / 16 + c, which are distinct for the same
 // reason (1 + floor(n / 16) >= ceil(n / 16)).
 
-// PENDING: the launch of a fused step, as in decode.hip.
-template <typename T, int PENDING>
+// PENDING: the launch of a fused step, as in decode.hip.  SHAPE: shaped scores (decode_common.hpp); lengths are then those
+// of the key ranges.
+template <typename T, int PENDING, int SHAPE = kShapeNone>
 __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeKernelArgs p) {
   __shared__ __attribute__((aligned(16))) uint16_t smem[kDecWaves * kWaveLdsHalves];
   __shared__ uint32_t prefix[kMaxBatch + 1];   // units of the sequences before sequence b (per plane)
@@ -47,11 +48,14 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
   const Lane t;
   const uint32_t B = p.batch;
 
+  // the last row of a sequence's keys, counted from its first (-1: no keys)
   auto position_of = [&](uint32_t b) {
+    if constexpr (SHAPE != kShapeNone) return key_range_of<SHAPE>(p, b).len - 1;
     uint32_t pos = min(p.positions[b], p.position);
     if (p.seq_caps) pos = min(pos, p.seq_caps[b] - 1);
     return pos;
   };
+  auto units_of = [&](uint32_t pos) { return SHAPE != kShapeNone && pos == 0xffffffffu ? 0u : pos / kUnitKeys + 1; };
   // Units per sequence and their running sum.  Up to 64 sequences: every wave keeps them in
   // registers, sequence b in lane b (no LDS, no barrier, and the look-up below is a ballot);
   // more: wave 0 scans them into LDS, 64 at a time.
@@ -79,7 +83,7 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
   if (in_registers) {
     const bool live = (uint32_t)t.lane < B;
     r_pos = live ? position_of(t.lane) : 0u;
-    r_units = live ? r_pos / kUnitKeys + 1 : 0u;
+    r_units = live ? units_of(r_pos) : 0u;
     r_incl = wave_scan(r_units);
     total_units = lane_value(r_incl, kWave - 1);
     umax_all = uni(wave_max(r_units));
@@ -91,7 +95,7 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
         const bool live = base + t.lane < B;
         const uint32_t pos_b = live ? position_of(base + t.lane) : 0u;
         if (live) s_pos[base + t.lane] = pos_b;
-        const uint32_t u = live ? pos_b / kUnitKeys + 1 : 0u;
+        const uint32_t u = live ? units_of(pos_b) : 0u;
         const uint32_t incl = wave_scan(u);
         if (live) prefix[base + t.lane + 1] = carry + incl;
         carry += __shfl(incl, kWave - 1, kWave);
@@ -110,6 +114,11 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
     umin_all = uni(s_umin);
   }
 
+  if constexpr (SHAPE != kShapeNone) {
+    for (uint32_t b = blockIdx.x; b < B; b += gridDim.x)   // sequences without keys are in nobody's share
+      if (uni(position_of(b)) == 0xffffffffu) emit_empty(p.out, p.lse, (size_t)b * p.n_q_heads, p.n_q_heads, t.tid);
+    if (total_units == 0) return;
+  }
   // Units without keys in front of every plane's first (decode_shares.hpp).
   const uint32_t charge = balanced_charge(umax_all, umin_all, total_units, B);
   r_units += charge;
@@ -197,8 +206,14 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
     const uint32_t k_end = min(pos + 1, a_end * kUnitKeys);
     const uint32_t kvh = pl / p.head_groups, hgrp = pl % p.head_groups;
     const uint32_t heads_here = min((uint32_t)kMaxHeadsPerGroup, p.group - hgrp * kMaxHeadsPerGroup);
-    const size_t plane = seq_plane_offset(p.seq_offsets, p.kv_stride_seq, seq) + kvh * p.kv_stride_head;
+    size_t plane = seq_plane_offset(p.seq_offsets, p.kv_stride_seq, seq) + kvh * p.kv_stride_head;
     const uint32_t head0 = kvh * p.group + hgrp * kMaxHeadsPerGroup;
+    KeyRange range{0u, pos + 1, (int32_t)pos};
+    if constexpr (SHAPE != kShapeNone) {
+      range = key_range_of<SHAPE>(p, seq);
+      plane += (size_t)range.first * p.kv_stride_pos;
+    }
+    const auto score = score_of<SHAPE>(p, head0 + min((uint32_t)t.c, heads_here - 1), range);
     const uint32_t row0 = seq * p.n_q_heads + head0;
     u32x4 qreg[4];
     float m_run, l_run;
@@ -213,7 +228,7 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
                                                k_end == pos + 1, hgrp == 0);
       if constexpr (PENDING == kPendRows) load_queries(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
       stream_keys<T, PENDING>(p.k + plane, p.v + plane, p.kv_stride_pos, k_begin, k_end, pos, qreg, smem, t,
-                              w * 7u + pl * 3u + seq * 5u, p.scale_log2, m_run, l_run, acc, &fresh,
+                              w * 7u + pl * 3u + seq * 5u, score, m_run, l_run, acc, &fresh,
                               PENDING == kPendSums ? &queries : nullptr, heads_here);
       if constexpr (PENDING == kPendSums) {
         if (fresh.present) store_queries(const_cast<uint16_t*>(p.q) + (size_t)row0 * kHeadDim, t, heads_here, qreg);
@@ -221,7 +236,7 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
     } else {
       load_queries(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
       stream_keys<T>(p.k + plane, p.v + plane, p.kv_stride_pos, k_begin, k_end, pos, qreg, smem, t,
-                     w * 7u + pl * 3u + seq * 5u, p.scale_log2, m_run, l_run, acc);
+                     w * 7u + pl * 3u + seq * 5u, score, m_run, l_run, acc);
     }
 
     auto final_row = [&](uint32_t h, uint32_t dq, const f32x4& av, float l, float m) {
@@ -275,7 +290,27 @@ bool decode_balanced_takes(const DecodeWorkspace& w, uint32_t batch, uint32_t n_
   return slots * G <= w.rows && cslots * G <= w.rows2 && cslots + planes <= w.counters;
 }
 
-hipError_t launch_decode_balanced(const AttnArgs& a, uint32_t wgs, hipStream_t stream) {
+namespace {
+template <typename T>
+void launch_shaped_balanced(const DecodeKernelArgs& p, dim3 grid, int shape, hipStream_t stream) {
+  const dim3 block(kDecThreads);
+  switch (shape) {
+    case kShapeOn:
+      hipLaunchKernelGGL((decode_balanced_kernel<T, kPendNone, kShapeOn>), grid, block, 0, stream, p);
+      break;
+    case kShapeOn | kShapeCap:
+      hipLaunchKernelGGL((decode_balanced_kernel<T, kPendNone, kShapeOn | kShapeCap>), grid, block, 0, stream, p);
+      break;
+    case kShapeOn | kShapeSlopes:
+      hipLaunchKernelGGL((decode_balanced_kernel<T, kPendNone, kShapeOn | kShapeSlopes>), grid, block, 0, stream, p);
+      break;
+    default:
+      hipLaunchKernelGGL((decode_balanced_kernel<T, kPendNone, kShapeOn | kShapeCap | kShapeSlopes>), grid, block, 0, stream, p);
+  }
+}
+}  // namespace
+
+hipError_t launch_decode_balanced(const AttnArgs& a, uint32_t wgs, hipStream_t stream, const ShapedState* shape) {
   DecodeKernelArgs p;
   p.q = (const uint16_t*)a.q;
   p.k = (const uint16_t*)a.k;
@@ -309,7 +344,13 @@ hipError_t launch_decode_balanced(const AttnArgs& a, uint32_t wgs, hipStream_t s
   p.counters_per_plane = 0;
   p.pend = a.pending;
   const dim3 grid(wgs), block(kDecThreads);
-  if (a.pending.raw) {
+  if (shape) {
+    const int kind = fill_shape(*shape, a, &p.shape);
+    if (a.dtype == 0)
+      launch_shaped_balanced<F16>(p, grid, kind, stream);
+    else
+      launch_shaped_balanced<BF16>(p, grid, kind, stream);
+  } else if (a.pending.raw) {
     if (a.dtype == 0)
       hipLaunchKernelGGL((decode_balanced_kernel<F16, kPendSums>), grid, block, 0, stream, p);
     else

@@ -6,6 +6,7 @@
 
 #include "common.hpp"
 #include "kernels.hpp"
+#include "shaped.hpp"
 
 namespace ellm {
 namespace dec {
@@ -25,6 +26,18 @@ constexpr int kItems = kMaxHeadsPerGroup * kQuads / kDecThreads;  // (head, four
 constexpr int kRedPitch = kHeadDim + 4;         // floats per (wave, head) row of the wave merge, 16-byte aligned
 static_assert(kDecWaves * kMaxHeadsPerGroup * kRedPitch * 4 <= kDecWaves * kWaveLdsHalves * 2,
               "reduction buffer must fit in the staging buffers");
+
+// Shaped scores in the single-token kernels (template argument SHAPE): none, or on, with a cap, with slopes.  A sequence's
+// key range is taken as a plane of its own that begins at the range's first row, so nothing but the scores changes.
+constexpr int kShapeNone = 0, kShapeOn = 1, kShapeCap = 2, kShapeSlopes = 4;
+struct ShapeArgs {
+  const float* slopes;
+  const uint32_t* key_begin;   // per position, as in ShapedState
+  const uint32_t* key_end;
+  size_t bounds_pitch;
+  uint32_t window, prefix, capacity;
+  ShapedScores f;
+};
 
 struct DecodeKernelArgs {
   const uint16_t* q;
@@ -49,7 +62,68 @@ struct DecodeKernelArgs {
   uint32_t wgs_one;   // workgroups that find a compute unit each (decode_balanced.hip)
   float scale_log2;   // scale * log2(e)
   PendingRows pend;   // raw query / key / value rows of a fused step (kernels built with PENDING)
+  ShapeArgs shape;    // kernels built with SHAPE
 };
+
+// What a sequence's query sees: `len` of the sequence's own rows from row `first` on (none: 0), itself at row `pos` counted
+// from `first` (below it where later keys are visible, or at it).
+struct KeyRange {
+  uint32_t first, len;
+  int32_t pos;
+};
+template <int SHAPE>
+__device__ __forceinline__ KeyRange key_range_of(const DecodeKernelArgs& p, uint32_t seq) {
+  uint32_t pos = p.position;
+  if (p.positions) pos = min(p.positions[seq], p.position);
+  if (p.seq_caps) pos = min(pos, p.seq_caps[seq] - 1);
+  if constexpr (SHAPE == kShapeNone) return KeyRange{0u, pos + 1, (int32_t)pos};
+  uint32_t lo = 0, hi = pos + 1;
+  if (p.shape.key_begin) lo = p.shape.key_begin[seq * p.shape.bounds_pitch + pos];
+  if (p.shape.key_end) hi = min(p.shape.key_end[seq * p.shape.bounds_pitch + pos], p.seq_caps ? p.seq_caps[seq] : p.shape.capacity);
+  if (p.shape.window && pos + 1 > p.shape.window) lo = max(lo, pos + 1 - p.shape.window);
+  return KeyRange{lo < hi ? lo : 0u, lo < hi ? hi - lo : 0u, (int32_t)(pos - lo)};
+}
+
+// Host: what a launch takes of a handle's shaped scores; the kernels' SHAPE.
+inline int fill_shape(const ShapedState& s, const AttnArgs& a, ShapeArgs* shape) {
+  shape->slopes = s.slopes;
+  shape->key_begin = s.key_begin;
+  shape->key_end = s.key_end;
+  shape->bounds_pitch = s.bounds_pitch;
+  shape->window = s.window;
+  shape->prefix = s.prefix;
+  shape->capacity = a.capacity;
+  shape->f = shaped_scores(s, a.scale);
+  return kShapeOn | (s.cap != 0.0f ? kShapeCap : 0) | (s.slopes ? kShapeSlopes : 0);
+}
+
+// A score from a product, in log2 units, by the key's row.
+struct PlainScore {
+  float scale_log2;
+  __device__ __forceinline__ float operator()(float qk, uint32_t) const { return qk * scale_log2; }
+};
+template <int SHAPE>
+struct ShapedScore {
+  ShapedScores f;
+  float slope2, pos;   // of this lane's head (log2 units); the query's row
+  __device__ __forceinline__ float operator()(float qk, uint32_t key) const {
+    float x = qk;
+    if constexpr ((SHAPE & kShapeCap) != 0) x = __builtin_amdgcn_rcpf(fast_exp2(x * f.c_in) + 1.0f);
+    x = __builtin_fmaf(x, f.a1, f.a0);
+    if constexpr ((SHAPE & kShapeSlopes) != 0) x = __builtin_fmaf(-slope2, fabsf(pos - (float)key), x);
+    return x;
+  }
+};
+// head: this lane's query head (any, of those past the group's end)
+template <int SHAPE>
+__device__ __forceinline__ auto score_of(const DecodeKernelArgs& p, uint32_t head, const KeyRange& range) {
+  if constexpr (SHAPE == kShapeNone) {
+    return PlainScore{p.scale_log2};
+  } else {
+    const float slope = (SHAPE & kShapeSlopes) != 0 ? p.shape.slopes[head] * kLog2e : 0.0f;
+    return ShapedScore<SHAPE>{p.shape.f, slope, (float)range.pos};
+  }
+}
 
 // Agent-scope (device-wide coherent) relaxed 8-byte load / store of a pair of floats.
 __device__ __forceinline__ uint64_t load_coherent64(const float* p) {
@@ -306,11 +380,11 @@ struct NewRowLoads<kPendNone> {
 // request (`queries` holds the requested raw query rows; qreg is filled here), so that both
 // trips to memory run side by side.  With kPendRows (a fused cache write) the new rows come as
 // stored 16-bit rows, the query rows are final (qreg filled by the caller, `queries` null).
-template <typename T, int PENDING = kPendNone>
+template <typename T, int PENDING = kPendNone, typename Score>
 __device__ __forceinline__ void stream_keys(const uint16_t* kplane, const uint16_t* vplane, size_t stride_pos,
                                             uint32_t k_begin, uint32_t k_end, uint32_t pos,
                                             u32x4 (&qreg)[4], uint16_t* smem, const Lane& t,
-                                            uint32_t rot_seed, float scale_log2, float& m_out, float& l_out,
+                                            uint32_t rot_seed, const Score& score, float& m_out, float& l_out,
                                             f32x4 (&acc)[8], const NewRow* fresh = nullptr,
                                             const PendingQueries* queries = nullptr, uint32_t heads_here = 0) {
   const int g = t.g, c = t.c, wave = t.wave;
@@ -378,7 +452,7 @@ __device__ __forceinline__ void stream_keys(const uint16_t* kplane, const uint16
     float tmax = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      tt[r] = (kb + 4 * g + r <= last) ? st[r] * scale_log2 : -INFINITY;
+      tt[r] = (kb + 4 * g + r <= last) ? score(st[r], kb + 4 * g + r) : -INFINITY;
       tmax = fmaxf(tmax, tt[r]);
     }
     tmax = fmaxf(tmax, xor_shuffle(tmax, 16));
@@ -500,6 +574,14 @@ __device__ __forceinline__ void emit_final(uint16_t* out, float* lse, size_t row
   w[1] = Mfma<T>::pack2(a[2] * inv, a[3] * inv);
   *(u32x2*)(out + row * kHeadDim + 4 * dq) = w;
   if (lse && dq == 0) lse[row] = (m + fast_log2(l)) * kLn2;
+}
+
+// Output rows of a group whose sequence sees no key: 0, log-sum-exp -infinity.
+__device__ __forceinline__ void emit_empty(uint16_t* out, float* lse, size_t row0, uint32_t heads_here, int tid) {
+  for (uint32_t i = tid; i < heads_here * kQuads; i += kDecThreads) {
+    *(u32x2*)(out + row0 * kHeadDim + 4 * i) = u32x2{0u, 0u};
+    if (lse && i % kQuads == 0) lse[row0 + i / kQuads] = -INFINITY;
+  }
 }
 
 // Partial row `prow` of a table of partials: columns 4 dq .. and, once per row, (max, sum).

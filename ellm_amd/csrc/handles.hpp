@@ -54,7 +54,7 @@ void attn_fill_args(const ellm_attn* h, AttnArgs* a);
 // the kernel for sequences of different lengths when the call is large enough, else the split plan.
 int attn_run_single_token(ellm_attn* h, AttnArgs* a, uint32_t max_position, hipStream_t stream);
 
-// Either kind of call of a handle with shaped scores or a shared prefix (a->position_interval set as well).
+// Chunks of a handle with shaped scores, any call of one with a shared prefix (a->position_interval set as well).
 int attn_run_shaped(ellm_attn* h, const AttnArgs& a, hipStream_t stream);
 
 // The range checks of ellm_matmul3_run / _run_ragged and the launch arguments of a call

@@ -76,12 +76,14 @@ struct AttnArgs {
   PendingRows pending;   // single-token path only
 };
 
-hipError_t launch_decode(const AttnArgs& a, hipStream_t stream);
+struct ShapedState;
+// (shape: null, or the shaped scores of the call's handle; then every sequence's own rows only, and nothing pending)
+hipError_t launch_decode(const AttnArgs& a, hipStream_t stream, const ShapedState* shape = nullptr);
 // Per-sequence positions, the planes' keys dealt evenly to `wgs` workgroups (decode_balanced.hip):
 // whether a call of this shape goes there, and the launch (a.positions must be set).
 bool decode_balanced_takes(const DecodeWorkspace& w, uint32_t batch, uint32_t n_kv_heads, uint32_t group,
                            uint32_t max_len, uint32_t wgs);
-hipError_t launch_decode_balanced(const AttnArgs& a, uint32_t wgs, hipStream_t stream);
+hipError_t launch_decode_balanced(const AttnArgs& a, uint32_t wgs, hipStream_t stream, const ShapedState* shape = nullptr);
 hipError_t launch_prefill(const AttnArgs& a, hipStream_t stream);
 // Any head size up to 256 and binary32 storage (dtype 2): chunk and single-token calls alike.
 hipError_t launch_attn_general(const AttnArgs& a, uint32_t head_size, hipStream_t stream);

@@ -36,6 +36,24 @@ struct ShapedState {
   bool active() const { return scores() || prefix; }
 };
 
+// Scores in the kernels' terms: y = a0 + a1 s, s as above (c_in: what q.k is multiplied by under a cap).
+struct ShapedScores {
+  float c_in, a0, a1;
+};
+inline ShapedScores shaped_scores(const ShapedState& s, float scale) {
+  constexpr float kLog2E = 1.4426950408889634f;
+  ShapedScores f{0.0f, 0.0f, scale * kLog2E};
+  if (s.cap != 0.0f) {
+    f.c_in = 2.0f * scale * kLog2E / s.cap;
+    f.a0 = s.cap * kLog2E;
+    f.a1 = -2.0f * f.a0;
+  } else if (!(f.a1 >= 1e-37f || f.a1 <= -1e-37f)) {
+    // (a hidden score is an infinity times a1: a scale of zero is taken as one that no finite sum of products feels)
+    f.a1 = 1e-37f;
+  }
+  return f;
+}
+
 struct ShapedArgs {
   AttnArgs a;   // description, tables and the run's own fields
   ShapedState s;

@@ -714,16 +714,10 @@ hipError_t launch_shaped(const ShapedArgs& args, hipStream_t stream) {
   p.prefix_tiles = plan.prefix_tiles;
   p.prefix_split = plan.prefix_split;
   p.n_part = plan.n_part;
-  if (s.cap != 0.0f) {
-    p.c_in = 2.0f * a.scale * kLog2e / s.cap;
-    p.a0 = s.cap * kLog2e;
-    p.a1 = -2.0f * p.a0;
-  } else {
-    p.a0 = 0.0f;
-    p.a1 = a.scale * kLog2e;
-    // (a hidden score is an infinity times a1: a scale of zero is taken as one that no finite sum of products feels)
-    if (!(fabsf(p.a1) >= 1e-37f)) p.a1 = 1e-37f;
-  }
+  const ShapedScores f = shaped_scores(s, a.scale);
+  p.c_in = f.c_in;
+  p.a0 = f.a0;
+  p.a1 = f.a1;
   return a.dtype == 0 ? launch<F16>(p, s.cap != 0.0f, s.slopes != nullptr, stream)
                       : launch<BF16>(p, s.cap != 0.0f, s.slopes != nullptr, stream);
 }
