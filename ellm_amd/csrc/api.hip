@@ -360,13 +360,29 @@ static bool takes_balanced(const ellm_attn* h, size_t batch, size_t max_position
 
 int ellm::attn_run_single_token(ellm_attn* h, ellm::AttnArgs* a, uint32_t max_position, hipStream_t stream) {
   const ellm::ShapedState* shape = h->shaped.active() ? &h->shaped : nullptr;
-  if (shape && shape->prefix) return ellm::attn_run_shaped(h, *a, stream);
+  ellm::ShapedState behind;   // the shape of a call behind a shared prefix: what the launch over the prefix left
+  if (shape && shape->prefix) {
+    const uint32_t own = max_position + 1;
+    const ellm::PrefixStep how = ellm::shaped_prefix_step(a->batch, a->n_kv_heads, a->group, own, shape->prefix, a->n_cu);
+    if (how == ellm::PrefixStep::kMixed || (size_t)a->batch * a->n_q_heads > shape->part_rows)
+      return ellm::attn_run_shaped(h, *a, stream);
+    behind = *shape;
+    if (how == ellm::PrefixStep::kWalk) {
+      behind.walk_prefix = true;
+    } else {
+      const hipError_t e = ellm::launch_shaped_prefix(ellm::ShapedArgs{*a, h->shaped}, &behind.prefix_parts, stream);
+      if (e != hipSuccess) return fail_hip(e, "attention launch (shared prefix)");
+    }
+    shape = &behind;
+  }
   if (h->general) {
     const hipError_t e = ellm::launch_attn_general(*a, (uint32_t)h->desc.head_size, stream);
     if (e != hipSuccess) return fail_hip(e, "attention launch (general head size)");
     return ELLM_OK;
   }
   uint32_t wgs = 0, longest = max_position + 1;   // keys that a sequence may see
+  const bool walk = shape && shape->walk_prefix;
+  if (walk) longest += shape->prefix;
   bool uneven = a->positions != nullptr;
   if (shape) {
     if (shape->key_end)
@@ -375,7 +391,7 @@ int ellm::attn_run_single_token(ellm_attn* h, ellm::AttnArgs* a, uint32_t max_po
       longest = shape->window;
     uneven = uneven || shape->key_begin || shape->key_end;
   }
-  if (uneven && takes_balanced(h, a->batch, longest - 1, &wgs)) {
+  if (uneven && !walk && takes_balanced(h, a->batch, longest - 1, &wgs)) {
     const hipError_t e = ellm::launch_decode_balanced(*a, wgs, stream, shape);
     if (e != hipSuccess) return fail_hip(e, "single-token attention launch");
     return ELLM_OK;

@@ -65,8 +65,7 @@ __global__ __launch_bounds__(kDecThreads, PENDING ? 2 : 4) void decode_split_ker
     return;
   }
 
-  const size_t plane = seq_plane_offset(p.seq_offsets, p.kv_stride_seq, seq) + kvh * p.kv_stride_head +
-                       (SHAPE != kShapeNone ? (size_t)range.first * p.kv_stride_pos : 0);
+  const size_t plane = seq_plane_offset(p.seq_offsets, p.kv_stride_seq, seq) + kvh * p.kv_stride_head;
   const auto score = score_of<SHAPE>(p, head0 + min((uint32_t)t.c, heads_here - 1), range);
   u32x4 qreg[4];
   float m_run, l_run;
@@ -80,7 +79,7 @@ __global__ __launch_bounds__(kDecThreads, PENDING ? 2 : 4) void decode_split_ker
                                              const_cast<uint16_t*>(p.v) + plane + (size_t)pos * p.kv_stride_pos,
                                              k_end == len, hgrp == 0);
     if constexpr (PENDING == kPendRows) load_queries(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
-    stream_keys<T, PENDING>(p.k + plane, p.v + plane, p.kv_stride_pos, k_begin, k_end, pos, qreg, smem, t,
+    stream_keys<T, PENDING>(planes_of<SHAPE>(p, plane, kvh, range), k_begin, k_end, pos, qreg, smem, t,
                             split * 7u + blockIdx.y * 3u + seq * 5u, score, m_run, l_run, acc, &fresh,
                             PENDING == kPendSums ? &queries : nullptr, heads_here);
     // the finished query rows, once per group: by the workgroup that also wrote the new key
@@ -89,12 +88,12 @@ __global__ __launch_bounds__(kDecThreads, PENDING ? 2 : 4) void decode_split_ker
     }
   } else {
     load_queries(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
-    stream_keys<T>(p.k + plane, p.v + plane, p.kv_stride_pos, k_begin, k_end, pos, qreg, smem, t,
+    stream_keys<T>(planes_of<SHAPE>(p, plane, kvh, range), k_begin, k_end, pos, qreg, smem, t,
                    split * 7u + blockIdx.y * 3u + seq * 5u, score, m_run, l_run, acc);
   }
 
   auto final_row = [&](uint32_t h, uint32_t dq, const f32x4& a, float l, float m) {
-    emit_final<T>(p.out, p.lse, row0 + h, dq, a, l, m);
+    emit_joined<T, SHAPE>(p, row0 + h, dq, a, l, m);
   };
   merge_waves(smem, t, heads_here, m_run, l_run, acc,
               [&](uint32_t h, uint32_t dq, const f32x4& a, float l, float m) {
@@ -139,21 +138,13 @@ __global__ __launch_bounds__(kDecThreads, PENDING ? 2 : 4) void decode_split_ker
 }  // namespace
 
 namespace {
-template <typename T>
-void launch_shaped_split(const DecodeKernelArgs& p, dim3 grid, int shape, hipStream_t stream) {
-  const dim3 block(kDecThreads);
-  switch (shape) {
-    case kShapeOn:
-      hipLaunchKernelGGL((decode_split_kernel<T, kPendNone, kShapeOn>), grid, block, 0, stream, p);
-      break;
-    case kShapeOn | kShapeCap:
-      hipLaunchKernelGGL((decode_split_kernel<T, kPendNone, kShapeOn | kShapeCap>), grid, block, 0, stream, p);
-      break;
-    case kShapeOn | kShapeSlopes:
-      hipLaunchKernelGGL((decode_split_kernel<T, kPendNone, kShapeOn | kShapeSlopes>), grid, block, 0, stream, p);
-      break;
-    default:
-      hipLaunchKernelGGL((decode_split_kernel<T, kPendNone, kShapeOn | kShapeCap | kShapeSlopes>), grid, block, 0, stream, p);
+// the kernel for the shape `kind`, found among KIND and those below it
+template <typename T, int KIND = kShapeOn | kShapeCap | kShapeSlopes | kShapeWalk>
+void launch_shaped_split(const DecodeKernelArgs& p, dim3 grid, int kind, hipStream_t stream) {
+  if (kind == KIND) {
+    hipLaunchKernelGGL((decode_split_kernel<T, kPendNone, KIND>), grid, dim3(kDecThreads), 0, stream, p);
+  } else if constexpr (KIND > kShapeOn) {
+    launch_shaped_split<T, KIND - 2>(p, grid, kind, stream);   // (kShapeOn is in all of them)
   }
 }
 }  // namespace

@@ -206,13 +206,10 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
     const uint32_t k_end = min(pos + 1, a_end * kUnitKeys);
     const uint32_t kvh = pl / p.head_groups, hgrp = pl % p.head_groups;
     const uint32_t heads_here = min((uint32_t)kMaxHeadsPerGroup, p.group - hgrp * kMaxHeadsPerGroup);
-    size_t plane = seq_plane_offset(p.seq_offsets, p.kv_stride_seq, seq) + kvh * p.kv_stride_head;
+    const size_t plane = seq_plane_offset(p.seq_offsets, p.kv_stride_seq, seq) + kvh * p.kv_stride_head;
     const uint32_t head0 = kvh * p.group + hgrp * kMaxHeadsPerGroup;
     KeyRange range{0u, pos + 1, (int32_t)pos};
-    if constexpr (SHAPE != kShapeNone) {
-      range = key_range_of<SHAPE>(p, seq);
-      plane += (size_t)range.first * p.kv_stride_pos;
-    }
+    if constexpr (SHAPE != kShapeNone) range = key_range_of<SHAPE>(p, seq);
     const auto score = score_of<SHAPE>(p, head0 + min((uint32_t)t.c, heads_here - 1), range);
     const uint32_t row0 = seq * p.n_q_heads + head0;
     u32x4 qreg[4];
@@ -227,7 +224,7 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
                                                const_cast<uint16_t*>(p.v) + plane + (size_t)pos * p.kv_stride_pos,
                                                k_end == pos + 1, hgrp == 0);
       if constexpr (PENDING == kPendRows) load_queries(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
-      stream_keys<T, PENDING>(p.k + plane, p.v + plane, p.kv_stride_pos, k_begin, k_end, pos, qreg, smem, t,
+      stream_keys<T, PENDING>(planes_of<SHAPE>(p, plane, kvh, range), k_begin, k_end, pos, qreg, smem, t,
                               w * 7u + pl * 3u + seq * 5u, score, m_run, l_run, acc, &fresh,
                               PENDING == kPendSums ? &queries : nullptr, heads_here);
       if constexpr (PENDING == kPendSums) {
@@ -235,12 +232,12 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
       }
     } else {
       load_queries(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
-      stream_keys<T>(p.k + plane, p.v + plane, p.kv_stride_pos, k_begin, k_end, pos, qreg, smem, t,
+      stream_keys<T>(planes_of<SHAPE>(p, plane, kvh, range), k_begin, k_end, pos, qreg, smem, t,
                      w * 7u + pl * 3u + seq * 5u, score, m_run, l_run, acc);
     }
 
     auto final_row = [&](uint32_t h, uint32_t dq, const f32x4& av, float l, float m) {
-      emit_final<T>(p.out, p.lse, (size_t)(row0 + h), dq, av, l, m);
+      emit_joined<T, SHAPE>(p, (size_t)(row0 + h), dq, av, l, m);
     };
     merge_waves(smem, t, heads_here, m_run, l_run, acc,
                 [&](uint32_t h, uint32_t dq, const f32x4& av, float l, float m) {
@@ -291,21 +288,13 @@ bool decode_balanced_takes(const DecodeWorkspace& w, uint32_t batch, uint32_t n_
 }
 
 namespace {
-template <typename T>
-void launch_shaped_balanced(const DecodeKernelArgs& p, dim3 grid, int shape, hipStream_t stream) {
-  const dim3 block(kDecThreads);
-  switch (shape) {
-    case kShapeOn:
-      hipLaunchKernelGGL((decode_balanced_kernel<T, kPendNone, kShapeOn>), grid, block, 0, stream, p);
-      break;
-    case kShapeOn | kShapeCap:
-      hipLaunchKernelGGL((decode_balanced_kernel<T, kPendNone, kShapeOn | kShapeCap>), grid, block, 0, stream, p);
-      break;
-    case kShapeOn | kShapeSlopes:
-      hipLaunchKernelGGL((decode_balanced_kernel<T, kPendNone, kShapeOn | kShapeSlopes>), grid, block, 0, stream, p);
-      break;
-    default:
-      hipLaunchKernelGGL((decode_balanced_kernel<T, kPendNone, kShapeOn | kShapeCap | kShapeSlopes>), grid, block, 0, stream, p);
+// the kernel for the shape `kind`, found among KIND and those below it
+template <typename T, int KIND = kShapeOn | kShapeCap | kShapeSlopes>
+void launch_shaped_balanced(const DecodeKernelArgs& p, dim3 grid, int kind, hipStream_t stream) {
+  if (kind == KIND) {
+    hipLaunchKernelGGL((decode_balanced_kernel<T, kPendNone, KIND>), grid, dim3(kDecThreads), 0, stream, p);
+  } else if constexpr (KIND > kShapeOn) {
+    launch_shaped_balanced<T, KIND - 2>(p, grid, kind, stream);   // (kShapeOn is in all of them)
   }
 }
 }  // namespace

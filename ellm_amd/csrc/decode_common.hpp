@@ -30,12 +30,23 @@ static_assert(kDecWaves * kMaxHeadsPerGroup * kRedPitch * 4 <= kDecWaves * kWave
 // Shaped scores in the single-token kernels (template argument SHAPE): none, or on, with a cap, with slopes.  A sequence's
 // key range is taken as a plane of its own that begins at the range's first row, so nothing but the scores changes.
 constexpr int kShapeNone = 0, kShapeOn = 1, kShapeCap = 2, kShapeSlopes = 4;
+// ... over the shared prefix and the sequence's own rows as one plane (few keys: nothing is gained by sharing)
+constexpr int kShapeWalk = 8;
 struct ShapeArgs {
   const float* slopes;
   const uint32_t* key_begin;   // per position, as in ShapedState
   const uint32_t* key_end;
   size_t bounds_pitch;
-  uint32_t window, prefix, capacity;
+  uint32_t window, capacity;
+  // the shared prefix's partial results, `prefix_parts` a row (0: none), to join to the sequence's own
+  uint32_t prefix_parts;
+  const float* prefix_o;
+  const float* prefix_ml;
+  // kShapeWalk: the prefix itself
+  uint32_t prefix;
+  const uint16_t* prefix_k;
+  const uint16_t* prefix_v;
+  size_t prefix_stride_head, prefix_stride_pos;
   ShapedScores f;
 };
 
@@ -65,8 +76,8 @@ struct DecodeKernelArgs {
   ShapeArgs shape;    // kernels built with SHAPE
 };
 
-// What a sequence's query sees: `len` of the sequence's own rows from row `first` on (none: 0), itself at row `pos` counted
-// from `first` (below it where later keys are visible, or at it).
+// What a sequence's query sees: `len` rows from row `first` on (none: 0) of the sequence's own, or with kShapeWalk of the
+// prefix's and its own, itself at row `pos` counted from `first` (below it where later keys are visible, or at it).
 struct KeyRange {
   uint32_t first, len;
   int32_t pos;
@@ -77,7 +88,8 @@ __device__ __forceinline__ KeyRange key_range_of(const DecodeKernelArgs& p, uint
   if (p.positions) pos = min(p.positions[seq], p.position);
   if (p.seq_caps) pos = min(pos, p.seq_caps[seq] - 1);
   if constexpr (SHAPE == kShapeNone) return KeyRange{0u, pos + 1, (int32_t)pos};
-  uint32_t lo = 0, hi = pos + 1;
+  if constexpr ((SHAPE & kShapeWalk) != 0) pos += p.shape.prefix;
+  uint32_t lo = 0, hi = pos + 1;   // (own rows alone: a window that reaches into the prefix leaves all of them)
   if (p.shape.key_begin) lo = p.shape.key_begin[seq * p.shape.bounds_pitch + pos];
   if (p.shape.key_end) hi = min(p.shape.key_end[seq * p.shape.bounds_pitch + pos], p.seq_caps ? p.seq_caps[seq] : p.shape.capacity);
   if (p.shape.window && pos + 1 > p.shape.window) lo = max(lo, pos + 1 - p.shape.window);
@@ -91,10 +103,50 @@ inline int fill_shape(const ShapedState& s, const AttnArgs& a, ShapeArgs* shape)
   shape->key_end = s.key_end;
   shape->bounds_pitch = s.bounds_pitch;
   shape->window = s.window;
+  shape->prefix_parts = s.prefix_parts;
+  shape->prefix_o = s.part_o;
+  shape->prefix_ml = s.part_ml;
   shape->prefix = s.prefix;
+  shape->prefix_k = (const uint16_t*)s.prefix_k;
+  shape->prefix_v = (const uint16_t*)s.prefix_v;
+  shape->prefix_stride_head = s.prefix_stride_head;
+  shape->prefix_stride_pos = s.prefix_stride_pos;
   shape->capacity = a.capacity;
   shape->f = shaped_scores(s, a.scale);
-  return kShapeOn | (s.cap != 0.0f ? kShapeCap : 0) | (s.slopes ? kShapeSlopes : 0);
+  return kShapeOn | (s.cap != 0.0f ? kShapeCap : 0) | (s.slopes ? kShapeSlopes : 0) | (s.walk_prefix ? kShapeWalk : 0);
+}
+
+// Where the rows of a key range are: in one plane, or the first of them in the prefix's.
+struct OnePlane {
+  const uint16_t* kplane;
+  const uint16_t* vplane;
+  size_t stride_pos;
+  __device__ __forceinline__ const uint16_t* k(uint32_t row) const { return kplane + (size_t)row * stride_pos; }
+  __device__ __forceinline__ const uint16_t* v(uint32_t row) const { return vplane + (size_t)row * stride_pos; }
+};
+struct TwoPlanes {
+  OnePlane prefix, own;   // (own: from the sequence's row 0 on)
+  uint32_t first, n;      // the range's first row, rows of the prefix
+  __device__ __forceinline__ const uint16_t* k(uint32_t row) const {
+    const uint32_t r = first + row;
+    return r < n ? prefix.k(r) : own.k(r - n);
+  }
+  __device__ __forceinline__ const uint16_t* v(uint32_t row) const {
+    const uint32_t r = first + row;
+    return r < n ? prefix.v(r) : own.v(r - n);
+  }
+};
+// plane: element offset of the sequence's own rows
+template <int SHAPE>
+__device__ __forceinline__ auto planes_of(const DecodeKernelArgs& p, size_t plane, uint32_t kvh, const KeyRange& range) {
+  if constexpr ((SHAPE & kShapeWalk) != 0) {
+    const size_t at = kvh * p.shape.prefix_stride_head;
+    return TwoPlanes{{p.shape.prefix_k + at, p.shape.prefix_v + at, p.shape.prefix_stride_pos},
+                     {p.k + plane, p.v + plane, p.kv_stride_pos}, range.first, p.shape.prefix};
+  } else {
+    if constexpr (SHAPE != kShapeNone) plane += (size_t)range.first * p.kv_stride_pos;
+    return OnePlane{p.k + plane, p.v + plane, p.kv_stride_pos};
+  }
 }
 
 // A score from a product, in log2 units, by the key's row.
@@ -380,9 +432,8 @@ struct NewRowLoads<kPendNone> {
 // request (`queries` holds the requested raw query rows; qreg is filled here), so that both
 // trips to memory run side by side.  With kPendRows (a fused cache write) the new rows come as
 // stored 16-bit rows, the query rows are final (qreg filled by the caller, `queries` null).
-template <typename T, int PENDING = kPendNone, typename Score>
-__device__ __forceinline__ void stream_keys(const uint16_t* kplane, const uint16_t* vplane, size_t stride_pos,
-                                            uint32_t k_begin, uint32_t k_end, uint32_t pos,
+template <typename T, int PENDING = kPendNone, typename Planes, typename Score>
+__device__ __forceinline__ void stream_keys(const Planes& planes, uint32_t k_begin, uint32_t k_end, uint32_t pos,
                                             u32x4 (&qreg)[4], uint16_t* smem, const Lane& t,
                                             uint32_t rot_seed, const Score& score, float& m_out, float& l_out,
                                             f32x4 (&acc)[8], const NewRow* fresh = nullptr,
@@ -411,8 +462,8 @@ __device__ __forceinline__ void stream_keys(const uint16_t* kplane, const uint16
       // rows past the last valid key are clamped onto it: always in bounds,
       // always initialised, and their probabilities are forced to zero below.
       const uint32_t row = min(kb + 4 * g + i, pos);
-      kreg[i] = stream_load16(kplane + (size_t)row * stride_pos + 8 * c);
-      vreg[i] = stream_load16(vplane + (size_t)row * stride_pos + 8 * c);
+      kreg[i] = stream_load16(planes.k(row) + 8 * c);
+      vreg[i] = stream_load16(planes.v(row) + 8 * c);
     }
   };
 
@@ -574,6 +625,25 @@ __device__ __forceinline__ void emit_final(uint16_t* out, float* lse, size_t row
   w[1] = Mfma<T>::pack2(a[2] * inv, a[3] * inv);
   *(u32x2*)(out + row * kHeadDim + 4 * dq) = w;
   if (lse && dq == 0) lse[row] = (m + fast_log2(l)) * kLn2;
+}
+
+// The same behind a shared prefix: the row's partial results over the prefix are joined first.
+template <typename T, int SHAPE>
+__device__ __forceinline__ void emit_joined(const DecodeKernelArgs& p, size_t row, uint32_t dq, const f32x4& a, float l, float m) {
+  if constexpr (SHAPE != kShapeNone) {
+    const uint32_t parts = p.shape.prefix_parts;
+    if (parts) {   // (uniform)
+      float lp;
+      f32x4 o;
+      const float mp = fold_splits<1, 8>(p.shape.prefix_ml + row * parts * 2, p.shape.prefix_o + row * parts * kHeadDim + 4 * dq,
+                                         kHeadDim, 0, parts, parts, lp, o);
+      const float both = fmaxf(m, mp);
+      const float w = m == -INFINITY ? 0.0f : fast_exp2(m - both), wp = mp == -INFINITY ? 0.0f : fast_exp2(mp - both);
+      emit_final<T>(p.out, p.lse, row, dq, w * a + wp * o, w * l + wp * lp, both);
+      return;
+    }
+  }
+  emit_final<T>(p.out, p.lse, row, dq, a, l, m);
 }
 
 // Output rows of a group whose sequence sees no key: 0, log-sum-exp -infinity.

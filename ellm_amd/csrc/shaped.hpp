@@ -32,6 +32,9 @@ struct ShapedState {
   float* part_o;               // partial rows [part_rows][128] and [part_rows][2], from the first set call to destroy
   float* part_ml;
   size_t part_rows;
+  // what a launch over the sequences' own rows joins to them: the prefix's partial results (0: none)
+  uint32_t prefix_parts;
+  bool walk_prefix;   // or it walks the prefix itself, ahead of every sequence's own rows
   bool scores() const { return cap != 0.0f || slopes || window || key_begin || key_end; }
   bool active() const { return scores() || prefix; }
 };
@@ -60,5 +63,7 @@ struct ShapedArgs {
 };
 
 hipError_t launch_shaped(const ShapedArgs& args, hipStream_t stream);
+// Single tokens: the shared prefix alone, left as *parts partial results a row (0: no room for them, nothing launched).
+hipError_t launch_shaped_prefix(const ShapedArgs& args, uint32_t* parts, hipStream_t stream);
 
 }  // namespace ellm

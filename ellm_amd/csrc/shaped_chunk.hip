@@ -21,7 +21,8 @@
 // that move only where a sum asks for it 8 %, addresses and descriptors in scalar registers that move on 5 %, priority 2 to
 // 9 %, walks from the last step where scores fall with the distance 24 % of those.  Tried and dropped: eight waves of two
 // groups half a step apart (256 rows; 5 % faster on long plain walks, 5 to 10 % slower on short ones), 64 rows a wave (scores land
-// in accumulation registers: twice the time), operands read 3, 6 or 8 ahead (the same).
+// in accumulation registers: twice the time), operands read 3, 6 or 8 ahead (the same), three steps on their way instead of
+// one where a workgroup has a unit to itself (1 to 8 % slower: the chain of a step, 1.7 us, bounds it, no trip to memory).
 #include <type_traits>
 
 #include "common.hpp"
@@ -32,9 +33,9 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
+constexpr int kBuffers = 2;   // tiles of K, and of V, in LDS
 constexpr int kRows = (int)kShapedRows;
 static_assert(kRows == 32 * kWaves, "32 rows a wave");
-constexpr int kBuffers = 2;   // tiles of K, and of V, in LDS
 constexpr int kAhead = 4;     // LDS operand reads in flight ahead of their products
 constexpr int kKeys = (int)kShapedKeys;
 constexpr int kTileBytes = kKeys * kHeadDim * 2;
@@ -42,6 +43,8 @@ constexpr uint32_t kNoKey = 0xffffffffu;
 
 typedef __attribute__((address_space(3))) uint16_t LdsHalf;
 typedef __attribute__((address_space(3))) u32x4 LdsU32x4;
+typedef __attribute__((address_space(3))) u32x2 LdsU32x2;
+typedef __attribute__((address_space(3))) f32x4 LdsF32x4;
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4 LdsI16x4;
 constexpr int kBufferFlags = 0x00020000;  // raw buffer of 32-bit data, no swizzle (word 3 of the descriptor)
@@ -68,13 +71,20 @@ struct ShapedKernelArgs {
   size_t prefix_stride_head, prefix_stride_pos;
   uint32_t batch, batch_pitch, n_q_heads, n_kv_heads, group;
   uint32_t interval, position, capacity, prefix, window;
-  uint32_t rows_plane, tiles_plane, n_split, planes, own_wgs;
+  uint32_t rows_plane, tiles_plane, n_split, own_wgs;
   uint32_t prefix_rows, prefix_tiles, prefix_split;
   uint32_t n_part;
+  uint32_t whole;   // rows are finished here (one partial result, and nothing to join it to)
+  Divisor by_planes, by_kv_heads, by_split, by_prefix_split, by_rows_plane, by_group;
   float c_in;     // with a cap: 2 scale log2(e) / cap
   float a0, a1;   // y = a0 + a1 s (shaped.hpp)
 };
 
+// The own row of a query: its sequence's position, `token` further on.
+__device__ __forceinline__ uint32_t own_row(const ShapedKernelArgs& p, uint32_t seq, uint32_t token) {
+  const uint32_t first = p.positions ? min(p.positions[seq], p.position) : p.position;
+  return min(first + token, (p.seq_caps ? p.seq_caps[seq] : p.capacity) - 1);
+}
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 __device__ __forceinline__ uint64_t uniform64(uint64_t x) {
   return ((uint64_t)uniform((uint32_t)(x >> 32)) << 32) | (uint64_t)uniform((uint32_t)x);
@@ -131,7 +141,7 @@ __device__ __forceinline__ u32x4 odd_values(u32x4 a, uint32_t but) {
 
 template <typename T, bool CAP, bool SLOPES>
 __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelArgs p) {
-  // K tiles [2][64][128] then V tiles [2][64][128]; of the sixteen 16-byte pieces of a row, piece x of K row r sits at
+  // K tiles [kBuffers][64][128] then V tiles [kBuffers][64][128]; of the sixteen 16-byte pieces of a row, piece x of K row r sits at
   // x ^ (r & 15), of V row r at x ^ 4 (r & 3): the lanes that a read serves at once (16 rows of a piece, 4 rows of 64
   // bytes) meet no bank twice
   __shared__ __attribute__((aligned(256))) uint16_t smem[2 * kBuffers * kKeys * kHeadDim];
@@ -144,21 +154,20 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
   // ---- which rows, which part of the keys -------------------------------------------------------
   const bool on_prefix = blockIdx.x >= p.own_wgs;   // packed rows of all sequences against the prefix alone
   uint32_t id = on_prefix ? blockIdx.x - p.own_wgs : blockIdx.x;
-  uint32_t seq0 = 0, kvh, split, n_split, tile;
+  uint32_t seq0 = 0, kvh, split, tile;
   if (on_prefix) {
-    kvh = id % p.n_kv_heads;
-    id /= p.n_kv_heads;
-    n_split = p.prefix_split;
-    split = id % n_split;
-    tile = id / n_split;
+    uint32_t rest = p.by_kv_heads.quotient(id);
+    kvh = p.by_kv_heads.rest(id, rest);
+    tile = p.by_prefix_split.quotient(rest);
+    split = p.by_prefix_split.rest(rest, tile);
   } else {   // planes fastest: those that share an XCD's cache stay on it; the longest walks of causal prompts first
-    const uint32_t plane = id % p.planes;
-    id /= p.planes;
-    seq0 = plane / p.n_kv_heads;
-    kvh = plane % p.n_kv_heads;
-    n_split = p.n_split;
-    split = id % n_split;
-    tile = p.tiles_plane - 1 - id / n_split;
+    uint32_t rest = p.by_planes.quotient(id);
+    const uint32_t plane = p.by_planes.rest(id, rest);
+    seq0 = p.by_kv_heads.quotient(plane);
+    kvh = p.by_kv_heads.rest(plane, seq0);
+    tile = p.by_split.quotient(rest);
+    split = p.by_split.rest(rest, tile);
+    tile = p.tiles_plane - 1 - tile;
   }
   const uint32_t n_rows = on_prefix ? p.prefix_rows : p.rows_plane;
   struct Row {   // this lane's query row: where it is, what it sees
@@ -167,79 +176,99 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
     uint32_t lo, hi;   // (rows that are not stored see everything: they never ask for a mask)
   };
   Row row;
-  uint32_t wlo = kNoKey, whi = 0;              // the keys that any row of the wave sees
-  uint32_t all_lo = 0, all_hi = kNoKey;        // the keys that every row of the wave sees
+  const uint32_t wave_row = tile * kRows + 32 * wave;
   {
-    const uint32_t at_row = tile * kRows + 32 * wave + j, r = min(at_row, n_rows - 1);
+    const uint32_t at_row = wave_row + j, r = min(at_row, n_rows - 1);
     row.valid = at_row < n_rows;
-    row.seq = on_prefix ? r / p.rows_plane : seq0;
-    const uint32_t in_plane = on_prefix ? r % p.rows_plane : r;
-    row.token = in_plane / p.group;
-    row.head = kvh * p.group + in_plane % p.group;
-    uint32_t own = p.position;   // the query's own row
-    if (p.positions) own = min(p.positions[row.seq], own);
-    const uint32_t cap_seq = p.seq_caps ? p.seq_caps[row.seq] : p.capacity;
-    own = min(own + row.token, cap_seq - 1);
+    const uint32_t packed = on_prefix ? p.by_rows_plane.quotient(r) : 0u, in_plane = p.by_rows_plane.rest(r, packed);
+    row.seq = seq0 + packed;
+    row.token = p.by_group.quotient(in_plane);
+    row.head = kvh * p.group + p.by_group.rest(in_plane, row.token);
+  }
+  u32x4 qreg[8];
+  {
+    const uint16_t* qrow = p.q + row.token * p.q_token_stride + ((size_t)row.seq * p.n_q_heads + row.head) * kHeadDim;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) qreg[s] = load16(qrow + 16 * s + 8 * g);
+  }
+  const float slope2 = SLOPES ? p.slopes[row.head] * kLog2e : 0.0f;
+
+  // ---- the keys that rows see, the steps from the first to the last of them, this split's share of those ---------------
+  struct Reach {
+    uint32_t lo, hi;           // the keys that any row sees (lo >= hi: none)
+    uint32_t all_lo, all_hi;   // the keys that every row sees
+  };
+  Reach mine, all;   // the wave's, the workgroup's
+  // this workgroup's part of what the query at `pos` sees: all, the prefix, or the sequence's own rows
+  auto first_seen = [&](uint32_t pos) {
+    const uint32_t lo = p.window && pos + 1 > p.window ? pos + 1 - p.window : 0u;
+    return !on_prefix && p.prefix_tiles ? max(lo, p.prefix) : lo;
+  };
+  auto end_seen = [&](uint32_t pos) { return on_prefix ? min(pos + 1, p.prefix) : pos + 1; };
+  if (uniform(!p.key_begin && !p.key_end && (on_prefix ? p.window == 0 : p.positions == nullptr))) {
+    // ranges that move on with the rows: those of the first and the last row are all there is to know
+    row.pos = p.prefix + p.position + row.token;
+    if (SLOPES && p.positions) row.pos = p.prefix + own_row(p, row.seq, row.token);
+    row.lo = on_prefix || !row.valid ? 0u : first_seen(row.pos);
+    row.hi = !row.valid ? kNoKey : on_prefix ? p.prefix : end_seen(row.pos);
+    auto reach = [&](uint32_t first, uint32_t last) {   // of rows first .. last
+      if (first >= n_rows) return Reach{kNoKey, 0u, 0u, kNoKey};
+      if (on_prefix) return Reach{0u, p.prefix, 0u, p.prefix};
+      const uint32_t base = p.prefix + p.position, a = base + p.by_group.quotient(first),
+                     b = base + p.by_group.quotient(min(last, n_rows - 1));
+      return Reach{first_seen(a), end_seen(b), first_seen(b), end_seen(a)};
+    };
+    mine = reach(wave_row, wave_row + 31);
+    all = reach(tile * kRows, tile * kRows + kRows - 1);
+    if (tid < kBuffers) s_odd[tid] = 0;   // (behind the walk's first barrier)
+  } else {
+    const uint32_t own = own_row(p, row.seq, row.token);
     row.pos = p.prefix + own;
-    uint32_t lo = 0, hi = row.pos + 1;
-    if (p.key_begin) lo = p.key_begin[row.seq * p.bounds_pitch + own];
-    if (p.key_end) hi = min(p.key_end[row.seq * p.bounds_pitch + own], cap_seq);
-    if (p.window && row.pos + 1 > p.window) lo = max(lo, row.pos + 1 - p.window);
-    // this workgroup's part of the keys: all, the prefix, or the sequence's own rows
-    if (on_prefix) hi = min(hi, p.prefix);
-    if (!on_prefix && p.prefix_tiles) lo = max(lo, p.prefix);
+    uint32_t lo = first_seen(row.pos), hi = end_seen(row.pos);
+    if (p.key_begin) lo = max(lo, p.key_begin[row.seq * p.bounds_pitch + own]);
+    if (p.key_end) hi = min(p.key_end[row.seq * p.bounds_pitch + own], p.seq_caps ? p.seq_caps[row.seq] : p.capacity);
     if (lo >= hi) lo = hi = 0;   // sees nothing
-    if (row.valid && lo < hi) {
-      wlo = min(wlo, lo);
-      whi = max(whi, hi);
-    }
     row.lo = row.valid ? lo : 0u;
     row.hi = row.valid ? hi : kNoKey;
-    all_lo = max(all_lo, row.lo);
-    all_hi = min(all_hi, row.hi);
-  }
-
-  // ---- the steps from the first to the last key that any row sees, this split's share of them -----
+    const bool live = row.valid && lo < hi;
+    mine = Reach{live ? lo : kNoKey, live ? hi : 0u, row.lo, row.hi};
 #pragma unroll
-  for (int x = 1; x < 32; x <<= 1) {
-    wlo = min(wlo, (uint32_t)__shfl_xor((int)wlo, x));
-    whi = max(whi, (uint32_t)__shfl_xor((int)whi, x));
-    all_lo = max(all_lo, (uint32_t)__shfl_xor((int)all_lo, x));
-    all_hi = min(all_hi, (uint32_t)__shfl_xor((int)all_hi, x));
-  }
-  if (lane == 0) {
-    s_lo[wave] = wlo;
-    s_hi[wave] = whi;
-    s_all_lo[wave] = all_lo;
-    s_all_hi[wave] = all_hi;
-  }
-  if (tid < kBuffers) s_odd[tid] = 0;
-  __syncthreads();
-  // over the workgroup: the keys that any row sees, those that every row sees
-  uint32_t hull_lo = kNoKey, hull_hi = 0, wg_lo = 0, wg_hi = kNoKey;
+    for (int x = 1; x < 32; x <<= 1) {
+      mine.lo = min(mine.lo, (uint32_t)__shfl_xor((int)mine.lo, x));
+      mine.hi = max(mine.hi, (uint32_t)__shfl_xor((int)mine.hi, x));
+      mine.all_lo = max(mine.all_lo, (uint32_t)__shfl_xor((int)mine.all_lo, x));
+      mine.all_hi = min(mine.all_hi, (uint32_t)__shfl_xor((int)mine.all_hi, x));
+    }
+    if (lane == 0) {
+      s_lo[wave] = mine.lo;
+      s_hi[wave] = mine.hi;
+      s_all_lo[wave] = mine.all_lo;
+      s_all_hi[wave] = mine.all_hi;
+    }
+    if (tid < kBuffers) s_odd[tid] = 0;
+    __syncthreads();
+    all = Reach{kNoKey, 0u, 0u, kNoKey};
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    hull_lo = min(hull_lo, uniform(s_lo[w]));
-    hull_hi = max(hull_hi, uniform(s_hi[w]));
-    wg_lo = max(wg_lo, uniform(s_all_lo[w]));
-    wg_hi = min(wg_hi, uniform(s_all_hi[w]));
+    for (int w = 0; w < kWaves; ++w) {
+      all.lo = min(all.lo, s_lo[w]);
+      all.hi = max(all.hi, s_hi[w]);
+      all.all_lo = max(all.all_lo, s_all_lo[w]);
+      all.all_hi = min(all.all_hi, s_all_hi[w]);
+    }
   }
-  wlo = uniform(wlo);
-  whi = uniform(whi);
-  all_lo = uniform(all_lo);
-  all_hi = uniform(all_hi);
-  hull_lo = uniform(hull_lo);
-  hull_hi = uniform(hull_hi);
-  wg_lo = uniform(wg_lo);
-  wg_hi = uniform(wg_hi);
+  const uint32_t wlo = uniform(mine.lo), whi = uniform(mine.hi), all_lo = uniform(mine.all_lo), all_hi = uniform(mine.all_hi);
+  const uint32_t hull_lo = uniform(all.lo), hull_hi = uniform(all.hi), wg_lo = uniform(all.all_lo), wg_hi = uniform(all.all_hi);
   const uint32_t prefix_steps = (p.prefix + kKeys - 1) / kKeys;
   auto step_of = [&](uint32_t key) { return key < p.prefix ? key / kKeys : prefix_steps + (key - p.prefix) / kKeys; };
   uint32_t step = 0, end = 0;
   if (hull_lo < hull_hi) {
     const uint32_t first = step_of(hull_lo), n = step_of(hull_hi - 1) + 1 - first;
-    step = first + (uint32_t)((uint64_t)n * split / n_split);
-    end = first + (uint32_t)((uint64_t)n * (split + 1) / n_split);
+    const Divisor& by = on_prefix ? p.by_prefix_split : p.by_split;
+    step = first + shaped_share(n, split, by);
+    end = first + shaped_share(n, split + 1, by);
   }
+  step = uniform(step);
+  end = uniform(end);
   // Scores that fall with the distance are walked from the last step to the first: their references are then found in
   // the first step instead of moving in every one.  Step s of the walk is step place(s) of the keys.
   const uint32_t mirror = step + end - 1;
@@ -261,14 +290,6 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
   }
   w_begin = uniform(w_begin);
   w_end = uniform(w_end);
-
-  u32x4 qreg[8];
-  {
-    const uint16_t* qrow = p.q + row.token * p.q_token_stride + ((size_t)row.seq * p.n_q_heads + row.head) * kHeadDim;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) qreg[s] = load16(qrow + 16 * s + 8 * g);
-  }
-  const float slope2 = SLOPES ? p.slopes[row.head] * kLog2e : 0.0f;
 
   // ---- staging ------------------------------------------------------------------------------------
   const size_t plane_at = seq_plane_offset(p.seq_offsets, p.kv_stride_seq, seq0) + kvh * p.kv_stride_head;
@@ -339,6 +360,7 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
   Source ksrc = source(p.k, p.prefix_k, step), vsrc = source(p.v, p.prefix_v, step);
 
   aim(step);
+
   // ---- walk ---------------------------------------------------------------------------------------
   // minus the row's reference (log2 units; +inf: no key seen yet; rows that will see none need none), this lane's share of its sum
   float neg_m = row.lo < row.hi ? INFINITY : 0.0f, l_run = 0.0f;
@@ -499,27 +521,34 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
   };
   auto meet = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
-  // Turn s multiplies K of step s + 1 and V of step s and sends for K of step s + 2 and V of step s + 1: P.V of a step runs
-  // beside the weights of the next, whose vector instructions so find their place between the wave's own matrix
-  // instructions.  Buffers and weights swap from turn to turn; the first turn has no V, the last no K.
-  auto turn = [&](auto kbuf, auto vbuf, u32x4 (&pk)[4], u32x4 (&next)[4], uint32_t s) __attribute__((always_inline)) {
-    // this wave's loads have arrived and its reads of the other buffers are done; behind the barrier so have all
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  // K of the walk's step i and V of the one before it on their way, into buffers i and i - 1 modulo kBuffers
+  const uint32_t n_steps = end - step;
+  auto send_pair = [&](uint32_t i) __attribute__((always_inline)) {
     // (V goes one step behind K: it is sent for first where K is to leave a part)
-    if (s + 1 < end) {
-      if (s + 1 == other_part) vsrc = source(p.v, p.prefix_v, other_part);
-      send(vsrc, off_v, kBuffers + 1 - vbuf);
+    if (i && i <= n_steps) {
+      if (step + i - 1 == other_part) vsrc = source(p.v, p.prefix_v, other_part);
+      send(vsrc, off_v, kBuffers + (i - 1) % kBuffers);
     }
-    if (s + 2 < end) {
-      if (s + 2 == other_part) {
+    if (i < n_steps) {
+      if (step + i == other_part) {
         aim(other_part);
         ksrc = source(p.k, p.prefix_k, other_part);
       }
-      send(ksrc, off_k, 1 - kbuf);
+      send(ksrc, off_k, i % kBuffers);
     }
+  };
+  // Turn t multiplies K of step t and V of step t - 1 (s + 1 and s, counted over the keys): P.V of a step runs beside the
+  // weights of the next, whose vector instructions so find their place between the wave's own matrix instructions.
+  // Weights swap registers from turn to turn; the first turn has no V, the last no K.
+  auto turn = [&](u32x4 (&pk)[4], u32x4 (&next)[4], uint32_t t) __attribute__((always_inline)) {
+    const uint32_t s = step + t - 1;
+    // this wave's loads have arrived and its reads of the buffers to be filled are done; behind the barrier so have all
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    send_pair(t + 1);
+    const uint32_t kbuf = t % kBuffers, vbuf = (t + 1) % kBuffers;
     const bool has_k = uniform(s + 1 >= w_begin && s + 1 < w_end) != 0, has_v = uniform(s + 1 > w_begin && s < w_end) != 0;
     const uint32_t vs = opaque(v_read + vbuf * kTileBytes);
-    const bool look = s + 1 != step && partly(wg_lo, wg_hi, s);   // (the first turn has no V; the same for all waves)
+    const bool look = t && partly(wg_lo, wg_hi, s);   // (the first turn has no V; the same for all waves)
     if (look) find_odd(vbuf);
     // Weights against the reference that each row already has: while no lane's sum of them passes kMaxSum the step's
     // maximum is not looked for.  A row without a reference (neg_m = +inf) makes its sums infinite or NaN and so asks for
@@ -562,27 +591,27 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
     if (!has_k) return;
     settle(st, next, sum);
   };
-  constexpr std::integral_constant<uint32_t, 0> kZero;
-  constexpr std::integral_constant<uint32_t, 1> kOne;
-  if (step < end) {
+  if (n_steps) {
     u32x4 even[4], odd[4];
-    send(ksrc, off_k, 0);
-    uint32_t s = step - 1;   // (step 0: one below zero, whose successor is 0 again)
-    for (;;) {
-      turn(kZero, kOne, odd, even, s);
-      if (++s == end) break;
-      turn(kOne, kZero, even, odd, s);
-      if (++s == end) break;
+    send_pair(0);
+    for (uint32_t t = 0;;) {
+      turn(odd, even, t);
+      if (t++ == n_steps) break;
+      turn(even, odd, t);
+      if (t++ == n_steps) break;
     }
   }
 
   // ---- results ------------------------------------------------------------------------------------
+  // A lane holds pieces of 4 dims of its row, 16 bytes of a row an instruction: rows go through LDS (each wave its own
+  // quarter, pieces permuted by the row so that no bank is met twice) and leave in whole lines.
   const float l = sum_with_partner_half(l_run);
   const float m = l == 0.0f ? -INFINITY : -neg_m;
-  if (!row.valid) return;
-  if (p.n_part == 1) {
+  meet();   // (the others' last reads of the tiles)
+  const uint32_t mine_lds = lds0 + (uint32_t)wave * (32 * kHeadDim * 4);
+  const size_t at = (size_t)row.token * p.batch_pitch + row.seq;
+  if (p.whole) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // (a row that sees no key is 0)
-    uint16_t* orow = p.out + row.token * p.q_token_stride + ((size_t)row.seq * p.n_q_heads + row.head) * kHeadDim;
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -590,20 +619,34 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
         u32x2 w;
         w[0] = Mfma<T>::pack2(oacc[db][4 * b] * inv, oacc[db][4 * b + 1] * inv);
         w[1] = Mfma<T>::pack2(oacc[db][4 * b + 2] * inv, oacc[db][4 * b + 3] * inv);
-        *(u32x2*)(orow + 32 * db + 8 * b + 4 * g) = w;
+        *(LdsU32x2*)(mine_lds + j * kHeadDim * 2 + 16 * ((4 * db + b) ^ (j & 15)) + 8 * g) = w;
       }
-    if (p.lse && g == 0)
-      p.lse[((size_t)row.token * p.batch_pitch + row.seq) * p.n_q_heads + row.head] = (m + fast_log2(l)) * kLn2;
+    if (p.lse && g == 0 && row.valid) p.lse[at * p.n_q_heads + row.head] = (m + fast_log2(l)) * kLn2;
+    const uint32_t to = (uint32_t)((at * p.n_q_heads + row.head));   // (below 2^31: rows of the whole call)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 4);
+      const u32x4 x = *(const LdsU32x4*)(mine_lds + r * kHeadDim * 2 + 16 * ((lane & 15) ^ (r & 15)));
+      const size_t to_r = (uint32_t)__shfl((int)to, r);
+      if (wave_row + r < n_rows) store16(p.out + to_r * kHeadDim + 8 * (lane & 15), x);
+    }
     return;
   }
-  const size_t part = (((size_t)row.token * p.batch + row.seq) * p.n_q_heads + row.head) * p.n_part + split + (on_prefix ? p.n_split : 0);
-  float* prow = p.part_o + part * kHeadDim;
+  const uint32_t part = ((row.token * p.batch + row.seq) * p.n_q_heads + row.head) * p.n_part + split + (on_prefix ? p.n_split : 0);
 #pragma unroll
   for (int db = 0; db < 4; ++db)
 #pragma unroll
     for (int b = 0; b < 4; ++b)
-      *(f32x4*)(prow + 32 * db + 8 * b + 4 * g) = f32x4{oacc[db][4 * b], oacc[db][4 * b + 1], oacc[db][4 * b + 2], oacc[db][4 * b + 3]};
-  if (g == 0) *(f32x2*)(p.part_ml + part * 2) = f32x2{m, l};
+      *(LdsF32x4*)(mine_lds + j * kHeadDim * 4 + 16 * ((8 * db + 2 * b + g) ^ j)) =
+          f32x4{oacc[db][4 * b], oacc[db][4 * b + 1], oacc[db][4 * b + 2], oacc[db][4 * b + 3]};
+  if (g == 0 && row.valid) *(f32x2*)(p.part_ml + (size_t)part * 2) = f32x2{m, l};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = 2 * i + g;
+    const f32x4 x = *(const LdsF32x4*)(mine_lds + r * kHeadDim * 4 + 16 * (j ^ r));
+    const size_t part_r = (uint32_t)__shfl((int)part, r);
+    if (wave_row + r < n_rows) *(f32x4*)(p.part_o + part_r * kHeadDim + 4 * j) = x;
+  }
 }
 
 // Joins the partial results of a row: G lanes share its four columns (fold_splits).
@@ -631,7 +674,7 @@ __global__ __launch_bounds__(256) void shaped_merge_kernel(ShapedKernelArgs p) {
 }
 
 template <typename T>
-hipError_t launch(const ShapedKernelArgs& p, bool cap, bool slopes, hipStream_t stream) {
+hipError_t launch(const ShapedKernelArgs& p, bool cap, bool slopes, bool merge, hipStream_t stream) {
   const dim3 grid(p.own_wgs + p.prefix_tiles * p.prefix_split * p.n_kv_heads), block(kThreads);
   if (cap && slopes)
     hipLaunchKernelGGL((shaped_tile_kernel<T, true, true>), grid, block, 0, stream, p);
@@ -642,7 +685,7 @@ hipError_t launch(const ShapedKernelArgs& p, bool cap, bool slopes, hipStream_t 
   else
     hipLaunchKernelGGL((shaped_tile_kernel<T, false, false>), grid, block, 0, stream, p);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.n_part == 1) return e;
+  if (e != hipSuccess || p.whole || !merge) return e;
   const size_t quads = (size_t)p.interval * p.batch * p.n_q_heads * (kHeadDim / 4);
   if (p.n_part > 8) {
     hipLaunchKernelGGL((shaped_merge_kernel<T, 8>), dim3((uint32_t)((quads * 8 + 255) / 256)), dim3(256), 0, stream, p);
@@ -654,24 +697,13 @@ hipError_t launch(const ShapedKernelArgs& p, bool cap, bool slopes, hipStream_t 
 
 }  // namespace
 
-hipError_t launch_shaped(const ShapedArgs& args, hipStream_t stream) {
+namespace {
+
+hipError_t launch_plan(const ShapedArgs& args, const ShapedPlan& plan, bool merge, hipStream_t stream) {
   const AttnArgs& a = args.a;
   const ShapedState& s = args.s;
-  // keys of a walk as far as the host knows them: the window bounds them, ranges of their own may shorten them
-  uint32_t own_keys = a.position_index + a.position_interval;
-  uint32_t prefix_keys = s.prefix;
-  if (s.window) {
-    const uint64_t reach = (uint64_t)s.window + a.position_interval;
-    if (reach < own_keys) {
-      own_keys = (uint32_t)reach;
-    } else if (!a.positions) {   // (own rows of sequences that are shorter than the bound on the host leave more to the prefix)
-      const uint64_t rest = reach - own_keys;
-      if (rest < prefix_keys) prefix_keys = (uint32_t)rest;
-    }
-  }
-  const ShapedPlan plan = shaped_plan(a.position_interval, a.batch, a.n_kv_heads, a.group, own_keys, prefix_keys, a.n_cu, s.part_rows);
-  // (sizes of a launch are 32-bit; 128-row tiles of that many rows would be a chunk of 2^31 (token, head) rows)
-  if ((uint64_t)a.position_interval * a.batch * a.n_q_heads > 0x7fffffffull) return hipErrorInvalidValue;
+  // (rows are counted in 32 bits: 2^31 of them would be 2^39 bytes of queries)
+  if ((uint64_t)a.position_interval * a.batch_pitch * a.n_q_heads > 0x7fffffffull) return hipErrorInvalidValue;
   ShapedKernelArgs p{};
   p.q = (const uint16_t*)a.q;
   p.k = (const uint16_t*)a.k;
@@ -708,18 +740,62 @@ hipError_t launch_shaped(const ShapedArgs& args, hipStream_t stream) {
   p.rows_plane = plan.rows_plane;
   p.tiles_plane = plan.tiles_plane;
   p.n_split = plan.n_split;
-  p.planes = a.batch * a.n_kv_heads;
-  p.own_wgs = p.planes * plan.tiles_plane * plan.n_split;
+  const uint32_t planes = a.batch * a.n_kv_heads;
+  p.own_wgs = planes * plan.tiles_plane * plan.n_split;
+  p.by_planes = divisor(planes);
+  p.by_kv_heads = divisor(a.n_kv_heads);
+  p.by_split = divisor(plan.n_split ? plan.n_split : 1);
+  p.by_prefix_split = divisor(plan.prefix_split ? plan.prefix_split : 1);
+  p.by_rows_plane = divisor(plan.rows_plane);
+  p.by_group = divisor(a.group);
   p.prefix_rows = plan.prefix_rows;
   p.prefix_tiles = plan.prefix_tiles;
   p.prefix_split = plan.prefix_split;
   p.n_part = plan.n_part;
+  p.whole = merge && plan.n_part == 1;
   const ShapedScores f = shaped_scores(s, a.scale);
   p.c_in = f.c_in;
   p.a0 = f.a0;
   p.a1 = f.a1;
-  return a.dtype == 0 ? launch<F16>(p, s.cap != 0.0f, s.slopes != nullptr, stream)
-                      : launch<BF16>(p, s.cap != 0.0f, s.slopes != nullptr, stream);
+  return a.dtype == 0 ? launch<F16>(p, s.cap != 0.0f, s.slopes != nullptr, merge, stream)
+                      : launch<BF16>(p, s.cap != 0.0f, s.slopes != nullptr, merge, stream);
+}
+
+}  // namespace
+
+hipError_t launch_shaped(const ShapedArgs& args, hipStream_t stream) {
+  const AttnArgs& a = args.a;
+  const ShapedState& s = args.s;
+  // keys of a walk as far as the host knows them: the window bounds them, ranges of their own may shorten them
+  uint32_t own_keys = a.position_index + a.position_interval;
+  uint32_t prefix_keys = s.prefix;
+  if (s.window) {
+    const uint64_t reach = (uint64_t)s.window + a.position_interval;
+    if (reach < own_keys) {
+      own_keys = (uint32_t)reach;
+    } else if (!a.positions) {   // (own rows of sequences that are shorter than the bound on the host leave more to the prefix)
+      const uint64_t rest = reach - own_keys;
+      if (rest < prefix_keys) prefix_keys = (uint32_t)rest;
+    }
+  }
+  const ShapedPlan plan = shaped_plan(a.position_interval, a.batch, a.n_kv_heads, a.group, own_keys, prefix_keys, a.n_cu, s.part_rows);
+  return launch_plan(args, plan, true, stream);
+}
+
+hipError_t launch_shaped_prefix(const ShapedArgs& args, uint32_t* parts, hipStream_t stream) {
+  const AttnArgs& a = args.a;
+  const ShapedState& s = args.s;
+  *parts = 0;
+  uint32_t seen = s.prefix;   // prefix rows that the window leaves, as far as the host knows
+  if (s.window && !a.positions) {
+    if (s.window <= a.position_index + 1) return hipSuccess;
+    const uint32_t rest = s.window - 1 - a.position_index;
+    seen = rest < seen ? rest : seen;
+  }
+  const ShapedPlan plan = shaped_prefix_plan(a.batch, a.n_kv_heads, a.group, seen, a.n_cu, s.part_rows);
+  if (plan.n_part == 0) return hipErrorInvalidValue;
+  *parts = plan.n_part;
+  return launch_plan(args, plan, false, stream);
 }
 
 }  // namespace ellm

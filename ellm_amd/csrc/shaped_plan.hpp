@@ -5,7 +5,28 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "decode_shares.hpp"
+
 namespace ellm {
+
+// Division by a number that the host knows, for dividends below 2^31: a product and a shift on the device, where a division is
+// some forty instructions.  With 2^(s-1) < d <= 2^s and m = floor(2^32 (2^s - d) / d) + 1 the quotient is
+// floor((floor(m n / 2^32) + n) / 2^s) (Granlund and Montgomery, Division by invariant integers using multiplication, 1994).
+struct Divisor {
+  uint32_t d, m, s;
+  ELLM_SHARES_FN uint32_t quotient(uint32_t n) const { return ((uint32_t)(((uint64_t)n * m) >> 32) + n) >> s; }
+  ELLM_SHARES_FN uint32_t rest(uint32_t n, uint32_t q) const { return n - q * d; }
+};
+inline Divisor divisor(uint32_t d) {
+  uint32_t s = 0;
+  while (((uint64_t)1 << s) < d) ++s;
+  return Divisor{d, (uint32_t)(((((uint64_t)1 << s) - d) << 32) / d + 1), s};
+}
+// Where split `split` of `n_split` begins in n steps (below 2^26; at most 2^12 splits): splits differ by a step at most.
+ELLM_SHARES_FN uint32_t shaped_share(uint32_t n, uint32_t split, const Divisor& n_split) {
+  const uint32_t whole = n_split.quotient(n);
+  return split * whole + n_split.quotient(split * n_split.rest(n, whole));
+}
 
 constexpr uint32_t kShapedRows = 128;   // query rows a workgroup of the tile kernel
 constexpr uint32_t kShapedKeys = 64;    // keys a step
@@ -21,13 +42,23 @@ struct ShapedPlan {
 
 inline uint32_t shaped_ceil(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
-// Splits of a walk of `steps` steps when `walks` of them are there for `slots` workgroups: as many as find a place,
-// none shorter than two steps.
-inline uint32_t shaped_split(uint32_t steps, uint64_t walks, uint32_t slots) {
+// Splits of a walk of `steps` steps when `walks` of them, `rows` query rows in all, are there for `slots` workgroups: as many
+// as find a place, none shorter than two steps, and no more than their partial results are worth.  A step is 1.7 us, a row's
+// partial result 1 KB of traffic, 0.3 ns: n splits cost 1.7 steps / n + 0.0003 rows n, least at sqrt(5700 steps / rows); the
+// launch that joins them adds some 4 us to the first split (241 tokens alone: 12.9 us whole, 16.9 in two).
+inline uint32_t shaped_split(uint32_t steps, uint64_t walks, uint32_t slots, uint64_t rows, bool joined_anyway) {
   uint32_t n = walks >= slots ? 1u : (uint32_t)(slots / walks);
   const uint32_t most = steps / 2 ? steps / 2 : 1;
-  return n < most ? n : most;
+  if (n > most) n = most;
+  while (n > 1 && (uint64_t)n * n * rows > 5700 * (uint64_t)steps) --n;
+  if (!joined_anyway && 1700 * (uint64_t)(steps - shaped_ceil(steps, n)) < 4000 + 3 * n * rows / 10) return 1;
+  return n;
 }
+
+// Places for workgroups of one kind: two a unit, or one where there are few steps for them, which halves the partial results
+// (33 tokens of 5 sequences on 777, 3 steps a unit: 21.3 -> 19.4 us; the prefix of 2 sequences, 4 K/V heads, 32000 keys, 8
+// steps a unit, ahead of the streaming kernels: 31.6 -> 26.2).
+inline uint32_t shaped_slots(uint64_t steps, uint32_t n_cu) { return steps <= 16 * (uint64_t)n_cu ? n_cu : 2 * n_cu; }
 
 // Rows of partial results a handle needs at most.
 inline size_t shaped_part_rows(size_t interval, size_t batch, size_t q_heads, uint32_t n_cu) {
@@ -41,7 +72,6 @@ inline size_t shaped_part_rows(size_t interval, size_t batch, size_t q_heads, ui
 inline ShapedPlan shaped_plan(uint32_t interval, uint32_t batch, uint32_t n_kv_heads, uint32_t group, uint32_t own_keys,
                               uint32_t prefix, uint32_t n_cu, size_t part_rows) {
   ShapedPlan p{};
-  const uint32_t slots = 2 * n_cu;
   p.rows_plane = interval * group;
   p.tiles_plane = shaped_ceil(p.rows_plane, kShapedRows);
   const uint64_t rows = (uint64_t)p.rows_plane * batch * n_kv_heads;
@@ -53,11 +83,14 @@ inline ShapedPlan shaped_plan(uint32_t interval, uint32_t batch, uint32_t n_kv_h
     p.prefix_rows = p.rows_plane * batch;
     p.prefix_tiles = shaped_ceil(p.prefix_rows, kShapedRows);
     const uint64_t prefix_walks = (uint64_t)p.prefix_tiles * n_kv_heads;
-    // places go to the two parts by their steps
+    // two places a unit go to the two parts by their steps (one place each for few steps makes the longer of the two wait: 24
+    // sequences, 8 K/V heads, behind 8000: 25.4 -> 49.6 us)
     const uint64_t total = prefix_walks * prefix_steps + walks * own_steps;
-    const uint32_t for_prefix = (uint32_t)(slots * (prefix_walks * prefix_steps) / total);
-    p.prefix_split = shaped_split(prefix_steps, prefix_walks, for_prefix ? for_prefix : 1);
-    p.n_split = shaped_split(own_steps, walks, slots > for_prefix ? slots - for_prefix : 1);
+    const uint32_t slots = 2 * n_cu;
+    uint32_t for_prefix = (uint32_t)(slots * (prefix_walks * prefix_steps) / total);
+    if (walks < slots && for_prefix > slots - walks) for_prefix = slots - (uint32_t)walks;   // (own walks take a place each)
+    p.prefix_split = shaped_split(prefix_steps, prefix_walks, for_prefix ? for_prefix : 1, rows, true);
+    p.n_split = shaped_split(own_steps, walks, slots > for_prefix ? slots - for_prefix : 1, rows, true);
     while (rows * (p.prefix_split + p.n_split) > part_rows && p.prefix_split + p.n_split > 2) {
       if (p.prefix_split >= p.n_split) --p.prefix_split; else --p.n_split;
     }
@@ -66,10 +99,46 @@ inline ShapedPlan shaped_plan(uint32_t interval, uint32_t batch, uint32_t n_kv_h
     p.prefix_rows = p.prefix_tiles = p.prefix_split = 0;
     p.n_split = 1;
   }
-  p.n_split = shaped_split(own_steps + prefix_steps, walks, slots);
+  p.n_split = shaped_split(own_steps + prefix_steps, walks, shaped_slots(walks * (own_steps + prefix_steps), n_cu), rows, false);
   if (rows * p.n_split > part_rows) p.n_split = (uint32_t)(part_rows / rows);
   if (p.n_split == 0) p.n_split = 1;
   p.n_part = p.n_split;
+  return p;
+}
+
+// How a single-token step behind a shared prefix runs.  Walk: every sequence streams the prefix and its own rows as one
+// plane (one launch; the prefix is small enough to be read again from the caches).  Mixed: prefix tiles and the sequences' own
+// planes as tiles of one launch, joined by a second.  Apart: prefix tiles first, then the kernels that stream own rows, which
+// join the two.  Own planes as tiles are the faster way while each has a unit and they are not the most of the work.  Us,
+// walk / mixed / apart, binary16, query heads / K/V heads, sequences, prefix, longest own rows:
+//   32 / 4,  2,  2000,    40:    9.4 /  11.8 /  14.4      64 / 8, 64,   300,    40:  13.2 /  22.2 /  16.6
+//   32 / 4, 24,  2000,    40:   19.6 /  16.2 /  18.1      32 / 4, 64,  8000,  1000: 148.6 /  39.2 /  51.2
+//   32 / 32, 8,  8000,    40:    154 /  31.2 /  31.4      64 / 8, 64,  8000,    40: 218.9 /  42.3 /  36.2
+//   64 / 8, 24,  2000,  4000:      - /  64.5 /  66.5      64 / 8, 24,  2000, 24000:     - / 314.3 / 237.0
+//   32 / 32, 24, 2000,    40:   95.8 /  28.1 /  18.7      64 / 8, 128, 32000, 4000:     - / 572.4 / 369.4
+enum class PrefixStep { kWalk, kMixed, kApart };
+inline PrefixStep shaped_prefix_step(uint32_t batch, uint32_t n_kv_heads, uint32_t group, uint32_t own_keys, uint32_t prefix,
+                                     uint32_t n_cu) {
+  const uint64_t planes = (uint64_t)batch * n_kv_heads;
+  if (planes * prefix <= 640 * (uint64_t)n_cu) return PrefixStep::kWalk;
+  const uint64_t own_steps = planes * shaped_ceil(own_keys, kShapedKeys);
+  return group <= kShapedRows / 2 && planes <= n_cu && own_steps <= 48 * (uint64_t)n_cu ? PrefixStep::kMixed : PrefixStep::kApart;
+}
+
+// Single tokens behind a shared prefix: the prefix alone, rows of all sequences of a K/V head packed into tiles, every walk
+// left as partial results for the launch that streams the sequences' own rows.
+inline ShapedPlan shaped_prefix_plan(uint32_t batch, uint32_t n_kv_heads, uint32_t group, uint32_t prefix, uint32_t n_cu,
+                                     size_t part_rows) {
+  ShapedPlan p{};
+  const uint64_t rows = (uint64_t)batch * n_kv_heads * group;
+  p.rows_plane = group;
+  p.prefix_rows = group * batch;
+  p.prefix_tiles = shaped_ceil(p.prefix_rows, kShapedRows);
+  const uint32_t steps = shaped_ceil(prefix, kShapedKeys);
+  const uint64_t walks = (uint64_t)p.prefix_tiles * n_kv_heads;
+  p.prefix_split = shaped_split(steps, walks, shaped_slots(walks * steps, n_cu), rows, true);
+  if (rows * p.prefix_split > part_rows) p.prefix_split = (uint32_t)(part_rows / rows);
+  p.n_part = p.prefix_split;   // (0: more rows than there is room for)
   return p;
 }
 
