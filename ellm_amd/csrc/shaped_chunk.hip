@@ -702,8 +702,6 @@ namespace {
 hipError_t launch_plan(const ShapedArgs& args, const ShapedPlan& plan, bool merge, hipStream_t stream) {
   const AttnArgs& a = args.a;
   const ShapedState& s = args.s;
-  // (rows are counted in 32 bits: 2^31 of them would be 2^39 bytes of queries)
-  if ((uint64_t)a.position_interval * a.batch_pitch * a.n_q_heads > 0x7fffffffull) return hipErrorInvalidValue;
   ShapedKernelArgs p{};
   p.q = (const uint16_t*)a.q;
   p.k = (const uint16_t*)a.k;

@@ -88,7 +88,8 @@ inline ShapedPlan shaped_plan(uint32_t interval, uint32_t batch, uint32_t n_kv_h
     const uint64_t total = prefix_walks * prefix_steps + walks * own_steps;
     const uint32_t slots = 2 * n_cu;
     uint32_t for_prefix = (uint32_t)(slots * (prefix_walks * prefix_steps) / total);
-    if (walks < slots && for_prefix > slots - walks) for_prefix = slots - (uint32_t)walks;   // (own walks take a place each)
+    if (for_prefix < prefix_walks) for_prefix = prefix_walks < slots ? (uint32_t)prefix_walks : slots;
+    if (walks < slots && for_prefix > slots - walks) for_prefix = slots - (uint32_t)walks;   // (a place for each walk at least)
     p.prefix_split = shaped_split(prefix_steps, prefix_walks, for_prefix ? for_prefix : 1, rows, true);
     p.n_split = shaped_split(own_steps, walks, slots > for_prefix ? slots - for_prefix : 1, rows, true);
     while (rows * (p.prefix_split + p.n_split) > part_rows && p.prefix_split + p.n_split > 2) {

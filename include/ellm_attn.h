@@ -172,9 +172,10 @@ int ellm_attn_run_ragged(ellm_attn* handle, const uint32_t* positions, size_t ma
  * on this handle: 0 = the single-token kernel of ellm_attn_run (every K/V plane split alike,
  * sized for max_position), 1 = the kernel that deals the keys of all planes to the workgroups
  * in equal shares, whatever the sequences' lengths (taken when the call is large enough for
- * the split to matter), 2 = the kernels for shaped scores and shared prefixes; negative: a status code (null handle, arguments out of range).  No
- * counterpart in the reference (its Attention::run has one code path); it lets a test or a
- * harness see which kernel its shapes reach.
+ * the split to matter), 2 = the handle has shaped scores or a shared prefix (either kernel in
+ * its form for those, or the tile kernel over the prefix); negative: a status code (null
+ * handle, arguments out of range).  No counterpart in the reference (its Attention::run has
+ * one code path); it lets a test or a harness see which kernel its shapes reach.
  */
 int ellm_attn_ragged_path(const ellm_attn* handle, size_t max_position, size_t batch_size);
 
