@@ -63,6 +63,8 @@ struct ShapedArgs {
 };
 
 hipError_t launch_shaped(const ShapedArgs& args, hipStream_t stream);
+// Chunks without a prefix and without positions of their own: 32 wr query rows a workgroup, wr 1 or 2.
+hipError_t launch_shaped_short(const ShapedArgs& args, uint32_t wr, bool along, hipStream_t stream);
 // Single tokens: the shared prefix alone, left as *parts partial results a row (0: no room for them, nothing launched).
 hipError_t launch_shaped_prefix(const ShapedArgs& args, uint32_t* parts, hipStream_t stream);
 

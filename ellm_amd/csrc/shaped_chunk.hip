@@ -15,6 +15,9 @@
 // sees is passed over, and in between the range is one compare a score.  Value rows that only some rows of a step see
 // may hold infinities and NaN: such a step looks at its values first (find_odd), multiplies odd ones apart and drops them.
 //
+// Weights are rounded to 16 bits for the second product (half a step each, relative: over random values that is as much as
+// the rounding of the result), their sums are taken before it, in 32 bits; so are scores, references and results.
+//
 // What bounds it (8192 tokens, 32 / 4 heads, binary16, 550 GFLOP): the board's power and the vector unit, 350 us with
 // constant operands and no weights, 555 without a cap, 645 with one (0.85 PFLOP/s; 69 us a plane's worth of transcendental
 // instructions), 560 with slopes.  Against a plain loop (Q.K, soft-max with a maximum every step, P.V) 740: references
@@ -25,8 +28,7 @@
 // one where a workgroup has a unit to itself (1 to 8 % slower: the chain of a step, 1.7 us, bounds it, no trip to memory).
 #include <type_traits>
 
-#include "common.hpp"
-#include "shaped.hpp"
+#include "shaped_common.hpp"
 
 namespace ellm {
 namespace {
@@ -39,104 +41,13 @@ static_assert(kRows == 32 * kWaves, "32 rows a wave");
 constexpr int kAhead = 4;     // LDS operand reads in flight ahead of their products
 constexpr int kKeys = (int)kShapedKeys;
 constexpr int kTileBytes = kKeys * kHeadDim * 2;
-constexpr uint32_t kNoKey = 0xffffffffu;
 
-typedef __attribute__((address_space(3))) uint16_t LdsHalf;
-typedef __attribute__((address_space(3))) u32x4 LdsU32x4;
-typedef __attribute__((address_space(3))) u32x2 LdsU32x2;
-typedef __attribute__((address_space(3))) f32x4 LdsF32x4;
-typedef short i16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) i16x4 LdsI16x4;
-constexpr int kBufferFlags = 0x00020000;  // raw buffer of 32-bit data, no swizzle (word 3 of the descriptor)
-
-struct ShapedKernelArgs {
-  const uint16_t* q;
-  const uint16_t* k;
-  const uint16_t* v;
-  const uint16_t* prefix_k;
-  const uint16_t* prefix_v;
-  uint16_t* out;
-  float* lse;
-  const uint32_t* positions;
-  const size_t* seq_offsets;
-  const uint32_t* seq_caps;
-  const float* slopes;
-  const uint32_t* key_begin;
-  const uint32_t* key_end;
-  float* part_o;    // [row][n_part][128]
-  float* part_ml;   // [row][n_part][2]: reference (log2 units), sum of weights
-  size_t bounds_pitch;
-  size_t q_token_stride;
-  size_t kv_stride_seq, kv_stride_head, kv_stride_pos;
-  size_t prefix_stride_head, prefix_stride_pos;
-  uint32_t batch, batch_pitch, n_q_heads, n_kv_heads, group;
-  uint32_t interval, position, capacity, prefix, window;
-  uint32_t rows_plane, tiles_plane, n_split, own_wgs;
-  uint32_t prefix_rows, prefix_tiles, prefix_split;
-  uint32_t n_part;
-  uint32_t whole;   // rows are finished here (one partial result, and nothing to join it to)
-  Divisor by_planes, by_kv_heads, by_split, by_prefix_split, by_rows_plane, by_group;
-  float c_in;     // with a cap: 2 scale log2(e) / cap
-  float a0, a1;   // y = a0 + a1 s (shaped.hpp)
-};
-
-// The own row of a query: its sequence's position, `token` further on.
-__device__ __forceinline__ uint32_t own_row(const ShapedKernelArgs& p, uint32_t seq, uint32_t token) {
-  const uint32_t first = p.positions ? min(p.positions[seq], p.position) : p.position;
-  return min(first + token, (p.seq_caps ? p.seq_caps[seq] : p.capacity) - 1);
-}
-__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
-__device__ __forceinline__ uint64_t uniform64(uint64_t x) {
-  return ((uint64_t)uniform((uint32_t)(x >> 32)) << 32) | (uint64_t)uniform((uint32_t)x);
-}
-// The same value, of which the compiler knows nothing: sums with it are formed where they are needed instead of being
-// kept in registers around a loop.
-__device__ __forceinline__ uint32_t opaque(uint32_t x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
 // 16 bytes a lane from memory straight to LDS address lds_at + 16 x lane.  Written as asm: the compiler's own form of
 // this load makes it wait for every outstanding one before each later LDS read.  (M0 is a register the compiler
 // reserves and never uses itself in these kernels; one wait state between its write and the load.)
 __device__ __forceinline__ void load_to_lds(const u32x4& rsrc, uint32_t voff, uint32_t lds_at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :: "s"(lds_at), "v"(voff), "s"(rsrc) : "memory");
-}
-
-// Packed pairs of 16-bit values: which are infinities or NaN, without compares (masks of lanes are scarce registers).
-template <typename T>
-struct Odd;
-template <>
-struct Odd<F16> {
-  static constexpr uint32_t kInf = 0x7c00u, kOne = 0x3c00u, kLast = 0x0400u;   // infinity, one, the exponent's last bit
-};
-template <>
-struct Odd<BF16> {
-  static constexpr uint32_t kInf = 0x7f80u, kOne = 0x3f80u, kLast = 0x0080u;
-};
-constexpr uint32_t both(uint32_t half) { return half * 0x10001u; }
-// the top bit of every half that is odd (an exponent of ones carries into it)
-template <typename T>
-__device__ __forceinline__ uint32_t odd_bits(uint32_t x) {
-  return ((x & both(Odd<T>::kInf)) + both(Odd<T>::kLast)) & both(0x8000u);
-}
-__device__ __forceinline__ uint32_t whole_halves(uint32_t top) { return (top - (top >> 15)) | top; }
-// The operand's finite values, zeros where it has others.
-template <typename T>
-__device__ __forceinline__ u32x4 finite_values(u32x4 a) {
-#pragma unroll
-  for (int w = 0; w < 4; ++w) a[w] &= ~whole_halves(odd_bits<T>(a[w]));
-  return a;
-}
-// Ones where the operand has infinities or NaN other than `but` (in both halves).
-template <typename T>
-__device__ __forceinline__ u32x4 odd_values(u32x4 a, uint32_t but) {
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const uint32_t d = a[w] ^ but, differs = ((d & both(0x7fffu)) + both(0x7fffu)) | d;   // (top bits)
-    a[w] = whole_halves(odd_bits<T>(a[w]) & differs) & both(Odd<T>::kOne);
-  }
-  return a;
 }
 
 template <typename T, bool CAP, bool SLOPES>
@@ -697,9 +608,7 @@ hipError_t launch(const ShapedKernelArgs& p, bool cap, bool slopes, bool merge, 
 
 }  // namespace
 
-namespace {
-
-hipError_t launch_plan(const ShapedArgs& args, const ShapedPlan& plan, bool merge, hipStream_t stream) {
+ShapedKernelArgs shaped_kernel_args(const ShapedArgs& args) {
   const AttnArgs& a = args.a;
   const ShapedState& s = args.s;
   ShapedKernelArgs p{};
@@ -735,28 +644,35 @@ hipError_t launch_plan(const ShapedArgs& args, const ShapedPlan& plan, bool merg
   p.capacity = a.capacity;
   p.prefix = s.prefix;
   p.window = s.window;
-  p.rows_plane = plan.rows_plane;
+  p.rows_plane = a.position_interval * a.group;
+  p.by_planes = divisor(a.batch * a.n_kv_heads);
+  p.by_kv_heads = divisor(a.n_kv_heads);
+  p.by_rows_plane = divisor(p.rows_plane);
+  p.by_group = divisor(a.group);
+  const ShapedScores f = shaped_scores(s, a.scale);
+  p.c_in = f.c_in;
+  p.a0 = f.a0;
+  p.a1 = f.a1;
+  return p;
+}
+
+namespace {
+
+hipError_t launch_plan(const ShapedArgs& args, const ShapedPlan& plan, bool merge, hipStream_t stream) {
+  const ShapedState& s = args.s;
+  ShapedKernelArgs p = shaped_kernel_args(args);
   p.tiles_plane = plan.tiles_plane;
   p.n_split = plan.n_split;
-  const uint32_t planes = a.batch * a.n_kv_heads;
-  p.own_wgs = planes * plan.tiles_plane * plan.n_split;
-  p.by_planes = divisor(planes);
-  p.by_kv_heads = divisor(a.n_kv_heads);
+  p.own_wgs = p.by_planes.d * plan.tiles_plane * plan.n_split;
   p.by_split = divisor(plan.n_split ? plan.n_split : 1);
   p.by_prefix_split = divisor(plan.prefix_split ? plan.prefix_split : 1);
-  p.by_rows_plane = divisor(plan.rows_plane);
-  p.by_group = divisor(a.group);
   p.prefix_rows = plan.prefix_rows;
   p.prefix_tiles = plan.prefix_tiles;
   p.prefix_split = plan.prefix_split;
   p.n_part = plan.n_part;
   p.whole = merge && plan.n_part == 1;
-  const ShapedScores f = shaped_scores(s, a.scale);
-  p.c_in = f.c_in;
-  p.a0 = f.a0;
-  p.a1 = f.a1;
-  return a.dtype == 0 ? launch<F16>(p, s.cap != 0.0f, s.slopes != nullptr, merge, stream)
-                      : launch<BF16>(p, s.cap != 0.0f, s.slopes != nullptr, merge, stream);
+  return args.a.dtype == 0 ? launch<F16>(p, s.cap != 0.0f, s.slopes != nullptr, merge, stream)
+                           : launch<BF16>(p, s.cap != 0.0f, s.slopes != nullptr, merge, stream);
 }
 
 }  // namespace
@@ -768,15 +684,26 @@ hipError_t launch_shaped(const ShapedArgs& args, hipStream_t stream) {
   uint32_t own_keys = a.position_index + a.position_interval;
   uint32_t prefix_keys = s.prefix;
   if (s.window) {
-    const uint64_t reach = (uint64_t)s.window + a.position_interval;
+    // (the positions a workgroup's rows span)
+    const uint32_t span = kShapedRows / a.group + 1;
+    const uint64_t reach = (uint64_t)s.window + (span < a.position_interval ? span : a.position_interval);
     if (reach < own_keys) {
       own_keys = (uint32_t)reach;
     } else if (!a.positions) {   // (own rows of sequences that are shorter than the bound on the host leave more to the prefix)
-      const uint64_t rest = reach - own_keys;
+      const uint64_t rest = (uint64_t)s.window + a.position_interval - own_keys;
       if (rest < prefix_keys) prefix_keys = (uint32_t)rest;
     }
   }
   const ShapedPlan plan = shaped_plan(a.position_interval, a.batch, a.n_kv_heads, a.group, own_keys, prefix_keys, a.n_cu, s.part_rows);
+  if (!s.prefix && !a.positions) {
+    ShapedShape c{a.position_interval * a.group, a.batch * a.n_kv_heads, a.n_cu, (double)own_keys,
+                  a.position_index + 0.5 * a.position_interval, (double)a.position_index + a.position_interval};
+    if (s.window) {
+      if (s.window < c.mean) c.mean = s.window;
+      if ((double)s.window + a.position_interval < c.rows) c.rows = (double)s.window + a.position_interval;
+    }
+    if (const uint32_t wr = shaped_short_rows(c, plan.n_split)) return launch_shaped_short(args, wr, shaped_short_along(c.planes, c.rows), stream);
+  }
   return launch_plan(args, plan, true, stream);
 }
 

@@ -107,6 +107,49 @@ inline ShapedPlan shaped_plan(uint32_t interval, uint32_t batch, uint32_t n_kv_h
   return p;
 }
 
+// ---- chunks without a prefix: the tile kernel or the one for short walks -----------------------------
+// Estimated times (us, launch included), fits to 230 back-to-back calls (binary16, capped; 32 / 4, 32 / 32 and 64 / 8 heads, 1
+// to 24 sequences, 8 to 1600 tokens on up to 4000): the longest walk's chain of steps, the work there is, or K and V from memory,
+// whichever is longest.  `longest` and `mean`: keys of the longest walk and of an average row; `rows`: K/V rows that are read.
+struct ShapedShape {
+  uint32_t rows_plane, planes, n_cu;
+  double longest, mean, rows;
+  double steps(double walks, double keys) const { return walks * (mean / keys + 1); }
+  double units() const { return 256.0 / n_cu; }
+  double stream_us() const { return planes * rows * 512 / 6.5e6; }
+};
+inline double shaped_longest(double a, double b, double c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); }
+// 250 tokens, 32 / 4 heads, 12.4 (measured 12.5); 1000 x 8 102 (101); 250 x 24 on 1000 146 (147); 8 on 4000, 31 splits, 16 (15.5).
+inline double shaped_tile_us(const ShapedShape& c, uint32_t n_split) {
+  const double walks = c.planes * (double)shaped_ceil(c.rows_plane, kShapedRows);
+  const double work = (0.0083 * walks * n_split + 0.0045 * c.steps(walks, kShapedKeys)) * c.units();
+  const double chain = 0.8 + 1.65 * shaped_ceil(shaped_ceil((uint64_t)c.longest, kShapedKeys), n_split);
+  const double partials = n_split > 1 ? 4.5 + 1e-4 * c.planes * (double)c.rows_plane * n_split : 0.0;
+  return 5.0 + shaped_longest(chain, work, c.stream_us()) + partials;
+}
+// wr = 1: 500 tokens, 32 / 4 heads, 10.7 (12.1); 33 x 5 on 800 14.1 (13.7); 250 x 24 on 1000 251 (265); wr = 2: 500 tokens 16.0
+// (15.7); 1000 x 8 136 (136); 33 x 24 on 800 28 (29).
+inline double shaped_short_us(const ShapedShape& c, uint32_t wr) {
+  const double wgs = c.planes * (double)shaped_ceil(c.rows_plane, 32 * wr);
+  const double tiles = c.steps(c.planes * (double)shaped_ceil(c.rows_plane, 32), 32);
+  const double work = (0.0075 * wgs + (wr == 1 ? 0.00092 : 0.00078) * tiles) * c.units();
+  const double chain = 1.2 + (wr == 1 ? 1.13 : 1.22) * shaped_ceil((uint64_t)c.longest, 128 / wr);
+  return 5.0 + shaped_longest(chain, work, c.stream_us() * (wr == 1 ? 1.0 : 1.02)) + (wr == 1 ? 0.0 : 0.1);
+}
+// Blocks of 32 rows a workgroup of the short-walk kernel, 1 or 2; 0: the tile kernel, unless it is estimated 5 % slower.  Over
+// those calls the choice is on average 0.4 % behind the best of the three and never 7 % behind the tile kernel; against that
+// kernel alone: 33 x 5 on 800 20.0 -> 13.7, 250 tokens 12.5 -> 7.6, 500 19.1 -> 12.1, 64 on 500 14.9 -> 11.0, 250 on 1000 24.5 -> 17.6.
+inline uint32_t shaped_short_rows(const ShapedShape& c, uint32_t tile_splits) {
+  const double tile = 1.05 * shaped_tile_us(c, tile_splits), one = shaped_short_us(c, 1), two = shaped_short_us(c, 2);
+  if (tile <= one && tile <= two) return 0;
+  return one <= two ? 1 : 2;
+}
+// Whether its workgroups are dealt along a plane's tiles, one XCD to a plane: where planes overflow the XCDs' caches or do not
+// come out even over them.
+inline bool shaped_short_along(uint32_t planes, double rows) {
+  return planes >= 32 && (planes % 8 || planes / 8.0 * rows * 512e-6 > 8.0);
+}
+
 // How a single-token step behind a shared prefix runs.  Walk: every sequence streams the prefix and its own rows as one
 // plane (one launch; the prefix is small enough to be read again from the caches).  Mixed: prefix tiles and the sequences' own
 // planes as tiles of one launch, joined by a second.  Apart: prefix tiles first, then the kernels that stream own rows, which

@@ -107,7 +107,25 @@ static void ways() {
   CHECK(shaped_plan(241, 1, 4, 8, 241, 0, 256, 1 << 17).n_part == 1);
 }
 
-int main() { divisors(); shares(); plans(); ways(); printf("done\n"); return 0; }
+static uint32_t chunk_way(uint32_t hq, uint32_t hkv, uint32_t batch, uint32_t start, uint32_t interval, uint32_t* splits) {
+  const uint32_t group = hq / hkv, keys = start + interval;
+  *splits = shaped_plan(interval, batch, hkv, group, keys, 0, 256, shaped_part_rows(interval, batch, hq, 256)).n_split;
+  return shaped_short_rows({interval * group, batch * hkv, 256, (double)keys, start + 0.5 * interval, (double)keys}, *splits);
+}
+
+static void chunks() {   // the calls that the GPU tests make for the sake of a kernel
+  uint32_t splits;
+  CHECK(chunk_way(16, 2, 2, 300, 70, &splits) == 1);
+  CHECK(chunk_way(8, 2, 3, 30, 150, &splits) == 1);
+  CHECK(chunk_way(64, 1, 2, 200, 120, &splits) == 2);
+  CHECK(chunk_way(64, 1, 7, 200, 33, &splits) == 2);
+  CHECK(chunk_way(64, 1, 12, 0, 70, &splits) == 0 && splits == 1);
+  CHECK(chunk_way(8, 1, 2, 2600, 9, &splits) == 0 && splits > 1);
+  CHECK(chunk_way(32, 4, 1, 0, 8192, &splits) == 0 && splits == 1);
+  CHECK(chunk_way(32, 4, 1, 0, 2, &splits) == 1);
+}
+
+int main() { divisors(); shares(); plans(); ways(); chunks(); printf("done\n"); return 0; }
 """
 
 
@@ -120,6 +138,12 @@ def test_plans_shares_and_divisions(tmp_path):
     subprocess.run([gxx, "-O2", "-std=c++17", "-Wall", "-Werror", "-I", CSRC, str(src), "-o", str(exe)], check=True, timeout=300)
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.endswith("done\n"), r.stdout
+
+
+def test_short_walk_kernel_keeps_no_scratch(tmp_path):
+    text = _listing("shaped_short.hip", tmp_path)
+    assert set(re.findall(r"\.private_segment_fixed_size:\s*(\d+)", text)) == {"0"}
+    assert set(re.findall(r"\.[sv]gpr_spill_count:\s*(\d+)", text)) == {"0"}
 
 
 def test_tile_kernel_keeps_no_scratch_and_leaves_m0_to_the_inline_asm(tmp_path):
