@@ -695,14 +695,16 @@ hipError_t launch_shaped(const ShapedArgs& args, hipStream_t stream) {
     }
   }
   const ShapedPlan plan = shaped_plan(a.position_interval, a.batch, a.n_kv_heads, a.group, own_keys, prefix_keys, a.n_cu, s.part_rows);
-  if (!s.prefix && !a.positions) {
-    ShapedShape c{a.position_interval * a.group, a.batch * a.n_kv_heads, a.n_cu, (double)own_keys,
-                  a.position_index + 0.5 * a.position_interval, (double)a.position_index + a.position_interval};
+  if (!a.positions && (!s.prefix || a.position_interval > 1)) {
+    const double end = (double)s.prefix + a.position_index + a.position_interval;
+    ShapedShape c{a.position_interval * a.group, a.batch * a.n_kv_heads, a.n_kv_heads, a.n_cu, (double)own_keys + prefix_keys,
+                  end - 0.5 * a.position_interval, (double)a.position_index + a.position_interval, (double)prefix_keys};
     if (s.window) {
       if (s.window < c.mean) c.mean = s.window;
       if ((double)s.window + a.position_interval < c.rows) c.rows = (double)s.window + a.position_interval;
+      if (c.prefix > c.mean) c.prefix = c.mean;
     }
-    if (const uint32_t wr = shaped_short_rows(c, plan.n_split)) return launch_shaped_short(args, wr, shaped_short_along(c.planes, c.rows), stream);
+    if (const uint32_t wr = shaped_short_rows(c, plan)) return launch_shaped_short(args, wr, shaped_short_along(c.planes, c.longest), stream);
   }
   return launch_plan(args, plan, true, stream);
 }

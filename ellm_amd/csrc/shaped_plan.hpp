@@ -107,40 +107,49 @@ inline ShapedPlan shaped_plan(uint32_t interval, uint32_t batch, uint32_t n_kv_h
   return p;
 }
 
-// ---- chunks without a prefix: the tile kernel or the one for short walks -----------------------------
-// Estimated times (us, launch included), fits to 230 back-to-back calls (binary16, capped; 32 / 4, 32 / 32 and 64 / 8 heads, 1
-// to 24 sequences, 8 to 1600 tokens on up to 4000): the longest walk's chain of steps, the work there is, or K and V from memory,
-// whichever is longest.  `longest` and `mean`: keys of the longest walk and of an average row; `rows`: K/V rows that are read.
+// ---- chunks: the tile kernel or the one for short walks ----------------------------------------------
+// Estimated times (us, launch included), fits to 565 back-to-back calls (binary16, capped; 32 / 4, 32 / 32 and 64 / 8 heads, 1
+// to 24 sequences, 2 to 1600 tokens on up to 4000, with and without a shared prefix of 60 to 2500): the longest walk's chain of
+// steps, the work there is, or K and V from memory, whichever is longest.  `longest` and `mean`: keys of the longest walk and
+// of an average row.
 struct ShapedShape {
-  uint32_t rows_plane, planes, n_cu;
-  double longest, mean, rows;
-  double steps(double walks, double keys) const { return walks * (mean / keys + 1); }
+  uint32_t rows_plane, planes, n_kv_heads, n_cu;
+  double longest, mean, rows;   // (rows: of a sequence's own)
+  double prefix;                // of those keys, as far as the window leaves them
+  double steps(double walks, double seen, double keys) const { return walks * (seen / keys + 1); }
   double units() const { return 256.0 / n_cu; }
-  double stream_us() const { return planes * rows * 512 / 6.5e6; }
+  double stream_us() const { return (planes * rows + n_kv_heads * prefix) * 512 / 6.5e6; }
 };
 inline double shaped_longest(double a, double b, double c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); }
-// 250 tokens, 32 / 4 heads, 12.4 (measured 12.5); 1000 x 8 102 (101); 250 x 24 on 1000 146 (147); 8 on 4000, 31 splits, 16 (15.5).
-inline double shaped_tile_us(const ShapedShape& c, uint32_t n_split) {
-  const double walks = c.planes * (double)shaped_ceil(c.rows_plane, kShapedRows);
-  const double work = (0.0083 * walks * n_split + 0.0045 * c.steps(walks, kShapedKeys)) * c.units();
-  const double chain = 0.8 + 1.65 * shaped_ceil(shaped_ceil((uint64_t)c.longest, kShapedKeys), n_split);
-  const double partials = n_split > 1 ? 4.5 + 1e-4 * c.planes * (double)c.rows_plane * n_split : 0.0;
-  return 5.0 + shaped_longest(chain, work, c.stream_us()) + partials;
+// Estimated (measured): 250 tokens, 32 / 4 heads, 12.4 (12.5); 1000 x 8 102 (101); 250 x 24 on 1000 146 (148); 8 on 4000, 31 splits,
+// 14.8 (15.5); behind a prefix of 1000, 9 x 8, 64 / 8 heads, 17.3 (19.2); 9 x 24 on 100, 32 / 32 heads, 29.6 (33.3).
+inline double shaped_tile_us(const ShapedShape& c, const ShapedPlan& p) {
+  const double walks = c.planes * (double)p.tiles_plane, ahead = c.n_kv_heads * (double)p.prefix_tiles;
+  const double apart = p.prefix_tiles ? c.prefix : 0.0;   // keys that packed rows of all sequences walk
+  const double wgs = walks * p.n_split + ahead * p.prefix_split;
+  const double work = (0.0083 * wgs + 0.0045 * (c.steps(walks, c.mean - apart, kShapedKeys) + c.steps(ahead, apart, kShapedKeys))) * c.units();
+  uint32_t longest = shaped_ceil(shaped_ceil((uint64_t)(c.longest - apart), kShapedKeys), p.n_split);
+  if (p.prefix_tiles) {
+    const uint32_t other = shaped_ceil(shaped_ceil((uint64_t)apart, kShapedKeys), p.prefix_split);
+    longest = other > longest ? other : longest;
+  }
+  const double partials = p.n_part > 1 ? 3.5 + 7.4e-5 * c.planes * (double)c.rows_plane * p.n_part : 0.0;
+  return (5.0 + shaped_longest(0.8 + 1.65 * longest, work, c.stream_us()) + partials) * (p.prefix_tiles ? 0.914 : 1.0);
 }
-// wr = 1: 500 tokens, 32 / 4 heads, 10.7 (12.1); 33 x 5 on 800 14.1 (13.7); 250 x 24 on 1000 251 (265); wr = 2: 500 tokens 16.0
-// (15.7); 1000 x 8 136 (136); 33 x 24 on 800 28 (29).
+// wr = 1: 500 tokens, 32 / 4 heads, 12.9 (12.7); 33 x 5 on 800 15.2 (14.9); 250 x 24 on 1000 271 (270); 40 x 2 on 100 behind 300, 64 / 8
+// heads, 11.3 (10.9); wr = 2: 500 tokens 18.2 (17.4); 1000 x 8 138 (148); 33 x 24 on 800 29.0 (31.4).
 inline double shaped_short_us(const ShapedShape& c, uint32_t wr) {
-  const double wgs = c.planes * (double)shaped_ceil(c.rows_plane, 32 * wr);
-  const double tiles = c.steps(c.planes * (double)shaped_ceil(c.rows_plane, 32), 32);
-  const double work = (0.0075 * wgs + (wr == 1 ? 0.00092 : 0.00078) * tiles) * c.units();
-  const double chain = 1.2 + (wr == 1 ? 1.13 : 1.22) * shaped_ceil((uint64_t)c.longest, 128 / wr);
+  const double wgs = c.planes * (double)shaped_ceil(c.rows_plane, 32 * wr), tiles = c.steps(wgs * wr, c.mean, 32);
+  const double work = (wr == 1 ? 0.0068 * wgs + 0.00103 * tiles : 0.0052 * wgs + 0.00084 * tiles) * c.units();
+  const double chain = 1.2 + (wr == 1 ? 1.28 : 1.49) * shaped_ceil((uint64_t)c.longest, 128 / wr);
   return 5.0 + shaped_longest(chain, work, c.stream_us() * (wr == 1 ? 1.0 : 1.02)) + (wr == 1 ? 0.0 : 0.1);
 }
 // Blocks of 32 rows a workgroup of the short-walk kernel, 1 or 2; 0: the tile kernel, unless it is estimated 5 % slower.  Over
-// those calls the choice is on average 0.4 % behind the best of the three and never 7 % behind the tile kernel; against that
-// kernel alone: 33 x 5 on 800 20.0 -> 13.7, 250 tokens 12.5 -> 7.6, 500 19.1 -> 12.1, 64 on 500 14.9 -> 11.0, 250 on 1000 24.5 -> 17.6.
-inline uint32_t shaped_short_rows(const ShapedShape& c, uint32_t tile_splits) {
-  const double tile = 1.05 * shaped_tile_us(c, tile_splits), one = shaped_short_us(c, 1), two = shaped_short_us(c, 2);
+// those calls the choice is on average 0.4 % behind the best of the three and at most 9 % behind the tile kernel; against that
+// kernel alone: 33 x 5 on 800 20.0 -> 14.9, 250 tokens 12.5 -> 8.1, 500 19.1 -> 12.7, 16 x 5 on 500, 32 / 32 heads, 20.0 -> 12.0, 40 x 2 on 100
+// behind 300, 64 / 8 heads, 19.8 -> 10.9.
+inline uint32_t shaped_short_rows(const ShapedShape& c, const ShapedPlan& plan) {
+  const double tile = 1.047 * shaped_tile_us(c, plan), one = shaped_short_us(c, 1), two = shaped_short_us(c, 2);
   if (tile <= one && tile <= two) return 0;
   return one <= two ? 1 : 2;
 }

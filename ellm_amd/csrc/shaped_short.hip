@@ -9,8 +9,8 @@
 // are not finite multiplied apart where only some rows see them, walks from the last key where scores fall with distance.
 // What bounds it: the chain of turns, 1.1 us each (32 keys: fetch, eight products, scores and weights, eight products), and up
 // to 6 us of launch, start and end.  Capped, binary16, us, tile kernel / this: 33 tokens x 5 on 777, 32 / 4 heads, 19.7 / 14.0; 241
-// tokens 12.7 / 7.3; 16 x 5 on 500, 32 / 32 heads, 19.9 / 11.2; 8 x 5 on 1500 42.2 / 21.9; 618 tokens 24.0 / 18.2 (shaped_plan.hpp
-// chooses).  The two kernels of plain scores it stands beside take 11.3, 7.0 and 9.4 us for the first three.
+// tokens 12.7 / 7.3; 16 x 5 on 500, 32 / 32 heads, 19.9 / 11.2; 8 x 5 on 1500 42.2 / 21.9; 618 tokens 24.0 / 17.7; 40 x 2 on 100
+// behind a prefix of 300, 64 / 8 heads, 19.8 / 10.9 (shaped_plan.hpp chooses).  The two kernels of plain scores it stands beside take 11.3, 7.0 and 9.4 us for the first three.
 #include "shaped_common.hpp"
 
 namespace ellm {
@@ -23,7 +23,8 @@ constexpr int kTileBytes = kKeys * kHeadDim * 2;           // of K, and of V
 // Waits for this wave's LDS accesses, then for the workgroup's waves (loads on their way to registers stay there).
 __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <typename T, bool CAP, bool SLOPES, int WR>
+// PREFIX: there is a shared prefix, whose last tile may be a part of one (6 % of a walk without it).
+template <typename T, bool CAP, bool SLOPES, bool PREFIX, int WR>
 __global__ __launch_bounds__(kThreads, 2) void shaped_short_kernel(ShapedKernelArgs p) {
   constexpr int kGroups = 4 / WR;
   constexpr int kBufs = WR == 1 ? 1 : 2;     // (one wave: its LDS accesses are in order, no second buffer)
@@ -73,12 +74,14 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_short_kernel(ShapedKernelA
   };
   Reach mine, all;   // the wave's, the workgroup's
   auto first_seen = [&](uint32_t pos) { return p.window && pos + 1 > p.window ? pos + 1 - p.window : 0u; };
-  const uint32_t pos = p.position + token;
+  // (read again where it is needed: as a value kept around the loop it costs the walks of one wave 80 spilled registers)
+  auto prefix = [&]() __attribute__((always_inline)) { return PREFIX ? p.prefix : 0u; };
+  const uint32_t base = prefix() + p.position, pos = base + token;   // (key ranges do not go with a prefix)
   uint32_t lo = first_seen(pos), hi = pos + 1;
   if (uniform(!p.key_begin && !p.key_end)) {   // ranges that move on with the rows
     auto reach = [&](uint32_t first, uint32_t last) {
       if (first >= n_rows) return Reach{kNoKey, 0u, 0u, kNoKey};
-      const uint32_t a = p.position + p.by_group.quotient(first), b = p.position + p.by_group.quotient(min(last, n_rows - 1));
+      const uint32_t a = base + p.by_group.quotient(first), b = base + p.by_group.quotient(min(last, n_rows - 1));
       return Reach{first_seen(a), b + 1, first_seen(b), a + 1};
     };
     mine = reach(wave_row, wave_row + 31);
@@ -113,22 +116,31 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_short_kernel(ShapedKernelA
   if (!valid) lo = 0, hi = kNoKey;   // (rows that are not stored never ask for a mask)
   const uint32_t w_lo = uniform(mine.lo), w_hi = uniform(mine.hi), all_lo = uniform(mine.all_lo), all_hi = uniform(mine.all_hi);
   const uint32_t hull_lo = uniform(all.lo), hull_hi = uniform(all.hi), wg_lo = uniform(all.all_lo), wg_hi = uniform(all.all_hi);
-  const uint32_t first = hull_lo / kKeys, n_tiles = hull_lo < hull_hi ? (hull_hi - 1) / kKeys + 1 - first : 0u;
-  auto key_of = [&](uint32_t i) { return kKeys * (SLOPES ? first + n_tiles - 1 - i : first + i); };   // tile i's first key
+  const uint32_t prefix_tiles = (prefix() + kKeys - 1) / kKeys;
+  auto tile_of = [&](uint32_t key) { return key < prefix() ? key / kKeys : prefix_tiles + (key - prefix()) / kKeys; };
+  const uint32_t first = tile_of(hull_lo), n_tiles = hull_lo < hull_hi ? tile_of(hull_hi - 1) + 1 - first : 0u;
+  auto place = [&](uint32_t i) { return SLOPES ? first + n_tiles - 1 - i : first + i; };   // of the walk's tile i among the keys'
+  auto key_of = [&](uint32_t i) {   // its first key
+    const uint32_t at = place(i);
+    return at < prefix_tiles ? at * kKeys : prefix() + (at - prefix_tiles) * kKeys;
+  };
+  auto keys_end = [&](uint32_t i) { return place(i) < prefix_tiles ? min(prefix(), key_of(i) + kKeys) : key_of(i) + kKeys; };
 
   // ---- staging: memory -> registers -> the group's tiles ------------------------------------------------
   const size_t plane_at = seq_plane_offset(p.seq_offsets, p.kv_stride_seq, seq) + kvh * p.kv_stride_head;
-  const uint64_t kplane = uniform64((uint64_t)(p.k + plane_at)), vplane = uniform64((uint64_t)(p.v + plane_at));
-  const uint32_t pitch = 2 * (uint32_t)p.kv_stride_pos;   // bytes; 32 rows of it stay below 2^31
   const int ld_r = 4 * rw + (lane >> 4), ld_x = lane & 15;   // rows ld_r + 4 WR i
   u32x4 kst[kPieces], vst[kPieces];
   auto load = [&](uint32_t i) __attribute__((always_inline)) {
-    const uint32_t at = key_of(i);
+    const bool ahead = place(i) < prefix_tiles;   // (uniform)
+    const uint32_t skip = ahead ? key_of(i) : key_of(i) - prefix(), n = ahead ? prefix() : hull_hi - prefix();
+    const uint32_t pitch = 2 * (uint32_t)(ahead ? p.prefix_stride_pos : p.kv_stride_pos);   // bytes; 32 rows of it stay below 2^31
+    const size_t plane = ahead ? kvh * p.prefix_stride_head : plane_at;
     // (bytes up to the end of the last row that is read: rows past it read as zeros)
-    const uint64_t off = (uint64_t)at * pitch, left = (uint64_t)(hull_hi - 1 - at) * pitch + 2 * kHeadDim;
+    const uint64_t off = 2 * plane + (uint64_t)skip * pitch, left = (uint64_t)(n - 1 - skip) * pitch + 2 * kHeadDim;
     const uint32_t room = uniform(left >> 32 ? 0xffffffffu : (uint32_t)left);
-    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)uniform64(kplane + off), 0, room, kBufferFlags);
-    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)uniform64(vplane + off), 0, room, kBufferFlags);
+    const uint64_t kat = uniform64((uint64_t)(ahead ? p.prefix_k : p.k) + off), vat = uniform64((uint64_t)(ahead ? p.prefix_v : p.v) + off);
+    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)kat, 0, room, kBufferFlags);
+    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)vat, 0, room, kBufferFlags);
     const uint32_t from = opaque(ld_r) * pitch + 16 * ld_x;   // (sums formed here, not kept around the loop)
 #pragma unroll
     for (int n = 0; n < kPieces; ++n) kst[n] = __builtin_amdgcn_raw_buffer_load_b128(kr, from + 4 * WR * n * pitch, 0, 0);
@@ -190,12 +202,21 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_short_kernel(ShapedKernelA
   const float hidden = a1 < 0.0f ? INFINITY : -INFINITY;
   auto off_of = [](int r) { return 8 * (r >> 2) + (r & 3); };   // keys of the lane: first key + 4 g + off
   bool started = false;
+  struct Seen {   // which keys of a tile a row sees: off - from < width, unsigned
+    int32_t from;
+    uint32_t width;
+  };
+  auto seen_of = [&](uint32_t i) {
+    const uint32_t last = min(hi, keys_end(i));
+    return Seen{(int32_t)(lo - key_of(i)) - 4 * g, last > lo ? last - lo : 0u};
+  };
 
   // Values that are not finite are multiplied apart, how many a row sees of those that lead to +inf and to -inf (a NaN is one
   // of each) ...
   auto add_odd = [&](uint32_t i, uint32_t buf) __attribute__((always_inline)) {
-    const uint32_t vs = v_read + buf * 2 * kTileBytes, width = opaque(hi - lo);
-    const int32_t from = (int32_t)opaque(lo - key_of(i)) - 4 * g;
+    const Seen see = seen_of(i);
+    const uint32_t vs = v_read + buf * 2 * kTileBytes, width = opaque(see.width);
+    const int32_t from = (int32_t)opaque((uint32_t)see.from);
     u32x4 ones[2];   // for the keys the row sees
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
@@ -236,8 +257,8 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_short_kernel(ShapedKernelA
   };
 
   auto compute = [&](uint32_t i, uint32_t buf) __attribute__((always_inline)) {
-    const uint32_t kb = key_of(i);
-    if (uniform(kb >= w_hi || kb + kKeys <= w_lo)) return;
+    const uint32_t kb = key_of(i), ke = keys_end(i);
+    if (uniform(kb >= w_hi || ke <= w_lo)) return;
     const uint32_t ks = opaque(k_read + buf * 2 * kTileBytes), vs = opaque(v_read + buf * 2 * kTileBytes);
     f32x16 st;
 #pragma unroll
@@ -254,11 +275,10 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_short_kernel(ShapedKernelA
         st[r] = x;
       }
     }
-    const int32_t from = (int32_t)(lo - kb) - 4 * g;   // the row sees the keys with off - from < width, unsigned
-    const uint32_t width = hi - lo;
-    if (uniform(all_lo > kb || all_hi < kb + kKeys)) {
+    if (uniform(all_lo > kb || all_hi < kb + kKeys || ke < kb + kKeys)) {
+      const Seen see = seen_of(i);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) st[r] = (uint32_t)(off_of(r) - from) < width ? st[r] : hidden;
+      for (int r = 0; r < 16; ++r) st[r] = (uint32_t)(off_of(r) - see.from) < see.width ? st[r] : hidden;
     }
     // Weights against the reference that each row already has; where their sum passes kMaxSum (or a row has none yet) rows
     // move to the turn's maximum and have them computed again.
@@ -382,18 +402,24 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_short_kernel(ShapedKernelA
   }
 }
 
-template <typename T, int WR>
+template <typename T, bool PREFIX, int WR>
 hipError_t launch(const ShapedKernelArgs& p, uint32_t wgs, bool cap, bool slopes, hipStream_t stream) {
   const dim3 grid(wgs), block(kThreads);
   if (cap && slopes)
-    hipLaunchKernelGGL((shaped_short_kernel<T, true, true, WR>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((shaped_short_kernel<T, true, true, PREFIX, WR>), grid, block, 0, stream, p);
   else if (cap)
-    hipLaunchKernelGGL((shaped_short_kernel<T, true, false, WR>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((shaped_short_kernel<T, true, false, PREFIX, WR>), grid, block, 0, stream, p);
   else if (slopes)
-    hipLaunchKernelGGL((shaped_short_kernel<T, false, true, WR>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((shaped_short_kernel<T, false, true, PREFIX, WR>), grid, block, 0, stream, p);
   else
-    hipLaunchKernelGGL((shaped_short_kernel<T, false, false, WR>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((shaped_short_kernel<T, false, false, PREFIX, WR>), grid, block, 0, stream, p);
   return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch(const ShapedKernelArgs& p, uint32_t wgs, uint32_t wr, bool cap, bool slopes, hipStream_t stream) {
+  if (p.prefix) return wr == 1 ? launch<T, true, 1>(p, wgs, cap, slopes, stream) : launch<T, true, 2>(p, wgs, cap, slopes, stream);
+  return wr == 1 ? launch<T, false, 1>(p, wgs, cap, slopes, stream) : launch<T, false, 2>(p, wgs, cap, slopes, stream);
 }
 
 }  // namespace
@@ -407,8 +433,7 @@ hipError_t launch_shaped_short(const ShapedArgs& args, uint32_t wr, bool along, 
   p.along = along;
   const uint32_t wgs = p.along ? (planes + 7) / 8 * 8 * p.tiles_plane : planes * p.tiles_plane;
   const bool cap = args.s.cap != 0.0f, slopes = args.s.slopes != nullptr;
-  if (a.dtype == 0) return wr == 1 ? launch<F16, 1>(p, wgs, cap, slopes, stream) : launch<F16, 2>(p, wgs, cap, slopes, stream);
-  return wr == 1 ? launch<BF16, 1>(p, wgs, cap, slopes, stream) : launch<BF16, 2>(p, wgs, cap, slopes, stream);
+  return a.dtype == 0 ? launch<F16>(p, wgs, wr, cap, slopes, stream) : launch<BF16>(p, wgs, wr, cap, slopes, stream);
 }
 
 }  // namespace ellm

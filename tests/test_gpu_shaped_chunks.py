@@ -14,8 +14,8 @@ pytestmark = pytest.mark.gpu
 CHUNKS = {  # query heads, K/V heads, sequences, start, interval
     "short 1": (16, 2, 2, 300, 70),
     "short 1, tails": (8, 2, 3, 30, 150),
-    "short 2": (64, 1, 2, 200, 120),
-    "short 2, tails": (64, 1, 7, 200, 33),
+    "short 2": (64, 1, 6, 200, 45),
+    "short 2, tails": (64, 1, 9, 200, 33),
     "tiles": (64, 1, 12, 0, 70),
     "tiles, split": (8, 1, 2, 2600, 9),
 }
@@ -160,3 +160,30 @@ def test_steep_scores_on_short_walks(dtype, scores):
         t.op.set_scores(**more)
         t.op.run(500, 64, 1)
         t.check(t.want([500], **more), f"ramp {step}")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("scores", [dict(), dict(cap=20.0, slopes=True), dict(window=70), dict(window=9, cap=30.0)])
+@pytest.mark.parametrize("hq,hkv,batch,prefix,start,interval", [
+    (8, 2, 2, 150, 10, 40), (64, 1, 13, 150, 0, 20), (32, 4, 2, 5000, 0, 9), (8, 2, 1, 1, 0, 33), (16, 1, 2, 32, 5, 64), (4, 4, 3, 65, 31, 2),
+])
+def test_short_walks_behind_a_prefix(hq, hkv, batch, prefix, start, interval, scores, dtype):
+    t = Setup(58, dtype, hq, hkv, batch, interval, start + interval + 2, prefix=prefix)
+    scores = dict(scores, slopes=slopes_of(hq) if scores.get("slopes") else None)
+    t.op.set_scores(**scores)
+    t.op.set_shared_prefix(*t.prefix)
+    t.op.run(start, interval, batch)
+    t.check(t.want([start] * batch, **scores), "behind a prefix")
+
+
+def test_prefix_rows_that_a_window_leaves_out_may_hold_anything():
+    for batch, prefix, interval in ((2, 150, 40), (13, 150, 20)):
+        t = Setup(59, F16, 64, 1, batch, interval, 100, prefix=prefix)
+        for x in t.prefix:
+            x[:, :-20] = float("nan")
+        t.op.set_shared_prefix(*t.prefix)
+        t.op.set_scores(window=20)
+        t.op.run(0, interval, batch)
+        for x in t.prefix:
+            x[:, :-20] = 0.0
+        t.check(t.want([0] * batch, window=20), f"{batch} sequences")

@@ -107,22 +107,27 @@ static void ways() {
   CHECK(shaped_plan(241, 1, 4, 8, 241, 0, 256, 1 << 17).n_part == 1);
 }
 
-static uint32_t chunk_way(uint32_t hq, uint32_t hkv, uint32_t batch, uint32_t start, uint32_t interval, uint32_t* splits) {
-  const uint32_t group = hq / hkv, keys = start + interval;
-  *splits = shaped_plan(interval, batch, hkv, group, keys, 0, 256, shaped_part_rows(interval, batch, hq, 256)).n_split;
-  return shaped_short_rows({interval * group, batch * hkv, 256, (double)keys, start + 0.5 * interval, (double)keys}, *splits);
+static uint32_t chunk_way(uint32_t hq, uint32_t hkv, uint32_t batch, uint32_t prefix, uint32_t start, uint32_t interval,
+                          uint32_t* splits) {
+  const uint32_t group = hq / hkv, own = start + interval, keys = prefix + own;
+  const ShapedPlan p = shaped_plan(interval, batch, hkv, group, own, prefix, 256, shaped_part_rows(interval, batch, hq, 256));
+  *splits = p.n_part;
+  return shaped_short_rows({interval * group, batch * hkv, hkv, 256, (double)keys, keys - 0.5 * interval, (double)own, (double)prefix}, p);
 }
 
 static void chunks() {   // the calls that the GPU tests make for the sake of a kernel
   uint32_t splits;
-  CHECK(chunk_way(16, 2, 2, 300, 70, &splits) == 1);
-  CHECK(chunk_way(8, 2, 3, 30, 150, &splits) == 1);
-  CHECK(chunk_way(64, 1, 2, 200, 120, &splits) == 2);
-  CHECK(chunk_way(64, 1, 7, 200, 33, &splits) == 2);
-  CHECK(chunk_way(64, 1, 12, 0, 70, &splits) == 0 && splits == 1);
-  CHECK(chunk_way(8, 1, 2, 2600, 9, &splits) == 0 && splits > 1);
-  CHECK(chunk_way(32, 4, 1, 0, 8192, &splits) == 0 && splits == 1);
-  CHECK(chunk_way(32, 4, 1, 0, 2, &splits) == 1);
+  CHECK(chunk_way(16, 2, 2, 0, 300, 70, &splits) == 1);
+  CHECK(chunk_way(8, 2, 3, 0, 30, 150, &splits) == 1);
+  CHECK(chunk_way(64, 1, 6, 0, 200, 45, &splits) == 2);
+  CHECK(chunk_way(64, 1, 9, 0, 200, 33, &splits) == 2);
+  CHECK(chunk_way(64, 1, 12, 0, 0, 70, &splits) == 0 && splits == 1);
+  CHECK(chunk_way(8, 1, 2, 0, 2600, 9, &splits) == 0 && splits > 1);
+  CHECK(chunk_way(32, 4, 1, 0, 0, 8192, &splits) == 0 && splits == 1);
+  CHECK(chunk_way(32, 4, 1, 0, 0, 2, &splits) == 1);
+  CHECK(chunk_way(8, 2, 2, 150, 10, 40, &splits) == 1);
+  CHECK(chunk_way(64, 1, 13, 150, 0, 20, &splits) == 2);
+  CHECK(chunk_way(32, 4, 2, 5000, 0, 9, &splits) == 0 && splits > 1);
 }
 
 int main() { divisors(); shares(); plans(); ways(); chunks(); printf("done\n"); return 0; }
