@@ -364,7 +364,8 @@ int ellm::attn_run_single_token(ellm_attn* h, ellm::AttnArgs* a, uint32_t max_po
   if (shape && shape->prefix) {
     const uint32_t own = max_position + 1;
     const ellm::PrefixStep how = ellm::shaped_prefix_step(a->batch, a->n_kv_heads, a->group, own, shape->prefix, a->n_cu);
-    if (how == ellm::PrefixStep::kMixed || (size_t)a->batch * a->n_q_heads > shape->part_rows)
+    if (how == ellm::PrefixStep::kMixed ||
+        (how == ellm::PrefixStep::kApart && (size_t)a->batch * a->n_q_heads > shape->part_rows))
       return ellm::attn_run_shaped(h, *a, stream);
     behind = *shape;
     if (how == ellm::PrefixStep::kWalk) {

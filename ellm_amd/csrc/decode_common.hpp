@@ -149,20 +149,25 @@ __device__ __forceinline__ auto planes_of(const DecodeKernelArgs& p, size_t plan
   }
 }
 
-// A score from a product, in log2 units, by the key's row.
+// A score from a product, in log2 units: that of key row first + r, with what far(first) gives.
 struct PlainScore {
   float scale_log2;
-  __device__ __forceinline__ float operator()(float qk, uint32_t) const { return qk * scale_log2; }
+  __device__ __forceinline__ float far(uint32_t) const { return 0.0f; }
+  __device__ __forceinline__ float operator()(float qk, float, int) const { return qk * scale_log2; }
 };
 template <int SHAPE>
 struct ShapedScore {
   ShapedScores f;
-  float slope2, pos;   // of this lane's head (log2 units); the query's row
-  __device__ __forceinline__ float operator()(float qk, uint32_t key) const {
+  float slope2;   // of this lane's head (log2 units)
+  int32_t pos;    // the query's row
+  __device__ __forceinline__ float far(uint32_t first) const {
+    return (SHAPE & kShapeSlopes) != 0 ? (float)(pos - (int32_t)first) : 0.0f;
+  }
+  __device__ __forceinline__ float operator()(float qk, float far, int r) const {
     float x = qk;
     if constexpr ((SHAPE & kShapeCap) != 0) x = __builtin_amdgcn_rcpf(fast_exp2(x * f.c_in) + 1.0f);
     x = __builtin_fmaf(x, f.a1, f.a0);
-    if constexpr ((SHAPE & kShapeSlopes) != 0) x = __builtin_fmaf(-slope2, fabsf(pos - (float)key), x);
+    if constexpr ((SHAPE & kShapeSlopes) != 0) x = __builtin_fmaf(-slope2, fabsf(far - (float)r), x);
     return x;
   }
 };
@@ -173,7 +178,7 @@ __device__ __forceinline__ auto score_of(const DecodeKernelArgs& p, uint32_t hea
     return PlainScore{p.scale_log2};
   } else {
     const float slope = (SHAPE & kShapeSlopes) != 0 ? p.shape.slopes[head] * kLog2e : 0.0f;
-    return ShapedScore<SHAPE>{p.shape.f, slope, (float)range.pos};
+    return ShapedScore<SHAPE>{p.shape.f, slope, __builtin_amdgcn_readfirstlane(range.pos)};
   }
 }
 
@@ -501,9 +506,10 @@ __device__ __forceinline__ void stream_keys(const Planes& planes, uint32_t k_beg
     }
     float tt[4];
     float tmax = -INFINITY;
+    const float far = score.far(kb + 4 * g);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      tt[r] = (kb + 4 * g + r <= last) ? score(st[r], kb + 4 * g + r) : -INFINITY;
+      tt[r] = (kb + 4 * g + r <= last) ? score(st[r], far, r) : -INFINITY;
       tmax = fmaxf(tmax, tt[r]);
     }
     tmax = fmaxf(tmax, xor_shuffle(tmax, 16));

@@ -61,6 +61,28 @@ def test_many_sequences_with_key_ranges(extra):
     assert empty and torch.count_nonzero(t.out[0, empty]) == 0
 
 
+def test_many_sequences_at_one_position_with_key_ranges():
+    batch, cap, at = 90, 2200, 1999
+    t = Setup(61, BF16, 8, 2, batch, 1, cap)
+    r = random.Random(62)
+    begin, end = [[0] * cap for _ in range(batch)], [[0] * cap for _ in range(batch)]
+    for i in range(batch):
+        lo = r.randrange(at)
+        begin[i][at], end[i][at] = r.choice([(lo, at + 1), (0, at + 1), (lo, lo), (lo, cap), (at, at + 1)])
+    t.op.set_scores(key_begin=_u32(begin, cap), key_end=_u32(end, cap), cap=30.0)
+    t.op.run(at, 1, batch)
+    t.check(t.want([at] * batch, begin=begin, end=end, cap=30.0), "even step")
+
+
+def test_a_short_prefix_of_more_rows_than_room():
+    batch = 2100
+    t = Setup(63, F16, 64, 1, batch, 1, 3, prefix=30)
+    t.op.set_shared_prefix(*t.prefix)
+    t.op.set_scores(slopes=slopes_of(64))
+    t.op.run(2, 1, batch)
+    t.check(t.want([2] * batch, slopes=slopes_of(64)), "one walk")
+
+
 # walk: the prefix of all planes together is small.  mixed: few planes.  apart: many planes, or a large group, or much of
 # the work behind the prefix; the last two rows have more rows than room for their partial results, and a single K/V row each.
 WAYS = [  # query heads, K/V heads, sequences, prefix, longest, scores
