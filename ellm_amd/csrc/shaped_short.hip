@@ -30,6 +30,7 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_short_kernel(ShapedKernelA
   constexpr int kBufs = WR == 1 ? 1 : 2;     // (one wave: its LDS accesses are in order, no second buffer)
   constexpr int kPieces = 8 / WR;            // 16-byte pieces of K, and of V, that a lane moves a turn
   constexpr int kRows = 32 * WR;
+  constexpr int kAhead = 4;                  // LDS operand reads ahead of their products
   // Tiles [group][buffer][K, V][32][128], pieces of a row permuted as in the tile kernel; then sums [group][row][128].
   constexpr int kBytes = kGroups * kBufs * 2 * kTileBytes;
   static_assert(kGroups * kRows * kHeadDim * 4 <= kBytes, "the groups' sums fit in the tiles' room");
@@ -263,8 +264,21 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_short_kernel(ShapedKernelA
     f32x16 st;
 #pragma unroll
     for (int r = 0; r < 16; ++r) st[r] = 0.0f;
+    // operands are read kAhead ahead of the products that take them, those of V ahead of the weights (the scheduling
+    // barriers keep the order as it is written: by itself the compiler reads one, waits, multiplies)
+    u32x4 ring[kAhead];
 #pragma unroll
-    for (int s = 0; s < 8; ++s) st = Mfma<T>::m32x32x16(*(const LdsU32x4*)(ks ^ (32 * s)), qreg[s], st);
+    for (int n = 0; n < kAhead; ++n) ring[n] = *(const LdsU32x4*)(ks ^ (32 * n));
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      st = Mfma<T>::m32x32x16(ring[s % kAhead], qreg[s], st);
+      if (s + kAhead < 8)
+        ring[s % kAhead] = *(const LdsU32x4*)(ks ^ (32 * (s + kAhead)));
+      else
+        ring[s % kAhead] = v_operand(vs, (s + kAhead - 8) >> 2, (s + kAhead - 8) & 3);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     if constexpr (CAP || SLOPES) {
       const float dist = SLOPES ? (float)((int32_t)(pos - kb) - 4 * g) : 0.0f;
 #pragma unroll
@@ -312,10 +326,13 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_short_kernel(ShapedKernelA
       weights(a0 + safe);
     }
     l_run += sum;
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-      for (int db = 0; db < 4; ++db) oacc[db] = Mfma<T>::m32x32x16(v_operand(vs, cc, db), pk[cc], oacc[db]);
+    for (int n = 0; n < 8; ++n) {
+      oacc[n & 3] = Mfma<T>::m32x32x16(ring[n % kAhead], pk[n >> 2], oacc[n & 3]);
+      if (n + kAhead < 8) ring[n % kAhead] = v_operand(vs, (n + kAhead) >> 2, (n + kAhead) & 3);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
 
   // ---- walk ---------------------------------------------------------------------------------------
