@@ -7,10 +7,11 @@
 // Products, masks and references are those of the tile kernel (shaped_chunk.hip): S^T = K . Q^T and O^T += V^T . P^T on
 // 32x32x16 instructions, one key range [lo, hi) a row, references that move where a sum of weights asks for it, values that
 // are not finite multiplied apart where only some rows see them, walks from the last key where scores fall with distance.
-// What bounds it: the chain of turns, 1.1 us each (32 keys: fetch, eight products, scores and weights, eight products), and up
-// to 6 us of launch, start and end.  Capped, binary16, us, tile kernel / this: 33 tokens x 5 on 777, 32 / 4 heads, 19.7 / 14.0; 241
-// tokens 12.7 / 7.3; 16 x 5 on 500, 32 / 32 heads, 19.9 / 11.2; 8 x 5 on 1500 42.2 / 21.9; 618 tokens 24.0 / 17.7; 40 x 2 on 100
-// behind a prefix of 300, 64 / 8 heads, 19.8 / 10.9 (shaped_plan.hpp chooses).  The two kernels of plain scores it stands beside take 11.3, 7.0 and 9.4 us for the first three.
+// What bounds it: the chain of turns, 1.05 us each (32 keys: fetch, eight products, scores and weights, eight products), and up
+// to 6 us of launch, start and end.  Capped, binary16, us, tile kernel / this: 33 tokens x 5 on 777, 32 / 4 heads, 19.7 / 12.9; 241
+// tokens 12.7 / 7.5; 16 x 5 on 500, 32 / 32 heads, 19.9 / 10.6; 8 x 5 on 1500 42.2 / 21.7; 618 tokens 24.0 / 16.8; 40 x 2 on 100
+// behind a prefix of 300, 64 / 8 heads, 19.8 / 10.4 (shaped_plan.hpp chooses).  The two kernels of plain scores it stands beside
+// take 11.2, 7.0 and 9.4 us for the first three; this one without a cap 11.6, 6.9 and 9.2.
 #include "shaped_common.hpp"
 
 namespace ellm {
