@@ -460,7 +460,17 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
     const bool has_k = uniform(s + 1 >= w_begin && s + 1 < w_end) != 0, has_v = uniform(s + 1 > w_begin && s < w_end) != 0;
     const uint32_t vs = opaque(v_read + vbuf * kTileBytes);
     const bool look = t && partly(wg_lo, wg_hi, s);   // (the first turn has no V; the same for all waves)
-    if (look) find_odd(vbuf);
+    if (look) {
+      find_odd(vbuf);
+      meet();
+      if (uniform(s_odd[vbuf])) {
+        if (has_v) add_odd(vs, s);
+        meet();
+        drop_odd(vbuf);
+        if (tid == 0) s_odd[vbuf] = 0;
+        meet();
+      }
+    }
     // Weights against the reference that each row already has: while no lane's sum of them passes kMaxSum the step's
     // maximum is not looked for.  A row without a reference (neg_m = +inf) makes its sums infinite or NaN and so asks for
     // one; so does a score that is not finite.
@@ -475,16 +485,6 @@ __global__ __launch_bounds__(kThreads, 2) void shaped_tile_kernel(ShapedKernelAr
       asm volatile("" : "=v"(st[0]), "=v"(st[1]));   // (whatever the registers hold: nothing comes of it)
     }
     __builtin_amdgcn_s_setprio(1);   // (P.V and the weights ahead of the other workgroup's Q.K: 1 to 9 %)
-    if (look) {
-      meet();
-      if (uniform(s_odd[vbuf])) {
-        if (has_v) add_odd(vs, s);
-        meet();
-        drop_odd(vbuf);
-        if (tid == 0) s_odd[vbuf] = 0;
-        meet();
-      }
-    }
     if (has_v) {
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) ring[n] = v_operand(vs, n >> 2, n & 3);
