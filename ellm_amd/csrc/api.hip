@@ -359,22 +359,24 @@ static bool takes_balanced(const ellm_attn* h, size_t batch, size_t max_position
 }
 
 int ellm::attn_run_single_token(ellm_attn* h, ellm::AttnArgs* a, uint32_t max_position, hipStream_t stream) {
-  const ellm::ShapedState* shape = h->shaped.active() ? &h->shaped : nullptr;
-  ellm::ShapedState behind;   // the shape of a call behind a shared prefix: what the launch over the prefix left
+  ellm::ShapedState state;
+  const ellm::ShapedState* shape = nullptr;
+  if (h->shaped.active()) {
+    state = ellm::shaped_seen(h->shaped, *a);
+    shape = &state;
+  }
   if (shape && shape->prefix) {
-    const uint32_t own = max_position + 1;
+    const uint32_t own = shape->window && shape->window <= max_position ? shape->window : max_position + 1;
     const ellm::PrefixStep how = ellm::shaped_prefix_step(a->batch, a->n_kv_heads, a->group, own, shape->prefix, a->n_cu);
     if (how == ellm::PrefixStep::kMixed ||
         (how == ellm::PrefixStep::kApart && (size_t)a->batch * a->n_q_heads > shape->part_rows))
       return ellm::attn_run_shaped(h, *a, stream);
-    behind = *shape;
     if (how == ellm::PrefixStep::kWalk) {
-      behind.walk_prefix = true;
+      state.walk_prefix = true;
     } else {
-      const hipError_t e = ellm::launch_shaped_prefix(ellm::ShapedArgs{*a, h->shaped}, &behind.prefix_parts, stream);
+      const hipError_t e = ellm::launch_shaped_prefix(ellm::ShapedArgs{*a, state}, &state.prefix_parts, stream);
       if (e != hipSuccess) return fail_hip(e, "attention launch (shared prefix)");
     }
-    shape = &behind;
   }
   if (h->general) {
     const hipError_t e = ellm::launch_attn_general(*a, (uint32_t)h->desc.head_size, stream);

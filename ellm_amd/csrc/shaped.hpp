@@ -39,6 +39,18 @@ struct ShapedState {
   bool active() const { return scores() || prefix; }
 };
 
+// The state that a call sees: prefix rows that the window hides from every one of its queries are left off the front (positions
+// count from the first row that stays: distances and windows are differences), and a prefix of which none stays is none.  With
+// positions on the device the host knows no more than that they are at least 0.
+inline ShapedState shaped_seen(ShapedState s, const AttnArgs& a) {
+  const uint32_t seen = shaped_prefix_seen(s.prefix, s.window, a.positions ? 0u : a.position_index);
+  const size_t hidden = (size_t)(s.prefix - seen) * s.prefix_stride_pos * sizeof(uint16_t);
+  s.prefix = seen;
+  s.prefix_k = seen ? (const char*)s.prefix_k + hidden : nullptr;
+  s.prefix_v = seen ? (const char*)s.prefix_v + hidden : nullptr;
+  return s;
+}
+
 // Scores in the kernels' terms: y = a0 + a1 s, s as above (c_in: what q.k is multiplied by under a cap).
 struct ShapedScores {
   float c_in, a0, a1;
@@ -65,7 +77,7 @@ struct ShapedArgs {
 hipError_t launch_shaped(const ShapedArgs& args, hipStream_t stream);
 // Chunks without a prefix and without positions of their own: 32 wr query rows a workgroup, wr 1 or 2.
 hipError_t launch_shaped_short(const ShapedArgs& args, uint32_t wr, bool along, hipStream_t stream);
-// Single tokens: the shared prefix alone, left as *parts partial results a row (0: no room for them, nothing launched).
+// Single tokens: the shared prefix alone, left as *parts partial results a row.
 hipError_t launch_shaped_prefix(const ShapedArgs& args, uint32_t* parts, hipStream_t stream);
 
 }  // namespace ellm

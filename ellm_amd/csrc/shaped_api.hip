@@ -42,7 +42,7 @@ int prepare(ellm_attn* h) {
 int ellm::attn_run_shaped(ellm_attn* h, const ellm::AttnArgs& a, hipStream_t stream) {
   if ((uint64_t)a.position_interval * a.batch_pitch > 0x7fffffffull / a.n_q_heads)   // (2^39 bytes of queries)
     return ellm::set_error(ELLM_ERR_UNSUPPORTED, "shaped scores and shared prefixes take fewer than 2^31 query rows");
-  const hipError_t e = ellm::launch_shaped(ellm::ShapedArgs{a, h->shaped}, stream);
+  const hipError_t e = ellm::launch_shaped(ellm::ShapedArgs{a, ellm::shaped_seen(h->shaped, a)}, stream);
   if (e != hipSuccess) return ellm::set_error(ELLM_ERR_HIP, "attention launch (shaped scores): %s", hipGetErrorString(e));
   return ELLM_OK;
 }

@@ -680,25 +680,13 @@ hipError_t launch_plan(const ShapedArgs& args, const ShapedPlan& plan, bool merg
 hipError_t launch_shaped(const ShapedArgs& args, hipStream_t stream) {
   const AttnArgs& a = args.a;
   const ShapedState& s = args.s;
-  // keys of a walk as far as the host knows them: the window bounds them, ranges of their own may shorten them
-  uint32_t own_keys = a.position_index + a.position_interval;
-  uint32_t prefix_keys = s.prefix;
-  if (s.window) {
-    // (the positions a workgroup's rows span)
-    const uint32_t span = kShapedRows / a.group + 1;
-    const uint64_t reach = (uint64_t)s.window + (span < a.position_interval ? span : a.position_interval);
-    if (reach < own_keys) {
-      own_keys = (uint32_t)reach;
-    } else if (!a.positions) {   // (own rows of sequences that are shorter than the bound on the host leave more to the prefix)
-      const uint64_t rest = (uint64_t)s.window + a.position_interval - own_keys;
-      if (rest < prefix_keys) prefix_keys = (uint32_t)rest;
-    }
-  }
-  const ShapedPlan plan = shaped_plan(a.position_interval, a.batch, a.n_kv_heads, a.group, own_keys, prefix_keys, a.n_cu, s.part_rows);
+  const ShapedWalks keys = shaped_walks(a.position_index, a.position_interval, a.group, s.prefix, s.window);
+  const ShapedPlan plan = shaped_plan(a.position_interval, a.batch, a.n_kv_heads, a.group, keys.own, s.prefix, a.n_cu, s.part_rows,
+                                      s.window ? keys.both : 0);
   if (!a.positions && (!s.prefix || a.position_interval > 1)) {
     const double end = (double)s.prefix + a.position_index + a.position_interval;
-    ShapedShape c{a.position_interval * a.group, a.batch * a.n_kv_heads, a.n_kv_heads, a.n_cu, (double)own_keys + prefix_keys,
-                  end - 0.5 * a.position_interval, (double)a.position_index + a.position_interval, (double)prefix_keys};
+    ShapedShape c{a.position_interval * a.group, a.batch * a.n_kv_heads, a.n_kv_heads, a.n_cu, (double)keys.both,
+                  end - 0.5 * a.position_interval, (double)a.position_index + a.position_interval, (double)s.prefix, (double)keys.own};
     if (s.window) {
       if (s.window < c.mean) c.mean = s.window;
       if ((double)s.window + a.position_interval < c.rows) c.rows = (double)s.window + a.position_interval;
@@ -712,14 +700,7 @@ hipError_t launch_shaped(const ShapedArgs& args, hipStream_t stream) {
 hipError_t launch_shaped_prefix(const ShapedArgs& args, uint32_t* parts, hipStream_t stream) {
   const AttnArgs& a = args.a;
   const ShapedState& s = args.s;
-  *parts = 0;
-  uint32_t seen = s.prefix;   // prefix rows that the window leaves, as far as the host knows
-  if (s.window && !a.positions) {
-    if (s.window <= a.position_index + 1) return hipSuccess;
-    const uint32_t rest = s.window - 1 - a.position_index;
-    seen = rest < seen ? rest : seen;
-  }
-  const ShapedPlan plan = shaped_prefix_plan(a.batch, a.n_kv_heads, a.group, seen, a.n_cu, s.part_rows);
+  const ShapedPlan plan = shaped_prefix_plan(a.batch, a.n_kv_heads, a.group, s.prefix, a.n_cu, s.part_rows);
   if (plan.n_part == 0) return hipErrorInvalidValue;
   *parts = plan.n_part;
   return launch_plan(args, plan, false, stream);

@@ -69,8 +69,32 @@ inline size_t shaped_part_rows(size_t interval, size_t batch, size_t q_heads, ui
   return rows * 4 * n_cu < most ? rows * 4 * n_cu : most;
 }
 
+// Rows of a prefix that any query of a call sees: what the window leaves to the first of them, at own row `first`.
+inline uint32_t shaped_prefix_seen(uint32_t prefix, uint32_t window, uint32_t first) {
+  if (!window) return prefix;
+  const uint32_t left = window - 1 > first ? window - 1 - first : 0u;
+  return left < prefix ? left : prefix;
+}
+
+// Keys that the longest walks of a call read, as far as the host knows them (ranges of their own may shorten them): over a
+// sequence's own rows, over the prefix (the rows that are seen of it) and own rows together.
+struct ShapedWalks {
+  uint32_t own, both;
+};
+inline ShapedWalks shaped_walks(uint32_t position, uint32_t interval, uint32_t group, uint32_t prefix, uint32_t window) {
+  ShapedWalks w{position + interval, prefix + position + interval};
+  if (window) {
+    const uint32_t span = kShapedRows / group + 1;   // the positions that a workgroup's rows span
+    const uint64_t reach = (uint64_t)window + (span < interval ? span : interval);
+    if (reach < w.own) w.own = (uint32_t)reach;
+    if (reach < w.both) w.both = (uint32_t)reach;
+  }
+  return w;
+}
+
+// (both_keys: ShapedWalks::both; 0: own_keys + prefix)
 inline ShapedPlan shaped_plan(uint32_t interval, uint32_t batch, uint32_t n_kv_heads, uint32_t group, uint32_t own_keys,
-                              uint32_t prefix, uint32_t n_cu, size_t part_rows) {
+                              uint32_t prefix, uint32_t n_cu, size_t part_rows, uint32_t both_keys = 0) {
   ShapedPlan p{};
   p.rows_plane = interval * group;
   p.tiles_plane = shaped_ceil(p.rows_plane, kShapedRows);
@@ -100,7 +124,9 @@ inline ShapedPlan shaped_plan(uint32_t interval, uint32_t batch, uint32_t n_kv_h
     p.prefix_rows = p.prefix_tiles = p.prefix_split = 0;
     p.n_split = 1;
   }
-  p.n_split = shaped_split(own_steps + prefix_steps, walks, shaped_slots(walks * (own_steps + prefix_steps), n_cu), rows, false);
+  uint32_t steps = own_steps + prefix_steps;
+  if (both_keys && shaped_ceil(both_keys, kShapedKeys) < steps) steps = shaped_ceil(both_keys, kShapedKeys);
+  p.n_split = shaped_split(steps, walks, shaped_slots((uint64_t)walks * steps, n_cu), rows, false);
   if (rows * p.n_split > part_rows) p.n_split = (uint32_t)(part_rows / rows);
   if (p.n_split == 0) p.n_split = 1;
   p.n_part = p.n_split;
@@ -116,6 +142,7 @@ struct ShapedShape {
   uint32_t rows_plane, planes, n_kv_heads, n_cu;
   double longest, mean, rows;   // (rows: of a sequence's own)
   double prefix;                // of those keys, as far as the window leaves them
+  double own = 0.0;             // keys of the longest walk over own rows alone (0: longest - prefix)
   double steps(double walks, double seen, double keys) const { return walks * (seen / keys + 1); }
   double units() const { return 256.0 / n_cu; }
   double stream_us() const { return (planes * rows + n_kv_heads * prefix) * 512 / 6.5e6; }
@@ -128,7 +155,8 @@ inline double shaped_tile_us(const ShapedShape& c, const ShapedPlan& p) {
   const double apart = p.prefix_tiles ? c.prefix : 0.0;   // keys that packed rows of all sequences walk
   const double wgs = walks * p.n_split + ahead * p.prefix_split;
   const double work = (0.0083 * wgs + 0.0045 * (c.steps(walks, c.mean - apart, kShapedKeys) + c.steps(ahead, apart, kShapedKeys))) * c.units();
-  uint32_t longest = shaped_ceil(shaped_ceil((uint64_t)(c.longest - apart), kShapedKeys), p.n_split);
+  const double own = p.prefix_tiles ? (c.own > 0.0 ? c.own : c.longest - apart) : c.longest;
+  uint32_t longest = shaped_ceil(shaped_ceil((uint64_t)own, kShapedKeys), p.n_split);
   if (p.prefix_tiles) {
     const uint32_t other = shaped_ceil(shaped_ceil((uint64_t)apart, kShapedKeys), p.prefix_split);
     longest = other > longest ? other : longest;
