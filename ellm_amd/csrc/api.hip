@@ -367,7 +367,8 @@ int ellm::attn_run_single_token(ellm_attn* h, ellm::AttnArgs* a, uint32_t max_po
   }
   if (shape && shape->prefix) {
     const uint32_t own = shape->window && shape->window <= max_position ? shape->window : max_position + 1;
-    const ellm::PrefixStep how = ellm::shaped_prefix_step(a->batch, a->n_kv_heads, a->group, own, shape->prefix, a->n_cu);
+    const ellm::PrefixStep how = ellm::shaped_prefix_step(a->batch, a->n_kv_heads, a->group, own, shape->prefix, a->n_cu,
+                                                              a->positions != nullptr);
     if (how == ellm::PrefixStep::kMixed ||
         (how == ellm::PrefixStep::kApart && (size_t)a->batch * a->n_q_heads > shape->part_rows))
       return ellm::attn_run_shaped(h, *a, stream);

@@ -197,11 +197,20 @@ inline bool shaped_short_along(uint32_t planes, double rows) {
 //   32 / 32, 8,  8000,    40:    154 /  31.2 /  31.4      64 / 8, 64,  8000,    40: 218.9 /  42.3 /  36.2
 //   64 / 8, 24,  2000,  4000:      - /  64.5 /  66.5      64 / 8, 24,  2000, 24000:     - / 314.3 / 237.0
 //   32 / 32, 24, 2000,    40:   95.8 /  28.1 /  18.7      64 / 8, 128, 32000, 4000:     - / 572.4 / 369.4
+// A walk is cut into equal splits for the longest sequence.  Where lengths are uneven (positions on the device: the host knows
+// the longest only), planes too few to even it out by their number and own rows long, that costs more than a launch over
+// the prefix ahead of equal shares of the own rows (us, without a prefix / walk / apart; sequences, prefix, own rows):
+//   32 / 4, 24,   100, 500-30000:   85 / 148 /  97        32 / 4,  8,  1000,   100-8000:  22.0 / 26.0 / 31.9
+//   64 / 8, 20,  1000, 500-30000:  188 / 253 / 204         8 / 1,100,  1500,    50-4000:  24.4 / 35.4 / 39.7
+//   32 / 4, 16,  2500, 500-16000:   47 /  83 /  64        32 /32,  8,   300,   100-1500:  29.0 / 33.6 / 42.7
+//   32 / 4, 64,   600,  100-3000:   38 /  61 /  54        64 / 8, 64,   300,    64-2000:  46.9 / 52.0 / 62.4 (512 planes)
+//   32 / 4, 32,   100,  100-4000:   27 /  41 /  39        32 / 4,  2,  2000, 1000-131072: 80.8 / 82.6 / 93.0 (nearly even)
 enum class PrefixStep { kWalk, kMixed, kApart };
 inline PrefixStep shaped_prefix_step(uint32_t batch, uint32_t n_kv_heads, uint32_t group, uint32_t own_keys, uint32_t prefix,
-                                     uint32_t n_cu) {
+                                     uint32_t n_cu, bool uneven = false) {
   const uint64_t planes = (uint64_t)batch * n_kv_heads;
-  if (planes * prefix <= 640 * (uint64_t)n_cu) return PrefixStep::kWalk;
+  if (planes * prefix <= 640 * (uint64_t)n_cu)
+    return uneven && planes < 2 * (uint64_t)n_cu && planes * own_keys >= 1792 * (uint64_t)n_cu ? PrefixStep::kApart : PrefixStep::kWalk;
   const uint64_t own_steps = planes * shaped_ceil(own_keys, kShapedKeys);
   return group <= kShapedRows / 2 && planes <= n_cu && own_steps <= 48 * (uint64_t)n_cu ? PrefixStep::kMixed : PrefixStep::kApart;
 }

@@ -65,3 +65,23 @@ def test_a_window_that_hides_a_part_of_the_prefix(dtype, hq, hkv, batch, prefix,
         first = [i * start // batch for i in range(batch)]
         t.op.run_ragged(torch.tensor(first, dtype=torch.int32, device="cuda"), start, batch)
         t.check(t.want(first, **scores), "ragged")
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,batch,prefix,longest,scores", [
+    (F16, 32, 4, 24, 100, 5000, dict(cap=30.0)),
+    (BF16, 16, 8, 20, 333, 4000, dict(slopes=True)),
+    (F16, 8, 1, 200, 65, 3000, dict(window=2900)),
+    (F16, 80, 2, 70, 1, 4000, dict()),
+])
+def test_a_short_prefix_ahead_of_long_uneven_own_rows(dtype, hq, hkv, batch, prefix, longest, scores):
+    t = Setup(73, dtype, hq, hkv, batch, 1, longest + 1, prefix=prefix)
+    scores = dict(scores, slopes=slopes_of(hq) if scores.get("slopes") else None)
+    t.op.set_scores(**scores)
+    t.op.set_shared_prefix(*t.prefix)
+    first = [(i * i * longest) // (batch * batch) for i in range(batch)]
+    first[batch // 2] = longest - 1
+    positions = torch.tensor(first, dtype=torch.int32, device="cuda")
+    for _ in range(2):
+        t.out.fill_(7.0)
+        t.op.run_ragged(positions, longest - 1, batch)
+        t.check(t.want(first, **scores), "uneven own rows")

@@ -78,3 +78,21 @@ int main() {
   return 0;
 }
 """)
+
+
+def test_a_short_prefix_ahead_of_long_uneven_own_rows_is_not_walked(tmp_path):
+    run_probe(tmp_path, r"""
+int main() {
+  // sequences, K/V heads, group, own keys, prefix
+  CHECK(shaped_prefix_step(24, 4, 8, 30000, 100, 256, true) == PrefixStep::kApart);
+  CHECK(shaped_prefix_step(20, 8, 8, 30000, 1000, 256, true) == PrefixStep::kApart);
+  CHECK(shaped_prefix_step(64, 4, 8, 3000, 600, 256, true) == PrefixStep::kApart);
+  CHECK(shaped_prefix_step(24, 4, 8, 30000, 100, 256, false) == PrefixStep::kWalk);   // even
+  CHECK(shaped_prefix_step(8, 4, 8, 8000, 1000, 256, true) == PrefixStep::kWalk);     // too little to share out
+  CHECK(shaped_prefix_step(4, 4, 8, 500, 2000, 256, true) == PrefixStep::kWalk);
+  CHECK(shaped_prefix_step(64, 8, 8, 2000, 300, 256, true) == PrefixStep::kWalk);     // planes that even it out
+  CHECK(shaped_prefix_step(24, 4, 8, 1000, 999, 256, true) == PrefixStep::kWalk);     // (all a window of 1000 leaves)
+  printf("done\n");
+  return 0;
+}
+""")
