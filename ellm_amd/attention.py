@@ -176,6 +176,10 @@ class Attention:
         check(self._lib.ellm_attn_set_shared_prefix(self._handle, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), length))
         self._prefix = (k, v)
 
+    def _shaped(self):
+        """Whether shaped scores or a shared prefix are set."""
+        return self._lib.ellm_attn_ragged_path(self._handle, 0, 1) == 2
+
     def run(self, position_index, position_interval, batch_size, cpu_num=1, thread_id=0,
             stream=None):
         if thread_id != 0:
@@ -199,7 +203,10 @@ class Attention:
 
     def run_noalloc(self, position, batch_size, positions=None, stream=None):
         """The single-token step through ellm_attn_run_noalloc: this operator's description,
-        the library's static device scratch instead of the handle's workspace."""
+        the library's static device scratch instead of the handle's workspace.  It knows nothing of
+        shaped scores or a shared prefix: refused while either is set."""
+        if self._shaped():
+            raise ValueError("run_noalloc computes plain scores over a sequence's own rows only")
         pos_ptr = _positions_ptr(positions, batch_size) if positions is not None else None
         check(self._lib.ellm_attn_run_noalloc(ctypes.byref(self.desc), pos_ptr, int(position),
                                               batch_size, _stream_ptr(stream)))

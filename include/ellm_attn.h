@@ -192,7 +192,8 @@ int ellm_attn_ragged_path(const ellm_attn* handle, size_t max_position, size_t b
  * Same kernel and split plan as ellm_attn_run and as the ellm_attn_run_ragged calls for which
  * ellm_attn_ragged_path returns 0, so those results are bit-identical (the kernel for large
  * calls with per-sequence positions, path 1, splits the keys differently: same tolerance,
- * other bits).
+ * other bits).  It has a description and no handle: shaped scores and shared prefixes
+ * (ellm_attn_set_scores, ellm_attn_set_shared_prefix) are a handle's and take no part here.
  * The split partials and arrival counters live in a static device array of 5,074,944
  * bytes that every device the library runs on holds until the process ends; the call
  * uses the current device's copy.  Limit: sequences x query heads x splits <= 8192

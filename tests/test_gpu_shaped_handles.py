@@ -1,0 +1,36 @@
+"""What a handle with shaped scores or a shared prefix keeps, refuses and allocates."""
+import pytest
+import torch
+
+import ellm_amd
+from shaped_util import slopes_of
+from test_gpu_shaped_scores import F16, Setup
+
+pytestmark = pytest.mark.gpu
+
+
+def test_the_call_without_a_handle_is_refused_while_scores_or_a_prefix_are_set():
+    """It reads the description alone, so it would compute the plain operator."""
+    t = Setup(81, F16, 8, 2, 2, 1, 64, prefix=16)
+    t.op.run(40, 1, 2)
+    torch.cuda.synchronize()
+    plain = t.out.clone()
+
+    def taken():
+        t.out.fill_(7.0)
+        t.op.run_noalloc(40, 2)
+        torch.cuda.synchronize()
+        return torch.equal(t.out, plain)
+
+    assert taken()
+    for on, off in ((lambda: t.op.set_scores(cap=30.0), t.op.set_scores), (lambda: t.op.set_scores(window=5), t.op.set_scores),
+                    (lambda: t.op.set_scores(slopes=slopes_of(8)), t.op.set_scores),
+                    (lambda: t.op.set_shared_prefix(*t.prefix), t.op.set_shared_prefix)):
+        on()
+        t.out.fill_(7.0)
+        with pytest.raises(ValueError):
+            t.op.run_noalloc(40, 2)
+        torch.cuda.synchronize()
+        assert (t.out == 7.0).all()
+        off()
+        assert taken()
