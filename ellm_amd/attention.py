@@ -125,11 +125,15 @@ class Attention:
         import torch
 
         d = self.desc
+        window = int(window)
         if window < 0:
             raise ValueError(f"a window of {window} positions")
+        window = min(window, 1 << 32)   # (beyond every position, and within the C type)
+        if cap != 0 and ctypes.c_float(cap).value == 0.0:
+            raise ValueError(f"a cap of {cap} is zero in 32 bits, which would be none")
         if slopes is not None:
-            if not slopes.is_contiguous():
-                raise ValueError("slopes must be contiguous")
+            if not slopes.is_contiguous() or slopes.numel() < d.attention_head_num:
+                raise ValueError(f"slopes must be contiguous, one for each of {d.attention_head_num} query heads")
             _device_buffer("slopes", slopes, d.attention_head_num, torch.float32)
         pitch = 0
         for name, bound in (("key_begin", key_begin), ("key_end", key_end)):
@@ -146,7 +150,7 @@ class Attention:
             pitch = bound.stride(0)
             _device_buffer(name, bound, (d.batch_size - 1) * pitch + d.sequence_capacity)
         ptr = [t.data_ptr() if t is not None else None for t in (slopes, key_begin, key_end)]
-        check(self._lib.ellm_attn_set_scores(self._handle, ctypes.c_float(cap), ptr[0], int(window), ptr[1], ptr[2], pitch))
+        check(self._lib.ellm_attn_set_scores(self._handle, ctypes.c_float(cap), ptr[0], window, ptr[1], ptr[2], pitch))
         self._scores = (slopes, key_begin, key_end)
 
     def set_shared_prefix(self, k=None, v=None, length=None):

@@ -34,3 +34,21 @@ def test_the_call_without_a_handle_is_refused_while_scores_or_a_prefix_are_set()
         assert (t.out == 7.0).all()
         off()
         assert taken()
+
+
+def test_arguments_that_the_c_types_would_change():
+    """A window past 64 bits is a window past every key; a cap that 32 bits hold as zero, or a view of fewer slopes than
+    heads in a longer buffer, is refused and nothing of it stays."""
+    t = Setup(82, F16, 8, 2, 2, 1, 64)
+    for window in (1 << 32, (1 << 64) + 5, 1 << 100):
+        t.op.set_scores(window=window)
+        t.op.run(40, 1, 2)
+        t.check(t.want([40, 40]), f"window {window}")
+    t.op.set_scores()
+    for bad in (dict(cap=1e-50), dict(cap=-1e-60), dict(slopes=slopes_of(16)[:7])):
+        with pytest.raises(ValueError):
+            t.op.set_scores(**bad)
+        assert t.op.ragged_path(40, 2) != 2
+    t.op.set_scores(slopes=slopes_of(16)[:8])
+    t.op.run(40, 1, 2)
+    t.check(t.want([40, 40], slopes=slopes_of(16)[:8]), "the first of a longer buffer")
