@@ -10,8 +10,8 @@ namespace {
 
 bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
-// What both set functions ask of a handle; the room for partial results, taken at the first of them.
-int prepare(ellm_attn* h) {
+// What both set functions ask of a handle; the room for partial results, taken at the first that sets anything (`on`).
+int prepare(ellm_attn* h, bool on) {
   if (!h) return ellm::set_error(ELLM_ERR_INVALID_ARGUMENT, "null handle");
   if (int st = ellm::check_current_device(h->device)) return st;
   if (h->general)
@@ -20,7 +20,7 @@ int prepare(ellm_attn* h) {
     return ellm::set_error(ELLM_ERR_INVALID_ARGUMENT, "inverse_sqrt_head %g is too large for shaped scores",
                            (double)h->desc.inverse_sqrt_head);
   ellm::ShapedState& s = h->shaped;
-  if (s.part_o) return ELLM_OK;
+  if (!on || s.part_o) return ELLM_OK;
   const ellm_attn_desc& d = h->desc;
   const size_t rows = ellm::shaped_part_rows(d.max_position_interval, d.batch_size, d.attention_head_num, (uint32_t)h->n_cu);
   float *o = nullptr, *ml = nullptr;
@@ -64,7 +64,7 @@ int ellm_attn_set_scores(ellm_attn* h, float score_cap, const float* distance_sl
                            bounds_pitch, h->desc.sequence_capacity);
   if ((key_begin || key_end) && h->shaped.prefix)
     return ellm::set_error(ELLM_ERR_UNSUPPORTED, "key ranges do not go with a shared prefix");
-  if (int st = prepare(h)) return st;
+  if (int st = prepare(h, score_cap != 0.0f || distance_slopes || window || key_begin || key_end)) return st;
   ellm::ShapedState& s = h->shaped;
   s.cap = score_cap;
   s.slopes = distance_slopes;
@@ -97,7 +97,7 @@ int ellm_attn_set_shared_prefix(ellm_attn* h, const void* k, const void* v, size
     if (h->shaped.key_begin || h->shaped.key_end)
       return ellm::set_error(ELLM_ERR_UNSUPPORTED, "key ranges do not go with a shared prefix");
   }
-  if (int st = prepare(h)) return st;
+  if (int st = prepare(h, length != 0)) return st;
   ellm::ShapedState& s = h->shaped;
   s.prefix = (uint32_t)length;
   s.prefix_k = length ? k : nullptr;

@@ -1,4 +1,6 @@
 """What a handle with shaped scores or a shared prefix keeps, refuses and allocates."""
+import gc
+
 import pytest
 import torch
 
@@ -52,3 +54,25 @@ def test_arguments_that_the_c_types_would_change():
     t.op.set_scores(slopes=slopes_of(16)[:8])
     t.op.run(40, 1, 2)
     t.check(t.want([40, 40], slopes=slopes_of(16)[:8]), "the first of a longer buffer")
+
+
+def test_setters_that_set_nothing_take_no_room():
+    """A handle that never had scores or a prefix keeps its memory when they are set to none; the first that sets
+    anything takes the room for partial results once."""
+    t = Setup(83, F16, 32, 4, 4, 64, 128, prefix=16)
+    gc.collect()
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    t.op.set_scores()
+    t.op.set_shared_prefix()
+    t.op.set_shared_prefix(*t.prefix, 0)
+    assert torch.cuda.mem_get_info()[0] == free
+    t.op.set_scores(cap=30.0)
+    after = torch.cuda.mem_get_info()[0]
+    assert 0 < free - after <= 80 << 20
+    t.op.set_shared_prefix(*t.prefix)
+    t.op.set_scores()
+    t.op.set_shared_prefix()
+    assert torch.cuda.mem_get_info()[0] == after
+    t.op.run(3, 64, 4)
+    torch.cuda.synchronize()
