@@ -12,7 +12,7 @@ computes with torch.
 """
 import ctypes
 
-from . import _lib
+from . import _lib, schedule
 from ._lib import AttnDesc, KvDesc, KvRaggedDesc, KvSeqTable, check, load_library
 
 
@@ -104,7 +104,7 @@ class Attention:
         d.sequence_capacity = cap
         d.max_position_interval = interval
         self.desc = d
-        self._scores = self._prefix = None   # tensors that the handle reads
+        self._scores = self._prefix = ()   # tensors that the handle reads
         self._handle = ctypes.c_void_p()
         if seq_table is not None:
             check(self._lib.ellm_attn_create_ragged(ctypes.byref(d), ctypes.byref(seq_table.table),
@@ -121,7 +121,9 @@ class Attention:
         position p and the key at position j becomes cap tanh(x / cap) - slopes[head] |p - j|, and the query sees the
         keys key_begin[sequence, p] <= j < key_end[sequence, p] with p - j < window.  slopes: float32 device tensor, one
         a query head; key_begin, key_end: uint32/int32 device tensors [batch, positions], positions at least the
-        capacity (None: 0 and p + 1).  Without arguments: the plain operator again."""
+        capacity (None: 0 and p + 1).  Without arguments: the plain operator again.
+        The tensors are read by every run, and kept until they are replaced; a StepGraph recorded meanwhile keeps them until
+        it is closed.  Runs on other streams, and graphs recorded by other means, have to be done with them before that."""
         import torch
 
         d = self.desc
@@ -157,10 +159,10 @@ class Attention:
         """A prefix that all sequences share, ahead of their own rows, for the runs from here on
         (ellm_attn_set_shared_prefix).  k, v: device tensors [kv_head, position, 128] (any view whose last dimension is
         contiguous), of which the first `length` positions count (None: all of them); runs count positions from the
-        prefix's end.  Without arguments: no prefix."""
+        prefix's end.  Without arguments: no prefix.  Kept as the tensors of set_scores are."""
         if k is None and v is None:
             check(self._lib.ellm_attn_set_shared_prefix(self._handle, None, None, 0, 0, 0))
-            self._prefix = None
+            self._prefix = ()
             return
         d = self.desc
         for name, t in (("k", k), ("v", v)):
@@ -184,16 +186,21 @@ class Attention:
         """Whether shaped scores or a shared prefix are set."""
         return self._lib.ellm_attn_ragged_path(self._handle, 0, 1) == 2
 
+    def _launching(self):
+        """The C handle, for a launch that reads the tensors of both setters."""
+        schedule.keep_while_recorded(*self._scores, *self._prefix)
+        return self._handle
+
     def run(self, position_index, position_interval, batch_size, cpu_num=1, thread_id=0,
             stream=None):
         if thread_id != 0:
             return  # the launch is enqueued once, by thread 0
-        check(self._lib.ellm_attn_run(self._handle, position_index, position_interval, batch_size,
+        check(self._lib.ellm_attn_run(self._launching(), position_index, position_interval, batch_size,
                                       _stream_ptr(stream)))
 
     def run_ragged(self, positions, max_position, batch_size, stream=None):
         """Single-token step; positions: uint32/int32 device tensor, one entry per sequence."""
-        check(self._lib.ellm_attn_run_ragged(self._handle, _positions_ptr(positions, batch_size),
+        check(self._lib.ellm_attn_run_ragged(self._launching(), _positions_ptr(positions, batch_size),
                                              int(max_position), batch_size, _stream_ptr(stream)))
 
     def ragged_path(self, max_position, batch_size):
@@ -367,11 +374,11 @@ class KVCache:
         vs = ctypes.c_void_p(_device_buffer("v_src", v_src, need, k_src.dtype))
         rp = ctypes.c_void_p(_device_buffer("rope", rope, rope.shape[0] * 128, k_src.dtype))
         if positions is None:
-            check(self._lib.ellm_kv_append_attn_run(self._handle, layer, attention._handle, position_index, batch_size,
+            check(self._lib.ellm_kv_append_attn_run(self._handle, layer, attention._launching(), position_index, batch_size,
                                                     ks, vs, rp, rope.shape[0], ctypes.c_float(eps), _stream_ptr(stream)))
         else:
             check(self._lib.ellm_kv_append_attn_run_ragged(
-                self._handle, layer, attention._handle, _positions_ptr(positions, batch_size), int(max_position),
+                self._handle, layer, attention._launching(), _positions_ptr(positions, batch_size), int(max_position),
                 batch_size, ks, vs, rp, rope.shape[0], ctypes.c_float(eps), _stream_ptr(stream)))
 
     def close(self):

@@ -85,10 +85,10 @@ class MatMul3:
         by attention.run(position, 1, batch) leaves, with the head rows finished by the attention
         launch.  positions: per-sequence device positions, position_index then their upper bound."""
         if positions is None:
-            check(self._lib.ellm_matmul3_attn_run(self._handle, attention._handle, int(position_index),
+            check(self._lib.ellm_matmul3_attn_run(self._handle, attention._launching(), int(position_index),
                                                   batch_size, _stream_ptr(stream)))
         else:
-            check(self._lib.ellm_matmul3_attn_run_ragged(self._handle, attention._handle,
+            check(self._lib.ellm_matmul3_attn_run_ragged(self._handle, attention._launching(),
                                                          _positions_ptr(positions, batch_size),
                                                          int(position_index), batch_size, _stream_ptr(stream)))
 

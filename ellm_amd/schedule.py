@@ -78,19 +78,34 @@ class SideStream:
             pass
 
 
+_recording = []   # the StepGraphs between begin and end
+
+
+def keep_while_recorded(*tensors):
+    """What the launch of a run reads now: the graphs that are being recorded keep it, whatever replaces it later."""
+    for graph in _recording:
+        for t in tensors:
+            if t is not None and not any(t is x for x in graph._keep):
+                graph._keep.append(t)
+
+
 class StepGraph:
-    """with StepGraph(stream) as g: <launches on `stream`> ; then g.launch() per step."""
+    """with StepGraph(stream) as g: <launches on `stream`> ; then g.launch() per step.  The graph keeps the tensors that
+    Attention.set_scores / set_shared_prefix had handed to the operators it records, until close."""
 
     def __init__(self, stream):
         self._lib = load_library()
         self._stream = stream
         self._handle = ctypes.c_void_p()
+        self._keep = []
 
     def __enter__(self):
         check(self._lib.ellm_graph_begin(ctypes.c_void_p(self._stream.cuda_stream)))
+        _recording.append(self)
         return self
 
     def __exit__(self, exc_type, exc, tb):
+        _recording.remove(self)
         handle = ctypes.c_void_p()
         status = self._lib.ellm_graph_end(ctypes.c_void_p(self._stream.cuda_stream),
                                           ctypes.byref(handle))
@@ -109,6 +124,7 @@ class StepGraph:
         if self._handle:
             check(self._lib.ellm_graph_destroy(self._handle))
             self._handle = ctypes.c_void_p()
+        self._keep = []
 
     def __del__(self):
         try:

@@ -232,7 +232,8 @@ int ellm_attn_run_noalloc(const ellm_attn_desc* desc, const uint32_t* positions,
  * A row that sees no key is 0, its lse -infinity.  Keys and values that a row does not see may hold anything, infinities
  * and NaN included.  All arguments 0 / NULL: the plain operator again.  Takes handles with head_size 128 and 16-bit
  * storage (else ELLM_ERR_UNSUPPORTED).  The arrays are read by every run, not copied.  Host-side: takes effect with the
- * next run; a recorded graph keeps what its runs were recorded with.  The first of this call and
+ * next run; a recorded graph keeps the addresses and values its runs were recorded with (the memory is the caller's to
+ * keep until the last replay).  The first of this call and
  * ellm_attn_set_shared_prefix that sets anything on a handle allocates room for the partial results of split walks (at
  * most 68 MB, kept until destroy), so it belongs ahead of a recording.  The reference has no counterpart (its leaf knows the scaled
  * product and the causal bound only, src/kernel/generic/flash_attention.rs:60-89).
