@@ -96,3 +96,22 @@ int main() {
   return 0;
 }
 """)
+
+
+def test_chunks_of_many_planes_are_dealt_along_their_tiles(tmp_path):
+    """The calls that the GPU tests make for the sake of that order."""
+    run_probe(tmp_path, r"""
+static uint32_t along(uint32_t hq, uint32_t hkv, uint32_t batch, uint32_t start, uint32_t interval, uint32_t prefix) {
+  const uint32_t group = hq / hkv, own = start + interval, keys = prefix + own;
+  const ShapedPlan p = shaped_plan(interval, batch, hkv, group, own, prefix, 256, shaped_part_rows(interval, batch, hq, 256));
+  const uint32_t wr = shaped_short_rows({interval * group, batch * hkv, hkv, 256, (double)keys, keys - 0.5 * interval, (double)own,
+                                         (double)prefix}, p);
+  return shaped_short_along(batch * hkv, keys) ? wr : 0;
+}
+int main() {
+  CHECK(along(32, 4, 9, 300, 16, 0) == 1 && along(8, 8, 9, 2100, 5, 0) == 1 && along(36, 9, 5, 300, 5, 50) == 1);
+  CHECK(along(8, 1, 37, 30, 33, 0) == 2 && along(8, 1, 33, 30, 45, 50) == 2);
+  printf("done\n");
+  return 0;
+}
+""")
