@@ -121,7 +121,8 @@ class Attention:
         position p and the key at position j becomes cap tanh(x / cap) - slopes[head] |p - j|, and the query sees the
         keys key_begin[sequence, p] <= j < key_end[sequence, p] with p - j < window.  slopes: float32 device tensor, one
         a query head; key_begin, key_end: uint32/int32 device tensors [batch, positions], positions at least the
-        capacity (None: 0 and p + 1).  Without arguments: the plain operator again.
+        capacity (None: 0 and p + 1); int32 entries are read as unsigned, so -1 is past every key (as key_begin: no key, as
+        key_end: up to the capacity, whose rows must then have been written).  Without arguments: the plain operator again.
         The tensors are read by every run, and kept until they are replaced; a StepGraph recorded meanwhile keeps them until
         it is closed.  Runs on other streams, and graphs recorded by other means, have to be done with them before that."""
         import torch

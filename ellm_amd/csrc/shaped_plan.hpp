@@ -148,8 +148,8 @@ struct ShapedShape {
   double stream_us() const { return (planes * rows + n_kv_heads * prefix) * 512 / 6.5e6; }
 };
 inline double shaped_longest(double a, double b, double c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); }
-// Estimated (measured): 250 tokens, 32 / 4 heads, 12.4 (12.5); 1000 x 8 102 (101); 250 x 24 on 1000 146 (148); 8 on 4000, 31 splits,
-// 14.8 (15.5); behind a prefix of 1000, 9 x 8, 64 / 8 heads, 17.3 (19.2); 9 x 24 on 100, 32 / 32 heads, 29.6 (33.3).
+// Estimated (measured): 250 tokens, 32 / 4 heads, 12.4 (12.4); 1000 x 8 102 (104); 250 x 24 on 1000 146 (152); 8 on 4000, 31 splits,
+// 14.8 (15.4); behind a prefix of 1000, 9 x 8, 64 / 8 heads, 17.3 (19.1); 9 x 24 on 100, 32 / 32 heads, 29.6 (33.3).
 inline double shaped_tile_us(const ShapedShape& c, const ShapedPlan& p) {
   const double walks = c.planes * (double)p.tiles_plane, ahead = c.n_kv_heads * (double)p.prefix_tiles;
   const double apart = p.prefix_tiles ? c.prefix : 0.0;   // keys that packed rows of all sequences walk
@@ -164,8 +164,8 @@ inline double shaped_tile_us(const ShapedShape& c, const ShapedPlan& p) {
   const double partials = p.n_part > 1 ? 3.5 + 7.4e-5 * c.planes * (double)c.rows_plane * p.n_part : 0.0;
   return (5.0 + shaped_longest(0.8 + 1.65 * longest, work, c.stream_us()) + partials) * (p.prefix_tiles ? 0.914 : 1.0);
 }
-// wr = 1: 500 tokens, 32 / 4 heads, 12.9 (11.8); 33 x 5 on 800 15.2 (13.0); 250 x 24 on 1000 271 (268); 40 x 2 on 100 behind 300, 64 / 8
-// heads, 11.3 (10.3); wr = 2: 500 tokens 18.2 (15.3); 1000 x 8 138 (134); 33 x 24 on 800 29.0 (29.0).
+// wr = 1: 500 tokens, 32 / 4 heads, 12.9 (11.4); 33 x 5 on 800 15.2 (13.0); 250 x 24 on 1000 271 (255); 40 x 2 on 100 behind 300, 64 / 8
+// heads, 11.3 (10.4); wr = 2: 500 tokens 18.2 (15.3); 1000 x 8 138 (132); 33 x 24 on 800 29.0 (28.7).
 inline double shaped_short_us(const ShapedShape& c, uint32_t wr) {
   const double wgs = c.planes * (double)shaped_ceil(c.rows_plane, 32 * wr), tiles = c.steps(wgs * wr, c.mean, 32);
   const double work = (wr == 1 ? 0.0068 * wgs + 0.00103 * tiles : 0.0052 * wgs + 0.00084 * tiles) * c.units();
@@ -173,8 +173,8 @@ inline double shaped_short_us(const ShapedShape& c, uint32_t wr) {
   return 5.0 + shaped_longest(chain, work, c.stream_us() * (wr == 1 ? 1.0 : 1.02)) + (wr == 1 ? 0.0 : 0.1);
 }
 // Blocks of 32 rows a workgroup of the short-walk kernel, 1 or 2; 0: the tile kernel, unless it is estimated 5 % slower.  Over
-// those calls the choice is on average 0.6 % behind the best of the three and at most 7 % behind the tile kernel; against that
-// kernel alone: 33 x 5 on 800 20.0 -> 13.0, 250 tokens 12.5 -> 7.5, 500 19.1 -> 11.8, 16 x 5 on 500, 32 / 32 heads, 19.9 -> 10.8, 40 x 2 on 100
+// those calls the choice was on average 0.6 % behind the best of the three; over 65 others and the kernels as they are now 1.4 %
+// (capped), 2.4 % (scores as they are) and 1.9 % (slopes), at worst 28 %.  Against the tile kernel alone: 33 x 5 on 800 20.0 -> 13.0, 250 tokens 12.5 -> 7.5, 500 19.1 -> 11.8, 16 x 5 on 500, 32 / 32 heads, 19.9 -> 10.8, 40 x 2 on 100
 // behind 300, 64 / 8 heads, 19.7 -> 10.3.
 inline uint32_t shaped_short_rows(const ShapedShape& c, const ShapedPlan& plan) {
   const double tile = 1.047 * shaped_tile_us(c, plan), one = shaped_short_us(c, 1), two = shaped_short_us(c, 2);

@@ -228,7 +228,9 @@ int ellm_attn_run_noalloc(const ellm_attn_desc* desc, const uint32_t* positions,
  *                     (bounds_pitch >= sequence_capacity), or NULL: 0 and p + 1.  They say which keys the query at that
  *                     position sees, later ones too: documents packed into a sequence (begin of the document, p + 1), a
  *                     prefix that all of its own positions see (0, max(p + 1, prefix length)), padding (0, 0).  key_end
- *                     counts up to the sequence's capacity; keys it admits must have been written.
+ *                     counts up to the sequence's capacity; keys it admits must have been written.  Entries are unsigned:
+ *                     a -1 stored there is 2^32 - 1, as key_begin past every key (the row sees none), as key_end the
+ *                     capacity.
  * A row that sees no key is 0, its lse -infinity.  Keys and values that a row does not see may hold anything, infinities
  * and NaN included.  All arguments 0 / NULL: the plain operator again.  Takes handles with head_size 128 and 16-bit
  * storage (else ELLM_ERR_UNSUPPORTED).  The arrays are read by every run, not copied.  Host-side: takes effect with the
