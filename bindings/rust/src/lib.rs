@@ -243,6 +243,41 @@ extern "C" {
         kv_strides: *mut usize, // [4]
         table: *mut ellm_kv_seq_table,
     ) -> c_int;
+    pub fn ellm_kv_create_e4m3(desc: *const ellm_kv_desc, out_cache: *mut *mut ellm_kv_cache) -> c_int;
+    pub fn ellm_kv_create_ragged_e4m3(
+        desc: *const ellm_kv_ragged_desc,
+        out_cache: *mut *mut ellm_kv_cache,
+    ) -> c_int;
+    pub fn ellm_kv_layer_e4m3(
+        cache: *const ellm_kv_cache,
+        layer: usize,
+        first_sequence: usize,
+        k: *mut *mut c_void,
+        v: *mut *mut c_void,
+        k_scale: *mut *mut u8,
+        v_scale: *mut *mut u8,
+        kv_strides: *mut usize,
+        table: *mut ellm_kv_seq_table,
+    ) -> c_int;
+    pub fn ellm_kv_read_e4m3(
+        cache: *const ellm_kv_cache,
+        layer: usize,
+        first_sequence: usize,
+        position_index: usize,
+        n_tokens: usize,
+        batch_size: usize,
+        k_dst: *mut c_void,
+        v_dst: *mut c_void,
+        dst_strides: *const usize,
+        stream: Stream,
+    ) -> c_int;
+    pub fn ellm_attn_create_e4m3(
+        desc: *const ellm_attn_desc,
+        k_scale: *const u8,
+        v_scale: *const u8,
+        table: *const ellm_kv_seq_table,
+        out_handle: *mut *mut ellm_attn,
+    ) -> c_int;
     pub fn ellm_kv_append(
         cache: *mut ellm_kv_cache,
         layer: usize,

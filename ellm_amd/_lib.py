@@ -139,6 +139,12 @@ ABI_SYMBOLS = {
     "ellm_kv_layer_ragged": (ctypes.c_int, [_vp, _sz, _sz, _pvp, _pvp, ctypes.POINTER(_sz * 4),
                                             ctypes.POINTER(KvSeqTable)]),
     "ellm_attn_create_ragged": (ctypes.c_int, [ctypes.POINTER(AttnDesc), ctypes.POINTER(KvSeqTable), _pvp]),
+    "ellm_kv_create_e4m3": (ctypes.c_int, [ctypes.POINTER(KvDesc), _pvp]),
+    "ellm_kv_create_ragged_e4m3": (ctypes.c_int, [ctypes.POINTER(KvRaggedDesc), _pvp]),
+    "ellm_kv_layer_e4m3": (ctypes.c_int, [_vp, _sz, _sz, _pvp, _pvp, _pvp, _pvp, ctypes.POINTER(_sz * 4),
+                                          ctypes.POINTER(KvSeqTable)]),
+    "ellm_kv_read_e4m3": (ctypes.c_int, [_vp, _sz, _sz, _sz, _sz, _sz, _vp, _vp, ctypes.POINTER(_sz * 3), _vp]),
+    "ellm_attn_create_e4m3": (ctypes.c_int, [ctypes.POINTER(AttnDesc), _vp, _vp, ctypes.POINTER(KvSeqTable), _pvp]),
     "ellm_matmul3_create_ragged": (ctypes.c_int, [ctypes.POINTER(MatMul3Desc), ctypes.POINTER(KvSeqTable),
                                                   _pvp]),
     "ellm_kv_destroy": (ctypes.c_int, [_vp]),

@@ -67,17 +67,21 @@ class Attention:
     k, v:   any 4-d view [sequence, kv_head, position, head_size] (strides are passed on)
     float16 / bfloat16 tensors with head_size 128 run the MFMA kernels; other head sizes up to
     256 and float32 tensors run kernels of their own (same arguments and results).
+    kv_scales = (k_scale, v_scale): k and v are planes in 8 bits (a KVCache made with e4m3=True, or any
+    in its format): float8_e4m3fn tensors, whose rows' scales are float8_e8m0fnu tensors laid out as the
+    rows are (the scale of the row that begins at element x is element x / 128); q is float16 or bfloat16.
     """
 
     def __init__(self, q, k, v, out, batch_size, attention_head_num, kv_head_num, head_size,
                  kv_strides, inverse_sqrt_head, lse=None, sequence_capacity=None,
-                 max_position_interval=None, seq_table=None):
-        """seq_table: a KVCache.layer_ragged(...) view, for a cache whose sequences have different
-        capacities (then kv_strides[0] and sequence_capacity are not used)."""
+                 max_position_interval=None, seq_table=None, kv_scales=None):
+        """seq_table: a KVCache.layer_ragged(...) or layer_e4m3(...) view, for a cache whose sequences have
+        different capacities (then kv_strides[0] and sequence_capacity are not used)."""
         import torch
 
         self._lib = load_library()
-        self._keep = (q, k, v, out, lse, seq_table)
+        self._keep = (q, k, v, out, lse, seq_table, kv_scales)
+        self._e4m3 = kv_scales is not None
         interval = int(max_position_interval if max_position_interval is not None else q.shape[0])
         rows = interval * batch_size * attention_head_num
         if seq_table is not None:
@@ -90,8 +94,12 @@ class Attention:
         d = AttnDesc()
         d.q = _device_buffer("q", q, rows * head_size)
         d.out = _device_buffer("out", out, rows * head_size, q.dtype)
-        d.k = _device_buffer("k", k, kv_span, q.dtype)
-        d.v = _device_buffer("v", v, kv_span, q.dtype)
+        kv_type = torch.float8_e4m3fn if self._e4m3 else q.dtype
+        d.k = _device_buffer("k", k, kv_span, kv_type)
+        d.v = _device_buffer("v", v, kv_span, kv_type)
+        if self._e4m3:
+            scales = [_device_buffer(name, t, (kv_span + 127) // 128, torch.float8_e8m0fnu)
+                      for name, t in zip(("k_scale", "v_scale"), kv_scales)]
         d.lse = _device_buffer("lse", lse, rows, torch.float32) if lse is not None else None
         d.batch_size = batch_size
         d.attention_head_num = attention_head_num
@@ -100,13 +108,16 @@ class Attention:
         for i in range(4):
             d.kv_strides[i] = int(kv_strides[i])
         d.inverse_sqrt_head = float(inverse_sqrt_head)
-        d.dtype = _dtype_code(q, allow_f32=True)
+        d.dtype = _dtype_code(q, allow_f32=not self._e4m3)
         d.sequence_capacity = cap
         d.max_position_interval = interval
         self.desc = d
         self._scores = self._prefix = ()   # tensors that the handle reads
         self._handle = ctypes.c_void_p()
-        if seq_table is not None:
+        if self._e4m3:
+            table = ctypes.byref(seq_table.table) if seq_table is not None else None
+            check(self._lib.ellm_attn_create_e4m3(ctypes.byref(d), *scales, table, ctypes.byref(self._handle)))
+        elif seq_table is not None:
             check(self._lib.ellm_attn_create_ragged(ctypes.byref(d), ctypes.byref(seq_table.table),
                                                     ctypes.byref(self._handle)))
         else:
@@ -216,7 +227,9 @@ class Attention:
     def run_noalloc(self, position, batch_size, positions=None, stream=None):
         """The single-token step through ellm_attn_run_noalloc: this operator's description,
         the library's static device scratch instead of the handle's workspace.  It knows nothing of
-        shaped scores or a shared prefix: refused while either is set."""
+        shaped scores, a shared prefix or planes in 8 bits: refused with any of them."""
+        if self._e4m3:
+            raise ValueError("run_noalloc reads planes of 16-bit rows only")
         if self._shaped():
             raise ValueError("run_noalloc computes plain scores over a sequence's own rows only")
         pos_ptr = _positions_ptr(positions, batch_size) if positions is not None else None
@@ -255,20 +268,37 @@ class RaggedLayerView:
                    for i in range(batch_size))
 
 
+class E4m3LayerView:
+    """One layer of a cache in 8 bits, from sequence `first_sequence` on: addresses of codes and scales, strides,
+    and for a cache with a capacity for each sequence (`table` not None) the sequence table."""
+
+    def __init__(self, cache, addresses, strides, table, first_sequence):
+        self.cache, self.strides, self.table, self.first_sequence = cache, strides, table, first_sequence
+        self.k, self.v, self.k_scale, self.v_scale = addresses
+        if table is not None:
+            self.capacities = cache.capacities[first_sequence:]
+            self.offsets = cache.offsets[first_sequence:]
+
+    span_elems = RaggedLayerView.span_elems
+
+
 class KVCache:
     """Keys and values of every layer in one allocation each: [layer][sequence][kv_head]
     [position][128] with one capacity, or (KVCache.ragged) [layer][kv_head][sequence: its own
-    positions][128] with a capacity per sequence."""
+    positions][128] with a capacity per sequence.  e4m3: rows in 8 bits (ellm_kv_create_e4m3), 128 e4m3 codes
+    and an e8m0 scale each; dtype_code is then the type of the rows that append* take and read gives."""
 
     def __init__(self, layers, sequences, kv_head_num, capacity, dtype_code, head_size=128,
-                 capacities=None):
+                 capacities=None, e4m3=False):
         self._lib = load_library()
         self._handle = ctypes.c_void_p()
         self.capacities = None
+        self.e4m3 = bool(e4m3)
         if capacities is None:
             d = KvDesc(layers, sequences, kv_head_num, head_size, capacity, dtype_code)
             self.desc = d
-            check(self._lib.ellm_kv_create(ctypes.byref(d), ctypes.byref(self._handle)))
+            create = self._lib.ellm_kv_create_e4m3 if e4m3 else self._lib.ellm_kv_create
+            check(create(ctypes.byref(d), ctypes.byref(self._handle)))
             return
         caps = (ctypes.c_size_t * len(capacities))(*[int(c) for c in capacities])
         rd = KvRaggedDesc(layers, len(capacities), kv_head_num, head_size, caps, dtype_code)
@@ -276,11 +306,12 @@ class KVCache:
         self.capacities = [int(c) for c in capacities]
         self.offsets = [128 * sum(self.capacities[:i]) for i in range(len(capacities))]
         self.layer_elems = 128 * sum(self.capacities) * kv_head_num
-        check(self._lib.ellm_kv_create_ragged(ctypes.byref(rd), ctypes.byref(self._handle)))
+        create = self._lib.ellm_kv_create_ragged_e4m3 if e4m3 else self._lib.ellm_kv_create_ragged
+        check(create(ctypes.byref(rd), ctypes.byref(self._handle)))
 
     @classmethod
-    def ragged(cls, layers, capacities, kv_head_num, dtype_code, head_size=128):
-        return cls(layers, len(capacities), kv_head_num, 0, dtype_code, head_size, capacities=capacities)
+    def ragged(cls, layers, capacities, kv_head_num, dtype_code, head_size=128, e4m3=False):
+        return cls(layers, len(capacities), kv_head_num, 0, dtype_code, head_size, capacities=capacities, e4m3=e4m3)
 
     def layer_ragged(self, layer, first_sequence=0):
         k, v = ctypes.c_void_p(), ctypes.c_void_p()
@@ -329,6 +360,64 @@ class KVCache:
 
         return wrap(k), wrap(v)
 
+    def layer_e4m3(self, layer, first_sequence=0):
+        """One layer of a cache in 8 bits: what Attention takes beside its tensors (seq_table, strides)."""
+        found = [ctypes.c_void_p() for _ in range(4)]
+        strides = (ctypes.c_size_t * 4)()
+        table = KvSeqTable() if self.capacities is not None else None
+        check(self._lib.ellm_kv_layer_e4m3(self._handle, layer, first_sequence, *(ctypes.byref(x) for x in found),
+                                           ctypes.byref(strides), ctypes.byref(table) if table is not None else None))
+        return E4m3LayerView(self, [x.value for x in found], list(strides), table, first_sequence)
+
+    def layer_e4m3_tensors(self, layer):
+        """Borrow one layer of a cache in 8 bits as torch tensors: (k, v, k_scale, v_scale), float8_e4m3fn
+        [sequence, kv_head, position, 128] and float8_e8m0fnu [sequence, kv_head, position]; with a capacity for each
+        sequence [kv_head, positions of all sequences, 128] and [kv_head, positions of all sequences].  The cache lives
+        as long as any of them does, unless it is closed."""
+        import torch
+
+        view, d = self.layer_e4m3(layer), self.desc
+        shape = (d.sequences, d.kv_head_num, d.capacity) if self.capacities is None else (d.kv_head_num, sum(self.capacities))
+
+        def wrap(ptr, shape, dtype):
+            n = 1
+            for x in shape:
+                n *= x
+            iface = {"shape": (n,), "typestr": "|u1", "data": (ptr, False), "version": 2}
+            holder = type("DevBuf", (), {"__cuda_array_interface__": iface, "cache": self})()   # (the tensor keeps the holder)
+            return torch.as_tensor(holder, device="cuda").view(dtype).view(shape)
+
+        return tuple([wrap(p, (*shape, d.head_size), torch.float8_e4m3fn) for p in (view.k, view.v)]
+                     + [wrap(p, shape, torch.float8_e8m0fnu) for p in (view.k_scale, view.v_scale)])
+
+    def _row_type(self):
+        """The torch type of the rows that a cache in 8 bits takes; None: rows of a 16-bit cache, stored as they come."""
+        import torch
+
+        if not self.e4m3:
+            return None
+        return torch.float16 if self.desc.dtype == _lib.DTYPE_F16 else torch.bfloat16
+
+    def read(self, layer, position_index, k_dst, v_dst, first_sequence=0, stream=None):
+        """Rows of a cache in 8 bits as 16-bit values (ellm_kv_read_e4m3): positions position_index .. + n_tokens - 1 of
+        sequences first_sequence .. + batch - 1 into k_dst / v_dst, device tensors [n_tokens, batch, kv_head, 128] of the
+        cache's dtype; any strides (the same of both) that keep rows contiguous."""
+        n_tokens, batch, heads, width = k_dst.shape
+        dtype = self._row_type()
+        if heads != self.desc.kv_head_num or width != self.desc.head_size or v_dst.shape != k_dst.shape:
+            raise ValueError(f"k_dst and v_dst must be [tokens, sequences, {self.desc.kv_head_num}, {self.desc.head_size}], "
+                             f"got {tuple(k_dst.shape)} and {tuple(v_dst.shape)}")
+        if n_tokens == 0 or batch == 0:
+            return
+        if k_dst.stride(3) != 1 or k_dst.stride() != v_dst.stride():
+            raise ValueError("k_dst and v_dst must have the same strides and contiguous rows")
+        strides = (ctypes.c_size_t * 3)(*k_dst.stride()[:3])
+        span = sum((n - 1) * s for n, s in zip(k_dst.shape, k_dst.stride())) + 1
+        check(self._lib.ellm_kv_read_e4m3(self._handle, layer, first_sequence, position_index, n_tokens, batch,
+                                          ctypes.c_void_p(_device_buffer("k_dst", k_dst, span, dtype)),
+                                          ctypes.c_void_p(_device_buffer("v_dst", v_dst, span, dtype)),
+                                          ctypes.byref(strides), _stream_ptr(stream)))
+
     def append(self, layer, position_index, k_src, v_src, batch_size=None, stream=None):
         """k_src / v_src: [n_tokens, src_batch_pitch, kv_head, 128] device tensors."""
         n_tokens, pitch = k_src.shape[0], k_src.shape[1]
@@ -336,7 +425,7 @@ class KVCache:
             batch_size = pitch
         need = n_tokens * pitch * self.desc.kv_head_num * self.desc.head_size
         check(self._lib.ellm_kv_append(self._handle, layer, position_index, n_tokens, batch_size,
-                                       ctypes.c_void_p(_device_buffer("k_src", k_src, need)),
+                                       ctypes.c_void_p(_device_buffer("k_src", k_src, need, self._row_type())),
                                        ctypes.c_void_p(_device_buffer("v_src", v_src, need, k_src.dtype)),
                                        pitch, _stream_ptr(stream)))
 
@@ -353,7 +442,7 @@ class KVCache:
         need = n_tokens * pitch * self.desc.kv_head_num * self.desc.head_size
         check(self._lib.ellm_kv_append_norm_rope(
             self._handle, layer, position_index, n_tokens, batch_size,
-            ctypes.c_void_p(_device_buffer("k_src", k_src, need)),
+            ctypes.c_void_p(_device_buffer("k_src", k_src, need, self._row_type())),
             ctypes.c_void_p(_device_buffer("v_src", v_src, need, k_src.dtype)), pitch,
             ctypes.c_void_p(_device_buffer("rope", rope, rope.shape[0] * 128, k_src.dtype)),
             rope.shape[0], ctypes.c_float(eps), pos_ptr, int(max_position), _stream_ptr(stream)))
@@ -371,7 +460,7 @@ class KVCache:
         if batch_size > pitch:
             raise ValueError(f"batch_size {batch_size} exceeds the {pitch} rows of k_src")
         need = pitch * self.desc.kv_head_num * self.desc.head_size
-        ks = ctypes.c_void_p(_device_buffer("k_src", k_src, need))
+        ks = ctypes.c_void_p(_device_buffer("k_src", k_src, need, self._row_type()))
         vs = ctypes.c_void_p(_device_buffer("v_src", v_src, need, k_src.dtype))
         rp = ctypes.c_void_p(_device_buffer("rope", rope, rope.shape[0] * 128, k_src.dtype))
         if positions is None:

@@ -144,10 +144,11 @@ void ellm::attn_args_from_desc(const ellm_attn_desc& d, ellm::AttnArgs* a) {
   a->seq_offsets = nullptr;
   a->seq_caps = nullptr;
   a->pending = ellm::PendingRows{};
+  a->k_scale = a->v_scale = nullptr;
 }
 
 struct ellm_kv_cache {
-  ellm_kv_desc desc;   // capacity = the largest per-sequence capacity
+  ellm_kv_desc desc;   // capacity = the largest per-sequence capacity; dtype: in 8 bits, that of the rows written and read
   int device;
   void* k;
   void* v;
@@ -162,6 +163,15 @@ struct ellm_kv_cache {
   std::vector<size_t> offsets_host;   // [sequences], elements
   size_t* seq_offsets_dev;            // ragged only
   uint32_t* seq_caps_dev;             // ragged only
+  // rows in 8 bits (ellm_kv_create_e4m3): k and v hold codes, one byte an element, and every row has a scale here
+  uint8_t* k_scale;                   // null: 16-bit rows
+  uint8_t* v_scale;
+  void* layer_k(size_t layer) const { return (char*)k + layer * layer_elems * (k_scale ? 1 : 2); }
+  void* layer_v(size_t layer) const { return (char*)v + layer * layer_elems * (k_scale ? 1 : 2); }
+  ellm::KvE4m3 layer_e4m3(size_t layer) const {
+    const size_t rows = layer * (layer_elems / 128);
+    return ellm::KvE4m3{(uint8_t*)layer_k(layer), (uint8_t*)layer_v(layer), k_scale + rows, v_scale + rows};
+  }
   ellm::KvLayout layout(size_t first_sequence = 0) const {
     ellm::KvLayout l;
     l.stride_seq = stride_seq;
@@ -169,6 +179,10 @@ struct ellm_kv_cache {
     l.seq_offsets = ragged ? seq_offsets_dev + first_sequence : nullptr;
     l.seq_caps = ragged ? seq_caps_dev + first_sequence : nullptr;
     return l;
+  }
+  ellm_kv_seq_table table(size_t first_sequence) const {   // (ragged)
+    return ellm_kv_seq_table{seq_offsets_dev + first_sequence, seq_caps_dev + first_sequence,
+                             caps_host.data() + first_sequence, desc.sequences - first_sequence};
   }
   // the smallest / largest capacity among sequences [0, n)
   size_t min_cap(size_t n) const {
@@ -220,7 +234,8 @@ int ellm_device_count(void) {
   return usable;
 }
 
-static int attn_create(const ellm_attn_desc* d, const ellm_kv_seq_table* table, ellm_attn** out_handle) {
+static int attn_create(const ellm_attn_desc* d, const ellm_kv_seq_table* table, ellm_attn** out_handle,
+                       const uint8_t* k_scale = nullptr, const uint8_t* v_scale = nullptr) {
   if (!d || !out_handle) return fail(ELLM_ERR_INVALID_ARGUMENT, "null descriptor or handle pointer");
   *out_handle = nullptr;
   ellm_attn_desc local;
@@ -240,10 +255,18 @@ static int attn_create(const ellm_attn_desc* d, const ellm_kv_seq_table* table, 
       cap = table->seq_capacity_host[i] > cap ? table->seq_capacity_host[i] : cap;
     }
     local.sequence_capacity = cap;
-    if (local.kv_strides[0] == 0) local.kv_strides[0] = 8;
+    if (local.kv_strides[0] == 0 || k_scale) local.kv_strides[0] = 128;
     d = &local;
   }
   if (int st = ellm::validate_attn_desc(d)) return st;
+  if (k_scale) {
+    if (ellm::attn_is_general(*d))
+      return fail(ELLM_ERR_UNSUPPORTED, "planes in 8 bits take head_size 128 and a 16-bit dtype of q and out only");
+    for (int i = 0; i < 3; ++i)   // (a row's scale is found from where its codes are)
+      if (d->kv_strides[i] % 128 != 0)
+        return fail(ELLM_ERR_INVALID_ARGUMENT, "kv_strides[%d] = %zu must be a multiple of 128 for planes in 8 bits", i,
+                    d->kv_strides[i]);
+  }
 
   int device = 0, n_cu = 0;
   int st = ellm::current_gfx950_device(&device, &n_cu);
@@ -257,6 +280,8 @@ static int attn_create(const ellm_attn_desc* d, const ellm_kv_seq_table* table, 
   h->n_cu = n_cu;
   h->seq_offsets = nullptr;
   h->seq_caps = nullptr;
+  h->k_scale = k_scale;
+  h->v_scale = v_scale;
   if (table) {
     h->seq_offsets = table->seq_offsets;
     h->seq_caps = table->seq_capacity;
@@ -315,6 +340,13 @@ int ellm_attn_create_ragged(const ellm_attn_desc* d, const ellm_kv_seq_table* ta
   return attn_create(d, table, out_handle);
 }
 
+int ellm_attn_create_e4m3(const ellm_attn_desc* d, const uint8_t* k_scale, const uint8_t* v_scale,
+                          const ellm_kv_seq_table* table, ellm_attn** out_handle) {
+  if (out_handle) *out_handle = nullptr;
+  if (!k_scale || !v_scale) return fail(ELLM_ERR_INVALID_ARGUMENT, "k_scale and v_scale must be non-null device pointers");
+  return attn_create(d, table, out_handle, k_scale, v_scale);
+}
+
 int ellm_attn_reset(ellm_attn* h, void* stream) {
   if (!h) return fail(ELLM_ERR_INVALID_ARGUMENT, "null handle");
   if (int st = ellm::check_current_device(h->device)) return st;
@@ -346,6 +378,8 @@ void ellm::attn_fill_args(const ellm_attn* h, ellm::AttnArgs* a) {
   a->n_cu = (uint32_t)h->n_cu;
   a->seq_offsets = h->seq_offsets;
   a->seq_caps = h->seq_caps;
+  a->k_scale = h->k_scale;
+  a->v_scale = h->v_scale;
 }
 
 // sequences of different lengths: equal shares of all keys; two workgroups per compute unit are
@@ -440,8 +474,11 @@ int ellm_attn_run(ellm_attn* h, size_t position_index, size_t position_interval,
   a.batch = (uint32_t)batch_size;
   if (position_interval == 1) return ellm::attn_run_single_token(h, &a, (uint32_t)position_index, (hipStream_t)stream);
   if (h->shaped.active()) return ellm::attn_run_shaped(h, a, (hipStream_t)stream);
-  hipError_t e = h->general ? ellm::launch_attn_general(a, (uint32_t)d.head_size, (hipStream_t)stream)
-                            : ellm::launch_prefill(a, (hipStream_t)stream);
+  if (h->k_scale && (uint64_t)position_interval * d.batch_size > 0x7fffffffull / d.attention_head_num)
+    return fail(ELLM_ERR_UNSUPPORTED, "chunks over planes in 8 bits take fewer than 2^31 query rows");
+  hipError_t e = h->general   ? ellm::launch_attn_general(a, (uint32_t)d.head_size, (hipStream_t)stream)
+                 : h->k_scale ? ellm::launch_chunk_e4m3(a, (hipStream_t)stream)
+                              : ellm::launch_prefill(a, (hipStream_t)stream);
   if (e != hipSuccess) return fail_hip(e, "chunk attention launch");
   return ELLM_OK;
 }
@@ -485,7 +522,7 @@ int ellm_attn_ragged_path(const ellm_attn* h, size_t max_position, size_t batch_
 // uniform -> [sequence][kv_head][position][128] with one capacity, else
 // [kv_head][sequence: its own positions][128] with offset / capacity tables on the device.
 static int kv_create(size_t layers, size_t kv_head_num, size_t head_size, int dtype,
-                     const std::vector<size_t>& caps, bool ragged, ellm_kv_cache** out_cache) {
+                     const std::vector<size_t>& caps, bool ragged, bool e4m3, ellm_kv_cache** out_cache) {
   if (dtype != ELLM_DTYPE_F16 && dtype != ELLM_DTYPE_BF16)
     return fail(ELLM_ERR_INVALID_ARGUMENT, "dtype %d is neither ELLM_DTYPE_F16 nor ELLM_DTYPE_BF16", dtype);
   if (head_size != 128)
@@ -509,6 +546,7 @@ static int kv_create(size_t layers, size_t kv_head_num, size_t head_size, int dt
       __builtin_mul_overflow(layer_elems, layers, &bytes) ||
       __builtin_mul_overflow(bytes, (size_t)2, &bytes))
     return fail(ELLM_ERR_UNSUPPORTED, "the cache's size in bytes does not fit 64 bits");
+  if (e4m3) bytes /= 2;
   int device = 0, n_cu = 0;
   int st = ellm::current_gfx950_device(&device, &n_cu);
   if (st != ELLM_OK) return st;
@@ -523,6 +561,7 @@ static int kv_create(size_t layers, size_t kv_head_num, size_t head_size, int dt
   c->caps_host = caps;
   c->offsets_host.resize(sequences);
   c->k = c->v = nullptr;
+  c->k_scale = c->v_scale = nullptr;
   c->seq_offsets_dev = nullptr;
   c->seq_caps_dev = nullptr;
   if (ragged) {
@@ -542,6 +581,12 @@ static int kv_create(size_t layers, size_t kv_head_num, size_t head_size, int dt
   if (e == hipSuccess) e = hipMalloc(&c->v, bytes);
   if (e == hipSuccess) e = hipMemset(c->k, 0, bytes);
   if (e == hipSuccess) e = hipMemset(c->v, 0, bytes);
+  if (e == hipSuccess && e4m3) {
+    e = hipMalloc((void**)&c->k_scale, bytes / 128);
+    if (e == hipSuccess) e = hipMalloc((void**)&c->v_scale, bytes / 128);
+    if (e == hipSuccess) e = hipMemset(c->k_scale, 0, bytes / 128);
+    if (e == hipSuccess) e = hipMemset(c->v_scale, 0, bytes / 128);
+  }
   if (e == hipSuccess && ragged) {
     std::vector<uint32_t> caps32(caps.begin(), caps.end());
     e = hipMalloc((void**)&c->seq_offsets_dev, sequences * sizeof(size_t));
@@ -554,6 +599,8 @@ static int kv_create(size_t layers, size_t kv_head_num, size_t head_size, int dt
   if (e != hipSuccess) {
     if (c->k) (void)hipFree(c->k);
     if (c->v) (void)hipFree(c->v);
+    if (c->k_scale) (void)hipFree(c->k_scale);
+    if (c->v_scale) (void)hipFree(c->v_scale);
     if (c->seq_offsets_dev) (void)hipFree(c->seq_offsets_dev);
     if (c->seq_caps_dev) (void)hipFree(c->seq_caps_dev);
     delete c;
@@ -563,7 +610,7 @@ static int kv_create(size_t layers, size_t kv_head_num, size_t head_size, int dt
   return ELLM_OK;
 }
 
-int ellm_kv_create(const ellm_kv_desc* d, ellm_kv_cache** out_cache) {
+static int kv_create_uniform(const ellm_kv_desc* d, bool e4m3, ellm_kv_cache** out_cache) {
   if (!d || !out_cache) return fail(ELLM_ERR_INVALID_ARGUMENT, "null descriptor or cache pointer");
   *out_cache = nullptr;
   if (d->sequences > 65535) return fail(ELLM_ERR_UNSUPPORTED, "capacity / sequences / kv_head_num too large");
@@ -577,23 +624,34 @@ int ellm_kv_create(const ellm_kv_desc* d, ellm_kv_cache** out_cache) {
   if (d->head_size != 128)
     return fail(ELLM_ERR_UNSUPPORTED, "head_size %zu: only 128 is supported", d->head_size);
   const std::vector<size_t> caps(d->sequences, d->capacity);
-  return kv_create(d->layers, d->kv_head_num, d->head_size, d->dtype, caps, false, out_cache);
+  return kv_create(d->layers, d->kv_head_num, d->head_size, d->dtype, caps, false, e4m3, out_cache);
 }
 
-int ellm_kv_create_ragged(const ellm_kv_ragged_desc* d, ellm_kv_cache** out_cache) {
+static int kv_create_uneven(const ellm_kv_ragged_desc* d, bool e4m3, ellm_kv_cache** out_cache) {
   if (!d || !out_cache) return fail(ELLM_ERR_INVALID_ARGUMENT, "null descriptor or cache pointer");
   *out_cache = nullptr;
   if (!d->capacities) return fail(ELLM_ERR_INVALID_ARGUMENT, "null capacities");
   if (d->sequences == 0 || d->sequences > 65535)
     return fail(d->sequences ? ELLM_ERR_UNSUPPORTED : ELLM_ERR_INVALID_ARGUMENT, "sequences %zu out of range", d->sequences);
   const std::vector<size_t> caps(d->capacities, d->capacities + d->sequences);
-  return kv_create(d->layers, d->kv_head_num, d->head_size, d->dtype, caps, true, out_cache);
+  return kv_create(d->layers, d->kv_head_num, d->head_size, d->dtype, caps, true, e4m3, out_cache);
+}
+
+int ellm_kv_create(const ellm_kv_desc* d, ellm_kv_cache** out_cache) { return kv_create_uniform(d, false, out_cache); }
+int ellm_kv_create_e4m3(const ellm_kv_desc* d, ellm_kv_cache** out_cache) { return kv_create_uniform(d, true, out_cache); }
+int ellm_kv_create_ragged(const ellm_kv_ragged_desc* d, ellm_kv_cache** out_cache) {
+  return kv_create_uneven(d, false, out_cache);
+}
+int ellm_kv_create_ragged_e4m3(const ellm_kv_ragged_desc* d, ellm_kv_cache** out_cache) {
+  return kv_create_uneven(d, true, out_cache);
 }
 
 int ellm_kv_destroy(ellm_kv_cache* c) {
   if (!c) return ELLM_OK;
   hipError_t e1 = hipFree(c->k);
   hipError_t e2 = hipFree(c->v);
+  if (c->k_scale) (void)hipFree(c->k_scale);
+  if (c->v_scale) (void)hipFree(c->v_scale);
   if (c->seq_offsets_dev) (void)hipFree(c->seq_offsets_dev);
   if (c->seq_caps_dev) (void)hipFree(c->seq_caps_dev);
   delete c;
@@ -604,13 +662,14 @@ int ellm_kv_destroy(ellm_kv_cache* c) {
 
 int ellm_kv_layer(const ellm_kv_cache* c, size_t layer, void** k, void** v, size_t kv_strides[4]) {
   if (!c || !k || !v || !kv_strides) return fail(ELLM_ERR_INVALID_ARGUMENT, "null argument");
+  if (c->k_scale) return fail(ELLM_ERR_INVALID_ARGUMENT, "the cache's rows are in 8 bits: use ellm_kv_layer_e4m3");
   if (c->ragged)
     return fail(ELLM_ERR_INVALID_ARGUMENT,
                 "this cache has per-sequence capacities: no single sequence stride exists, use ellm_kv_layer_ragged");
   if (layer >= c->desc.layers)
     return fail(ELLM_ERR_OUT_OF_RANGE, "layer %zu of %zu", layer, c->desc.layers);
-  *k = (char*)c->k + layer * c->layer_elems * 2;
-  *v = (char*)c->v + layer * c->layer_elems * 2;
+  *k = c->layer_k(layer);
+  *v = c->layer_v(layer);
   kv_strides[0] = c->stride_seq;
   kv_strides[1] = c->stride_head;
   kv_strides[2] = c->desc.head_size;
@@ -621,22 +680,44 @@ int ellm_kv_layer(const ellm_kv_cache* c, size_t layer, void** k, void** v, size
 int ellm_kv_layer_ragged(const ellm_kv_cache* c, size_t layer, size_t first_sequence, void** k, void** v,
                          size_t kv_strides[4], ellm_kv_seq_table* table) {
   if (!c || !k || !v || !kv_strides || !table) return fail(ELLM_ERR_INVALID_ARGUMENT, "null argument");
+  if (c->k_scale) return fail(ELLM_ERR_INVALID_ARGUMENT, "the cache's rows are in 8 bits: use ellm_kv_layer_e4m3");
   if (!c->ragged)
     return fail(ELLM_ERR_INVALID_ARGUMENT, "this cache has one capacity for every sequence: use ellm_kv_layer");
   if (layer >= c->desc.layers)
     return fail(ELLM_ERR_OUT_OF_RANGE, "layer %zu of %zu", layer, c->desc.layers);
   if (first_sequence >= c->desc.sequences)
     return fail(ELLM_ERR_OUT_OF_RANGE, "first_sequence %zu of %zu", first_sequence, c->desc.sequences);
-  *k = (char*)c->k + layer * c->layer_elems * 2;
-  *v = (char*)c->v + layer * c->layer_elems * 2;
+  *k = c->layer_k(layer);
+  *v = c->layer_v(layer);
   kv_strides[0] = c->layer_elems;   // not used with a table (every sequence has its own offset)
   kv_strides[1] = c->stride_head;
   kv_strides[2] = c->desc.head_size;
   kv_strides[3] = 1;
-  table->seq_offsets = c->seq_offsets_dev + first_sequence;
-  table->seq_capacity = c->seq_caps_dev + first_sequence;
-  table->seq_capacity_host = c->caps_host.data() + first_sequence;
-  table->sequences = c->desc.sequences - first_sequence;
+  *table = c->table(first_sequence);
+  return ELLM_OK;
+}
+
+int ellm_kv_layer_e4m3(const ellm_kv_cache* c, size_t layer, size_t first_sequence, void** k, void** v, uint8_t** k_scale,
+                       uint8_t** v_scale, size_t kv_strides[4], ellm_kv_seq_table* table) {
+  if (!c || !k || !v || !k_scale || !v_scale || !kv_strides) return fail(ELLM_ERR_INVALID_ARGUMENT, "null argument");
+  if (!c->k_scale) return fail(ELLM_ERR_INVALID_ARGUMENT, "the cache's rows are in 16 bits: use ellm_kv_layer");
+  if (layer >= c->desc.layers) return fail(ELLM_ERR_OUT_OF_RANGE, "layer %zu of %zu", layer, c->desc.layers);
+  if (first_sequence >= c->desc.sequences)
+    return fail(ELLM_ERR_OUT_OF_RANGE, "first_sequence %zu of %zu", first_sequence, c->desc.sequences);
+  if (c->ragged != (table != nullptr))
+    return fail(ELLM_ERR_INVALID_ARGUMENT, c->ragged ? "this cache has per-sequence capacities: a table is needed"
+                                                     : "this cache has one capacity for every sequence: no table");
+  const ellm::KvE4m3 l = c->layer_e4m3(layer);
+  const size_t at = c->ragged ? 0 : first_sequence * c->stride_seq;   // (a table's offsets are from the layer's start)
+  *k = l.k + at;
+  *v = l.v + at;
+  *k_scale = l.k_scale + at / 128;
+  *v_scale = l.v_scale + at / 128;
+  kv_strides[0] = c->ragged ? c->layer_elems : c->stride_seq;
+  kv_strides[1] = c->stride_head;
+  kv_strides[2] = c->desc.head_size;
+  kv_strides[3] = 1;
+  if (table) *table = c->table(first_sequence);
   return ELLM_OK;
 }
 
@@ -660,11 +741,14 @@ int ellm_kv_append(ellm_kv_cache* c, size_t layer, size_t position_index, size_t
                 position_index, position_index + n_tokens, room);
   if (n_tokens > 0xffffffffu / 2 || src_batch_pitch > 65535)
     return fail(ELLM_ERR_UNSUPPORTED, "n_tokens or src_batch_pitch too large");
-  void* k = (char*)c->k + layer * c->layer_elems * 2;
-  void* v = (char*)c->v + layer * c->layer_elems * 2;
-  hipError_t e = ellm::launch_kv_append(k, v, k_src, v_src, (uint32_t)n_tokens, (uint32_t)batch_size,
-                                        (uint32_t)src_batch_pitch, (uint32_t)c->desc.kv_head_num,
-                                        c->layout(), (uint32_t)position_index, (hipStream_t)stream);
+  const hipError_t e =
+      c->k_scale
+          ? ellm::launch_kv_append_e4m3(c->layer_e4m3(layer), k_src, v_src, nullptr, nullptr, (uint32_t)n_tokens,
+                                        (uint32_t)batch_size, (uint32_t)src_batch_pitch, (uint32_t)c->desc.kv_head_num,
+                                        c->layout(), (uint32_t)position_index, 0, 0.0f, c->desc.dtype, (hipStream_t)stream)
+          : ellm::launch_kv_append(c->layer_k(layer), c->layer_v(layer), k_src, v_src, (uint32_t)n_tokens,
+                                   (uint32_t)batch_size, (uint32_t)src_batch_pitch, (uint32_t)c->desc.kv_head_num,
+                                   c->layout(), (uint32_t)position_index, (hipStream_t)stream);
   if (e != hipSuccess) return fail_hip(e, "kv append launch");
   return ELLM_OK;
 }
@@ -698,13 +782,54 @@ int ellm_kv_append_norm_rope(ellm_kv_cache* c, size_t layer, size_t position_ind
                 first, first + n_tokens, rope_positions);
   if (n_tokens > 0xffffffffu / 2 || src_batch_pitch > 65535)
     return fail(ELLM_ERR_UNSUPPORTED, "n_tokens or src_batch_pitch too large");
-  void* k = (char*)c->k + layer * c->layer_elems * 2;
-  void* v = (char*)c->v + layer * c->layer_elems * 2;
-  hipError_t e = ellm::launch_kv_append_norm_rope(
-      k, v, k_src, v_src, rope, positions, (uint32_t)n_tokens, (uint32_t)batch_size,
-      (uint32_t)src_batch_pitch, (uint32_t)c->desc.kv_head_num, c->layout(),
-      (uint32_t)position_index, (uint32_t)max_position, eps, c->desc.dtype, (hipStream_t)stream);
+  const hipError_t e =
+      c->k_scale
+          ? ellm::launch_kv_append_e4m3(c->layer_e4m3(layer), k_src, v_src, rope, positions, (uint32_t)n_tokens,
+                                        (uint32_t)batch_size, (uint32_t)src_batch_pitch, (uint32_t)c->desc.kv_head_num,
+                                        c->layout(), (uint32_t)position_index, (uint32_t)max_position, eps, c->desc.dtype,
+                                        (hipStream_t)stream)
+          : ellm::launch_kv_append_norm_rope(c->layer_k(layer), c->layer_v(layer), k_src, v_src, rope, positions,
+                                             (uint32_t)n_tokens, (uint32_t)batch_size, (uint32_t)src_batch_pitch,
+                                             (uint32_t)c->desc.kv_head_num, c->layout(), (uint32_t)position_index,
+                                             (uint32_t)max_position, eps, c->desc.dtype, (hipStream_t)stream);
   if (e != hipSuccess) return fail_hip(e, "kv append (norm + rope) launch");
+  return ELLM_OK;
+}
+
+int ellm_kv_read_e4m3(const ellm_kv_cache* c, size_t layer, size_t first_sequence, size_t position_index, size_t n_tokens,
+                      size_t batch_size, void* k_dst, void* v_dst, const size_t dst_strides[3], void* stream) {
+  if (!c) return fail(ELLM_ERR_INVALID_ARGUMENT, "null cache");
+  if (!c->k_scale) return fail(ELLM_ERR_INVALID_ARGUMENT, "the cache's rows are in 16 bits already");
+  if (n_tokens == 0 || batch_size == 0) return ELLM_OK;
+  if (!k_dst || !v_dst || !dst_strides) return fail(ELLM_ERR_INVALID_ARGUMENT, "null destination or strides");
+  if (int st = ellm::check_current_device(c->device)) return st;
+  if (!aligned16(k_dst) || !aligned16(v_dst))
+    return fail(ELLM_ERR_INVALID_ARGUMENT, "destinations must be 16-byte aligned");
+  const size_t extent[3] = {n_tokens, batch_size, c->desc.kv_head_num};
+  for (int i = 0; i < 3; ++i)
+    if (dst_strides[i] % 8 != 0 || (extent[i] > 1 && dst_strides[i] < 128))
+      return fail(ELLM_ERR_INVALID_ARGUMENT, "dst_strides[%d] = %zu must be a multiple of 8 elements, and 128 at least", i,
+                  dst_strides[i]);
+  if (layer >= c->desc.layers) return fail(ELLM_ERR_OUT_OF_RANGE, "layer %zu of %zu", layer, c->desc.layers);
+  if (first_sequence >= c->desc.sequences || batch_size > c->desc.sequences - first_sequence)
+    return fail(ELLM_ERR_OUT_OF_RANGE, "sequences [%zu, %zu) of %zu", first_sequence, first_sequence + batch_size,
+                c->desc.sequences);
+  size_t room = c->caps_host[first_sequence];   // the shortest of the sequences read
+  for (size_t i = 1; i < batch_size; ++i)
+    room = c->caps_host[first_sequence + i] < room ? c->caps_host[first_sequence + i] : room;
+  if (position_index >= room || n_tokens > room - position_index)
+    return fail(ELLM_ERR_OUT_OF_RANGE, "positions [%zu, %zu) do not fit the capacity %zu", position_index,
+                position_index + n_tokens, room);
+  ellm::KvE4m3 l = c->layer_e4m3(layer);
+  if (!c->ragged) {
+    const size_t at = first_sequence * c->stride_seq;
+    l = ellm::KvE4m3{l.k + at, l.v + at, l.k_scale + at / 128, l.v_scale + at / 128};
+  }
+  const hipError_t e = ellm::launch_kv_read_e4m3(l, k_dst, v_dst, dst_strides[0], dst_strides[1], dst_strides[2],
+                                                 (uint32_t)n_tokens, (uint32_t)batch_size, (uint32_t)c->desc.kv_head_num,
+                                                 c->layout(first_sequence), (uint32_t)position_index, c->desc.dtype,
+                                                 (hipStream_t)stream);
+  if (e != hipSuccess) return fail_hip(e, "kv read launch");
   return ELLM_OK;
 }
 
@@ -716,9 +841,12 @@ static const char* append_mismatch(const ellm_kv_cache* c, size_t layer, const e
   if (c->device != a->device) return "the cache and the operator were created on different devices";
   if (d.dtype != c->desc.dtype) return "the cache and the operator differ in dtype";
   if (d.kv_head_num != c->desc.kv_head_num) return "the cache and the operator differ in kv_head_num";
-  const void* k = (const char*)c->k + layer * c->layer_elems * 2;
-  const void* v = (const char*)c->v + layer * c->layer_elems * 2;
-  if (d.k != k || d.v != v) return "the operator's k / v are not this layer of the cache";
+  if ((c->k_scale == nullptr) != (a->k_scale == nullptr)) return "one of the cache and the operator is in 8 bits, the other not";
+  if (c->k_scale) {
+    const ellm::KvE4m3 l = c->layer_e4m3(layer);
+    if (a->k_scale != l.k_scale || a->v_scale != l.v_scale) return "the operator's scales are not this layer's of the cache";
+  }
+  if (d.k != c->layer_k(layer) || d.v != c->layer_v(layer)) return "the operator's k / v are not this layer of the cache";
   if (d.kv_strides[1] != c->stride_head || d.kv_strides[2] != 128 || d.kv_strides[3] != 1)
     return "the operator's kv_strides are not the cache's";
   if (c->ragged) {
@@ -760,7 +888,7 @@ static int kv_append_attn(ellm_kv_cache* c, size_t layer, ellm_attn* a, const vo
   args.position_interval = 1;
   args.batch = (uint32_t)batch_size;
   args.positions = positions;
-  if (a->shaped.active()) {   // the kernels for shaped scores read finished rows: the two calls one after the other
+  if (a->shaped.active() || a->k_scale) {   // those kernels read finished rows: the two calls one after the other
     const int st = ellm_kv_append_norm_rope(c, layer, position_index, 1, batch_size, k_src, v_src, batch_size, rope,
                                             rope_positions, eps, positions, max_position, stream);
     return st != ELLM_OK ? st : ellm::attn_run_single_token(a, &args, (uint32_t)first, (hipStream_t)stream);

@@ -23,7 +23,7 @@
 //   that finishes last for a (sequence, head group) combines that group's
 //   splits (a self-resetting arrival counter per group; no second launch).
 
-#include "decode_common.hpp"
+#include "decode_e4m3.hpp"
 
 namespace ellm {
 using namespace dec;
@@ -32,9 +32,9 @@ namespace {
 // PENDING = kPendSums: the launch of a fused step (ellm_matmul3_attn_run): the query rows and the
 // new key / value row of every plane come as the projection's raw sums (p.pend) and are finished
 // here.  kPendRows (ellm_kv_append_attn_run): the new key / value rows come as stored 16-bit rows.
-// SHAPE: shaped scores (decode_common.hpp).
-template <typename T, int PENDING, int SHAPE = kShapeNone>
-__global__ __launch_bounds__(kDecThreads, PENDING ? 2 : 4) void decode_split_kernel(DecodeKernelArgs p) {
+// SHAPE: shaped scores (decode_common.hpp).  E4M3: planes of rows in 8 bits (decode_e4m3.hpp).
+template <typename T, int PENDING, int SHAPE = kShapeNone, bool E4M3 = false>
+__global__ __launch_bounds__(kDecThreads, PENDING || E4M3 ? 2 : 4) void decode_split_kernel(DecodeKernelArgs p) {
   __shared__ __attribute__((aligned(16))) uint16_t smem[kDecWaves * kWaveLdsHalves];
   __shared__ uint32_t s_last;
 
@@ -86,6 +86,10 @@ __global__ __launch_bounds__(kDecThreads, PENDING ? 2 : 4) void decode_split_ker
     if constexpr (PENDING == kPendSums) {
       if (fresh.present) store_queries(const_cast<uint16_t*>(p.q) + (size_t)row0 * kHeadDim, t, heads_here, qreg);
     }
+  } else if constexpr (E4M3) {
+    load_queries8(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
+    stream_keys8<T>(p, plane, k_begin, k_end, pos, qreg, smem, t, split * 7u + blockIdx.y * 3u + seq * 5u, m_run, l_run, acc);
+    order_columns8(acc);
   } else {
     load_queries(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
     stream_keys<T>(planes_of<SHAPE>(p, plane, kvh, range), k_begin, k_end, pos, qreg, smem, t,
@@ -95,13 +99,13 @@ __global__ __launch_bounds__(kDecThreads, PENDING ? 2 : 4) void decode_split_ker
   auto final_row = [&](uint32_t h, uint32_t dq, const f32x4& a, float l, float m) {
     emit_joined<T, SHAPE>(p, row0 + h, dq, a, l, m);
   };
-  merge_waves(smem, t, heads_here, m_run, l_run, acc,
-              [&](uint32_t h, uint32_t dq, const f32x4& a, float l, float m) {
-                if (p.n_split == 1)
-                  final_row(h, dq, a, l, m);
-                else
-                  store_partial(p.ws_acc, p.ws_ml, (size_t)((row0 + h) * p.n_split + split), dq, a, l, m);
-              });
+  merge_waves<E4M3 ? 4 : 16, E4M3 ? 32 : 4>(
+      smem, t, heads_here, m_run, l_run, acc, [&](uint32_t h, uint32_t dq, const f32x4& a, float l, float m) {
+        if (p.n_split == 1)
+          final_row(h, dq, a, l, m);
+        else
+          store_partial(p.ws_acc, p.ws_ml, (size_t)((row0 + h) * p.n_split + split), dq, a, l, m);
+      });
   if (p.n_split == 1) return;
 
   // ---- the last workgroup to arrive merges: two levels, 16 partials each -----
@@ -179,10 +183,17 @@ hipError_t launch_decode(const AttnArgs& a, hipStream_t stream, const ShapedStat
   p.batch = a.batch;
   p.scale_log2 = a.scale * kLog2e;
   p.pend = a.pending;
+  p.k_scale = a.k_scale;
+  p.v_scale = a.v_scale;
 
   dim3 grid(a.n_split, a.n_kv_heads * p.head_groups, a.batch);
   dim3 block(kDecThreads);
-  if (shape) {
+  if (a.k_scale) {
+    if (a.dtype == 0)
+      hipLaunchKernelGGL((decode_split_kernel<F16, kPendNone, kShapeNone, true>), grid, block, 0, stream, p);
+    else
+      hipLaunchKernelGGL((decode_split_kernel<BF16, kPendNone, kShapeNone, true>), grid, block, 0, stream, p);
+  } else if (shape) {
     const int kind = fill_shape(*shape, a, &p.shape);
     if (a.dtype == 0)
       launch_shaped_split<F16>(p, grid, kind, stream);

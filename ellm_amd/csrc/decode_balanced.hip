@@ -17,7 +17,7 @@
 //
 // Reference semantics unchanged: per (sequence, query head) the result of flash_attention
 // (src/kernel/x86_64/f16_512/flash_attention.rs:30-92) over keys 0..=position of the sequence.
-#include "decode_common.hpp"
+#include "decode_e4m3.hpp"
 #include "decode_shares.hpp"
 
 namespace ellm {
@@ -38,8 +38,8 @@ __device__ __forceinline__ uint32_t uni(uint32_t v) { return (uint32_t)__builtin
 // reason (1 + floor(n / 16) >= ceil(n / 16)).
 
 // PENDING: the launch of a fused step, as in decode.hip.  SHAPE: shaped scores (decode_common.hpp); lengths are then those
-// of the key ranges.
-template <typename T, int PENDING, int SHAPE = kShapeNone>
+// of the key ranges.  E4M3: planes of rows in 8 bits (decode_e4m3.hpp).
+template <typename T, int PENDING, int SHAPE = kShapeNone, bool E4M3 = false>
 __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeKernelArgs p) {
   __shared__ __attribute__((aligned(16))) uint16_t smem[kDecWaves * kWaveLdsHalves];
   __shared__ uint32_t prefix[kMaxBatch + 1];   // units of the sequences before sequence b (per plane)
@@ -230,6 +230,10 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
       if constexpr (PENDING == kPendSums) {
         if (fresh.present) store_queries(const_cast<uint16_t*>(p.q) + (size_t)row0 * kHeadDim, t, heads_here, qreg);
       }
+    } else if constexpr (E4M3) {
+      load_queries8(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
+      stream_keys8<T>(p, plane, k_begin, k_end, pos, qreg, smem, t, w * 7u + pl * 3u + seq * 5u, m_run, l_run, acc);
+      order_columns8(acc);
     } else {
       load_queries(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
       stream_keys<T>(planes_of<SHAPE>(p, plane, kvh, range), k_begin, k_end, pos, qreg, smem, t,
@@ -239,13 +243,13 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
     auto final_row = [&](uint32_t h, uint32_t dq, const f32x4& av, float l, float m) {
       emit_joined<T, SHAPE>(p, (size_t)(row0 + h), dq, av, l, m);
     };
-    merge_waves(smem, t, heads_here, m_run, l_run, acc,
-                [&](uint32_t h, uint32_t dq, const f32x4& av, float l, float m) {
-                  if (n_pieces == 1)
-                    final_row(h, dq, av, l, m);
-                  else
-                    store_partial(p.ws_acc, p.ws_ml, (size_t)((slot0 + piece) * G + h), dq, av, l, m);
-                });
+    merge_waves<E4M3 ? 4 : 16, E4M3 ? 32 : 4>(
+        smem, t, heads_here, m_run, l_run, acc, [&](uint32_t h, uint32_t dq, const f32x4& av, float l, float m) {
+          if (n_pieces == 1)
+            final_row(h, dq, av, l, m);
+          else
+            store_partial(p.ws_acc, p.ws_ml, (size_t)((slot0 + piece) * G + h), dq, av, l, m);
+        });
     if (n_pieces > 1) {
       const uint32_t n_clusters = (n_pieces + kMergeFan - 1) / kMergeFan;
       const uint32_t cluster = piece / kMergeFan;
@@ -332,8 +336,15 @@ hipError_t launch_decode_balanced(const AttnArgs& a, uint32_t wgs, hipStream_t s
   p.n_cluster_max = balanced_cluster_slots(wgs, planes);
   p.counters_per_plane = 0;
   p.pend = a.pending;
+  p.k_scale = a.k_scale;
+  p.v_scale = a.v_scale;
   const dim3 grid(wgs), block(kDecThreads);
-  if (shape) {
+  if (a.k_scale) {
+    if (a.dtype == 0)
+      hipLaunchKernelGGL((decode_balanced_kernel<F16, kPendNone, kShapeNone, true>), grid, block, 0, stream, p);
+    else
+      hipLaunchKernelGGL((decode_balanced_kernel<BF16, kPendNone, kShapeNone, true>), grid, block, 0, stream, p);
+  } else if (shape) {
     const int kind = fill_shape(*shape, a, &p.shape);
     if (a.dtype == 0)
       launch_shaped_balanced<F16>(p, grid, kind, stream);

@@ -74,6 +74,8 @@ struct DecodeKernelArgs {
   float scale_log2;   // scale * log2(e)
   PendingRows pend;   // raw query / key / value rows of a fused step (kernels built with PENDING)
   ShapeArgs shape;    // kernels built with SHAPE
+  const uint8_t* k_scale;   // kernels built for rows in 8 bits (decode_e4m3.hpp)
+  const uint8_t* v_scale;
 };
 
 // What a sequence's query sees: `len` rows from row `first` on (none: 0) of the sequence's own, or with kShapeWalk of the
@@ -578,8 +580,9 @@ __device__ __forceinline__ void stream_keys(const Planes& planes, uint32_t k_beg
 // Merge the four waves through LDS (red[wave][head][128 acc + max + sum], in the staging
 // buffers).  Afterwards a thread owns four consecutive columns of one head (an item; eight heads
 // make 256 items, one per thread, sixteen heads two per thread) and hands them to
-// emit(h, dq, a[4], sum, max): columns 4 dq .. 4 dq + 3 of head h of the group.
-template <typename Emit>
+// emit(h, dq, a[4], sum, max): columns 4 dq .. 4 dq + 3 of head h of the group.  acc[b] of lane (head, g): columns
+// QUAD_B b + QUAD_G g .. + 3.
+template <int QUAD_B = 16, int QUAD_G = 4, typename Emit>
 __device__ __forceinline__ void merge_waves(uint16_t* smem, const Lane& t, uint32_t heads_here, float m_run,
                                             float l_run, const f32x4 (&acc)[8], Emit emit) {
   __syncthreads();
@@ -587,7 +590,7 @@ __device__ __forceinline__ void merge_waves(uint16_t* smem, const Lane& t, uint3
   if ((uint32_t)t.c < heads_here) {
     float* row = red + (t.wave * kMaxHeadsPerGroup + t.c) * kRedPitch;
 #pragma unroll
-    for (int b = 0; b < 8; ++b) *(f32x4*)(row + 16 * b + 4 * t.g) = acc[b];
+    for (int b = 0; b < 8; ++b) *(f32x4*)(row + QUAD_B * b + QUAD_G * t.g) = acc[b];
     if (t.g == 0) *(f32x2*)(row + kHeadDim) = f32x2{m_run, l_run};
   }
   __syncthreads();

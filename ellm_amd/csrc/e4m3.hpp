@@ -1,0 +1,80 @@
+// Rows of a cache in 8 bits, as the kernels read and write them.
+//
+// A row of 128 elements is 128 codes of the type e4m3 (sign, 4 bits of exponent, 3 of mantissa, the largest 448, code 0x7f
+// NaN) and one byte of the type e8m0, the biased exponent of its scale 2^(b - 127); 255 is NaN.  The rows of a plane lie
+// wherever their codes do: the scale of the row whose codes begin at byte x of a layer is byte x / 128 of the layer's
+// scales.  A power of two as scale costs e4m3 nothing (its error is relative down to 2^-9 of a row's scale) and makes every
+// step exact but one, the rounding of x / 2^e to four significant bits: what is read back is a 16-bit value as it stands.
+#pragma once
+
+#include "common.hpp"
+
+namespace ellm {
+
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+
+constexpr uint32_t kScaleNan = 255;
+
+// The scale of a row as the conversions take it (they look at the exponent field alone, as e8m0: 0 is 2^-127, 255 NaN).
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
+
+// Two codes of a register (the low or the high pair) times a scale as two 16-bit values: exact, where the type has the value.
+template <typename T>
+struct Codes;
+template <>
+struct Codes<F16> {
+  template <bool HI>
+  static __device__ __forceinline__ uint32_t pair(uint32_t codes, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, HI));
+  }
+  // the largest value of four significant bits: what a row's values are cut to ahead of their rounding
+  static constexpr float kLargest = 61440.0f;   // 1.875 x 2^15
+};
+template <>
+struct Codes<BF16> {
+  template <bool HI>
+  static __device__ __forceinline__ uint32_t pair(uint32_t codes, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, HI));
+  }
+  static constexpr float kLargest = 0x1.ep127f;
+};
+
+// Four codes as four 16-bit values.
+template <typename T>
+__device__ __forceinline__ u32x2 values4(uint32_t codes, float scale) {
+  return u32x2{Codes<T>::template pair<false>(codes, scale), Codes<T>::template pair<true>(codes, scale)};
+}
+
+// The byte of the smallest scale 2^e with top <= 448 2^e, e >= -126; `top`: the bits of the row's largest magnitude (those of
+// infinities and NaN: the scale is NaN).  448 is 1.75 x 2^8: a mantissa above 1.75 (0x600000) carries into the exponent.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
+  const uint32_t b = (top + 0x1fffffu) >> 23;
+  return top >= 0x7f800000u ? kScaleNan : b > 9 ? b - 8 : 1;
+}
+
+// Sixteen lanes hold a row, eight values each: their codes, and the scale's byte.  Every lane of the wave must call this.
+template <typename T>
+__device__ __forceinline__ u32x2 row_codes16(const float (&x)[8], uint32_t& byte) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = max(top, __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffffu);
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, 16));
+  byte = scale_byte(top);
+  const float scale = scale_of(byte);
+  u32x2 codes;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    float c[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      c[e] = __builtin_amdgcn_fmed3f(x[4 * w + e], -Codes<T>::kLargest, Codes<T>::kLargest);
+    i16x2 to = {0, 0};
+    to = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(to, c[0], c[1], scale, false);
+    to = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(to, c[2], c[3], scale, true);
+    codes[w] = byte == kScaleNan ? 0u : __builtin_bit_cast(uint32_t, to);   // (a row that is NaN holds no values)
+  }
+  return codes;
+}
+
+}  // namespace ellm

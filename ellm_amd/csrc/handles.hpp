@@ -32,6 +32,9 @@ struct ellm_attn {
   bool general;
   // shaped scores and shared prefix (shaped_api.hip); inactive until one of them is set
   ellm::ShapedState shaped{};
+  // k and v are planes in 8 bits (ellm_attn_create_e4m3): their rows' scales; null otherwise
+  const uint8_t* k_scale = nullptr;
+  const uint8_t* v_scale = nullptr;
 };
 
 struct ellm_matmul3 {

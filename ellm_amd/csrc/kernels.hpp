@@ -74,6 +74,9 @@ struct AttnArgs {
   size_t prefill_part_rows;
   uint32_t n_cu;
   PendingRows pending;   // single-token path only
+  // planes in 8 bits (k, v: codes; null: 16-bit rows): the rows' scales (e4m3.hpp)
+  const uint8_t* k_scale;
+  const uint8_t* v_scale;
 };
 
 struct ShapedState;
@@ -111,6 +114,25 @@ hipError_t launch_kv_append_norm_rope(void* k_dst, void* v_dst, const void* k_sr
                                       const KvLayout& layout, uint32_t position_index,
                                       uint32_t max_start, float eps, int dtype,
                                       hipStream_t stream);
+
+// One layer of a cache in 8 bits: codes and scales (e4m3.hpp); KvLayout's strides count codes.
+struct KvE4m3 {
+  uint8_t* k;
+  uint8_t* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+};
+// The two writes above into such a layer; rope null: key rows as they are.  dtype: of the rows that come.
+hipError_t launch_kv_append_e4m3(const KvE4m3& cache, const void* k_src, const void* v_src, const void* rope,
+                                 const uint32_t* positions, uint32_t n_tokens, uint32_t batch, uint32_t src_batch_pitch,
+                                 uint32_t n_kv_heads, const KvLayout& layout, uint32_t position_index, uint32_t max_start,
+                                 float eps, int dtype, hipStream_t stream);
+// Rows back in 16 bits: token t of sequence s, head h to t x dst_token + s x dst_sequence + h x dst_head (elements).
+hipError_t launch_kv_read_e4m3(const KvE4m3& cache, void* k_dst, void* v_dst, size_t dst_token, size_t dst_sequence,
+                               size_t dst_head, uint32_t n_tokens, uint32_t batch, uint32_t n_kv_heads,
+                               const KvLayout& layout, uint32_t position_index, int dtype, hipStream_t stream);
+// Chunks over planes in 8 bits (e4m3_chunk.hip).
+hipError_t launch_chunk_e4m3(const AttnArgs& a, hipStream_t stream);
 
 hipError_t launch_positions_advance(uint32_t* positions, uint32_t n, uint32_t by,
                                     hipStream_t stream);

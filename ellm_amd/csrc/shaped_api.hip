@@ -16,6 +16,8 @@ int prepare(ellm_attn* h, bool on) {
   if (int st = ellm::check_current_device(h->device)) return st;
   if (h->general)
     return ellm::set_error(ELLM_ERR_UNSUPPORTED, "shaped scores and shared prefixes take head_size 128 and 16-bit storage only");
+  if (h->k_scale)
+    return ellm::set_error(ELLM_ERR_UNSUPPORTED, "shaped scores and shared prefixes take planes of 16-bit rows only");
   if (!std::isfinite(h->desc.inverse_sqrt_head * 4.0f))
     return ellm::set_error(ELLM_ERR_INVALID_ARGUMENT, "inverse_sqrt_head %g is too large for shaped scores",
                            (double)h->desc.inverse_sqrt_head);

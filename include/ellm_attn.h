@@ -339,6 +339,52 @@ int ellm_attn_create_ragged(const ellm_attn_desc* desc, const ellm_kv_seq_table*
                             ellm_attn** out_handle);
 
 /*
+ * A cache in 8 bits: half the bytes of a 16-bit one, for steps that are bound by reading them.  A row (the 128 elements of
+ * one position of a K/V head) is 128 codes of the type e4m3 (1 sign, 4 exponent, 3 mantissa bits; the largest 448, no
+ * infinities, 0x7f and 0xff NaN) and one byte of the type e8m0, the row's scale 2^(byte - 127); 255 is NaN.  Element i is
+ * code i times the scale.  Written rows take, with a = the largest |x| of the row,
+ *     scale = the smallest 2^e with a <= 448 * 2^e, e >= -126
+ *     code  = x / scale, rounded to the nearest e4m3 (ties to even), x first cut to +-1.875 * 2^15 (binary16 rows) or
+ *             +-1.875 * 2^127 (bfloat16), the largest such value that the type holds: an element is off by 2^-4 of itself at
+ *             most, or by 2^-10 of the scale where it is below 2^-6 of it
+ * and a row that holds an infinity or a NaN reads as NaN as a whole (scale 255, codes 0).  What is read back is a value of
+ * the 16-bit type as it stands, and attention over the cache is attention over those values.
+ * desc->dtype: the type of the rows that are written and read back.  The other calls for caches take such a cache too:
+ * ellm_kv_append, ellm_kv_append_norm_rope (key rows are normalised and rotated in binary32 and rounded once, to e4m3),
+ * ellm_kv_append_attn_run*, ellm_kv_destroy; ellm_kv_layer and ellm_kv_layer_ragged refuse it.  No counterpart in the
+ * reference, whose caches hold the element type of the graph (src/memory/cache.rs:23).
+ */
+int ellm_kv_create_e4m3(const ellm_kv_desc* desc, ellm_kv_cache** out_cache);
+int ellm_kv_create_ragged_e4m3(const ellm_kv_ragged_desc* desc, ellm_kv_cache** out_cache);
+
+/* One layer of such a cache from sequence first_sequence on: codes, scales and the strides, which count codes; the scale of
+ * the row whose codes begin at k[x] is k_scale[x / 128], with v likewise.  table: NULL for a cache with one capacity, to be
+ * filled for one with a capacity for each sequence (as by ellm_kv_layer_ragged). */
+int ellm_kv_layer_e4m3(const ellm_kv_cache* cache, size_t layer, size_t first_sequence, void** k, void** v,
+                       uint8_t** k_scale, uint8_t** v_scale, size_t kv_strides[4], ellm_kv_seq_table* table);
+
+/* Rows of such a cache in 16 bits (desc->dtype): positions [position_index, position_index + n_tokens) of sequences
+ * [first_sequence, first_sequence + batch_size).  The row of token t, sequence s, head h (counted from 0) goes to
+ * k_dst + t * dst_strides[0] + s * dst_strides[1] + h * dst_strides[2] (elements, multiples of 8, at least 128 along axes
+ * longer than one), v_dst likewise: {batch_size * kv_head_num * 128, kv_head_num * 128, 128} is the order ellm_kv_append
+ * takes rows in, {128, kv_strides[0], kv_strides[1]} that of a 16-bit cache.  Destinations are 16-byte aligned and outside
+ * the cache. */
+int ellm_kv_read_e4m3(const ellm_kv_cache* cache, size_t layer, size_t first_sequence, size_t position_index,
+                      size_t n_tokens, size_t batch_size, void* k_dst, void* v_dst, const size_t dst_strides[3],
+                      void* stream);
+
+/* ellm_attn_create / _create_ragged (table not NULL) over planes in 8 bits: desc->k and v are codes, kv_strides count codes
+ * and are multiples of 128 (so are a table's offsets); k_scale[x / 128] is the scale of the row whose codes begin at k[x],
+ * with v likewise; desc->dtype is the type of q and out, in which the rows' values are taken (exact for rows that the cache
+ * wrote from that type, or from binary16 under bfloat16).  head_size 128, 16-bit dtype.  Any codes and scales in that layout
+ * will do, not only a cache's; codes of NaN in value rows count as infinities do in ellm_attn_run (rows that do not see
+ * them yet must not meet them in a chunk), scales of NaN are seen by the rows that see the key only.
+ * Runs as of any handle (ellm_attn_run, ellm_attn_run_ragged; as part of ellm_kv_append_attn_run*: the cache write and the
+ * run, two launches).  ellm_attn_set_scores, ellm_attn_set_shared_prefix and ellm_matmul3_attn_run* refuse such a handle. */
+int ellm_attn_create_e4m3(const ellm_attn_desc* desc, const uint8_t* k_scale, const uint8_t* v_scale,
+                          const ellm_kv_seq_table* table, ellm_attn** out_handle);
+
+/*
  * Writes n_tokens new positions [position_index, position_index + n_tokens) of
  * sequences [0, batch_size) of one layer.  k_src / v_src: device,
  * [n_tokens][src_batch_pitch][kv_head_num][128] — the layout in which the
