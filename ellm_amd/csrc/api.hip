@@ -474,11 +474,8 @@ int ellm_attn_run(ellm_attn* h, size_t position_index, size_t position_interval,
   a.batch = (uint32_t)batch_size;
   if (position_interval == 1) return ellm::attn_run_single_token(h, &a, (uint32_t)position_index, (hipStream_t)stream);
   if (h->shaped.active()) return ellm::attn_run_shaped(h, a, (hipStream_t)stream);
-  if (h->k_scale && (uint64_t)position_interval * d.batch_size > 0x7fffffffull / d.attention_head_num)
-    return fail(ELLM_ERR_UNSUPPORTED, "chunks over planes in 8 bits take fewer than 2^31 query rows");
-  hipError_t e = h->general   ? ellm::launch_attn_general(a, (uint32_t)d.head_size, (hipStream_t)stream)
-                 : h->k_scale ? ellm::launch_chunk_e4m3(a, (hipStream_t)stream)
-                              : ellm::launch_prefill(a, (hipStream_t)stream);
+  hipError_t e = h->general ? ellm::launch_attn_general(a, (uint32_t)d.head_size, (hipStream_t)stream)
+                            : ellm::launch_prefill(a, (hipStream_t)stream);
   if (e != hipSuccess) return fail_hip(e, "chunk attention launch");
   return ELLM_OK;
 }

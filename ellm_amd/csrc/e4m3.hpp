@@ -45,6 +45,18 @@ __device__ __forceinline__ u32x2 values4(uint32_t codes, float scale) {
   return u32x2{Codes<T>::template pair<false>(codes, scale), Codes<T>::template pair<true>(codes, scale)};
 }
 
+// Eight codes of a row as eight 16-bit values.
+template <typename T>
+__device__ __forceinline__ u32x4 values8(u32x2 codes, uint32_t scale) {
+  const u32x2 lo = values4<T>(codes[0], scale_of(scale)), hi = values4<T>(codes[1], scale_of(scale));
+  return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+// The scales that a chunk's kernels take a key row and its value row with.  A value row whose scale is NaN is taken as what its codes
+// say (zeros, where the cache wrote them) and its key's scale as NaN instead: rows that see the key get weights, and so
+// results, of NaN; rows that do not see it yet give it a weight of exactly 0, and 0 x NaN would be NaN.
+__device__ __forceinline__ uint32_t key_scale(uint32_t k, uint32_t v) { return v == kScaleNan ? kScaleNan : k; }
+__device__ __forceinline__ uint32_t value_scale(uint32_t v) { return v == kScaleNan ? 127u : v; }
+
 // The byte of the smallest scale 2^e with top <= 448 2^e, e >= -126; `top`: the bits of the row's largest magnitude (those of
 // infinities and NaN: the scale is NaN).  448 is 1.75 x 2^8: a mantissa above 1.75 (0x600000) carries into the exponent.
 __device__ __forceinline__ uint32_t scale_byte(uint32_t top) {

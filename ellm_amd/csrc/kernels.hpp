@@ -131,8 +131,6 @@ hipError_t launch_kv_append_e4m3(const KvE4m3& cache, const void* k_src, const v
 hipError_t launch_kv_read_e4m3(const KvE4m3& cache, void* k_dst, void* v_dst, size_t dst_token, size_t dst_sequence,
                                size_t dst_head, uint32_t n_tokens, uint32_t batch, uint32_t n_kv_heads,
                                const KvLayout& layout, uint32_t position_index, int dtype, hipStream_t stream);
-// Chunks over planes in 8 bits (e4m3_chunk.hip).
-hipError_t launch_chunk_e4m3(const AttnArgs& a, hipStream_t stream);
 
 hipError_t launch_positions_advance(uint32_t* positions, uint32_t n, uint32_t by,
                                     hipStream_t stream);

@@ -29,7 +29,7 @@
 #include <type_traits>
 
 #include "chunk_plan.hpp"
-#include "common.hpp"
+#include "e4m3.hpp"
 #include "kernels.hpp"
 
 namespace ellm {
@@ -66,7 +66,33 @@ struct PrefillKernelArgs {
   uint32_t n_split, split_tiles;
   float* part_o;
   float* part_ml;
+  const uint8_t* k_scale;   // E4M3
+  const uint8_t* v_scale;
 };
+
+// Rows on their way from memory to LDS, eight elements a lane and piece.  E4M3 (the template argument of the kernels below):
+// planes of rows in 8 bits (e4m3.hpp), strides in codes.  Eight codes are eight bytes to load, and their row's scale one
+// more; they are converted between the load's registers and LDS, once for all the rows that read the tile, so that
+// nothing else of a kernel changes.  (A lane of K takes the value row's scale as well: key_scale.)
+template <bool E4M3>
+struct Piece {
+  u32x4 rows;
+};
+template <>
+struct Piece<true> {
+  u32x2 codes;
+  uint32_t k_scale, v_scale;
+};
+constexpr uint32_t kElemBytes[2] = {2, 1};   // of a plane's element: [E4M3]
+// What a piece is in LDS: of a key row (KEYS) or a value row.
+template <typename T, bool KEYS>
+__device__ __forceinline__ u32x4 staged(const Piece<false>& x) {
+  return x.rows;
+}
+template <typename T, bool KEYS>
+__device__ __forceinline__ u32x4 staged(const Piece<true>& x) {
+  return values8<T>(x.codes, KEYS ? key_scale(x.k_scale, x.v_scale) : value_scale(x.v_scale));
+}
 
 // ---------------------------------------------------------------------------
 // Ping-pong kernel: 8 waves, two per SIMD.  Waves 0-3 and waves 4-7 run the
@@ -135,6 +161,17 @@ constexpr int kPpAhead = kPpBuffers - 1;     // DIRECT: tiles requested ahead of
 static_assert(kPpAhead == 3, "s_waitcnt vmcnt literals in prefill_pingpong_kernel");
 constexpr int kBufferFlags = 0x00020000;  // raw buffer of 32-bit data, no swizzle (word 3 of the descriptor)
 
+// Rows that the scales' descriptor covers where that of the codes covers `left` bytes.
+__device__ __forceinline__ uint32_t rows_left(uint32_t left) { return left / kHeadDim + (left % kHeadDim ? 1u : 0u); }
+// The scales of a key row and its value row: of the row that holds byte `at` from byte `off` of the cache's layer on, of which `left`
+// bytes may be read (rows past those: 0).
+__device__ __forceinline__ void load_scales(const PrefillKernelArgs& p, uint64_t off, uint32_t left, uint32_t at, Piece<true>& x) {
+  const uint32_t rows = rows_left(left);
+  const uint64_t ks = uniform64(p.k_scale + off / kHeadDim), vs = uniform64(p.v_scale + off / kHeadDim);
+  x.k_scale = __builtin_amdgcn_raw_buffer_load_b8(__builtin_amdgcn_make_buffer_rsrc((void*)ks, 0, rows, kBufferFlags), at / kHeadDim, 0, 0);
+  x.v_scale = __builtin_amdgcn_raw_buffer_load_b8(__builtin_amdgcn_make_buffer_rsrc((void*)vs, 0, rows, kBufferFlags), at / kHeadDim, 0, 0);
+}
+
 // 16 bytes a lane from memory straight to LDS address lds_at + 16 x lane.  Written as asm: the compiler's
 // own form of this load makes it wait for every outstanding one before each later LDS read (it cannot see
 // that the two touch different buffers).  M0 carries the address; one wait state between its write and the
@@ -144,8 +181,9 @@ __device__ __forceinline__ void load_to_lds(const u32x4& rsrc, uint32_t voff, ui
                :: "s"(lds_at), "v"(voff), "s"(rsrc) : "memory");
 }
 
-template <typename T, bool SPLIT, bool DIRECT>
+template <typename T, bool SPLIT, bool DIRECT, bool E4M3 = false>
 __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(PrefillKernelArgs p) {
+  static_assert(!(DIRECT && E4M3), "rows in 8 bits are converted on their way");
   // Through registers: K tiles [2][64][kVsPitch] then V tiles [3][64][kVsPitch]; V is staged one step
   // earlier than it is read, so that every operand of a matrix step is in LDS a whole
   // phase before the step starts and can be requested ahead of the barrier.  (288-byte rows: the sixteen lanes that
@@ -206,8 +244,9 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(Prefill
   const float c = p.c;
 
   const size_t plane_at = seq_plane_offset(p.seq_offsets, p.kv_stride_seq, seq) + kvh * p.kv_stride_head;
-  const uint16_t* kplane = p.k + plane_at;
-  const uint16_t* vplane = p.v + plane_at;
+  constexpr uint32_t kElem = kElemBytes[E4M3];
+  const char* kplane = (const char*)p.k + plane_at * kElem;
+  const char* vplane = (const char*)p.v + plane_at * kElem;
 
   // staging: the 256 threads of a group move one 64 x 128 tile, four 16-byte pieces
   // each (rows ld_r + 16 i, columns 8 ld_c ..), K and V alike: V sits in LDS row by
@@ -215,7 +254,7 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(Prefill
   const int st_tid = tid & 255;
   const int ld_r = st_tid >> 4;
   const int ld_c = DIRECT ? (st_tid & 15) ^ (grp ? 2 * (ld_r & 7) : ld_r) : st_tid & 15;
-  const uint16_t* plane = grp ? vplane : kplane;                  // wave-uniform
+  const char* plane = grp ? vplane : kplane;                  // wave-uniform
   const uint32_t stride_pos = (uint32_t)p.kv_stride_pos;
   // Tiles are fetched with buffer loads: the descriptor (base of tile kt, bytes
   // left up to the last key this workgroup may see) is scalar arithmetic, the
@@ -227,11 +266,11 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(Prefill
   const uint32_t plane_lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uint64_t)plane);
   const uint32_t plane_hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)plane >> 32));
   const uint64_t plane_u = ((uint64_t)plane_hi << 32) | (uint64_t)plane_lo;
-  const uint32_t tile_bytes = kBK * stride_pos * 2;   // (API bound: 64 rows span < 2^32 bytes)
-  const uint64_t valid_bytes = uniform_u64(((uint64_t)kmax * stride_pos + kHeadDim) * 2);
+  const uint32_t tile_bytes = kBK * stride_pos * kElem;   // (API bound: 64 rows span < 2^32 bytes)
+  const uint64_t valid_bytes = uniform_u64(((uint64_t)kmax * stride_pos + kHeadDim) * kElem);
   uint32_t piece_off[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) piece_off[i] = ((ld_r + 16 * i) * stride_pos + 8 * ld_c) * 2;
+  for (int i = 0; i < 4; ++i) piece_off[i] = ((ld_r + 16 * i) * stride_pos + 8 * ld_c) * kElem;
   // LDS addresses are kept as byte offsets: the buffers span more than the 64 KB an
   // instruction's immediate offset reaches, so each step forms one base register
   // per tile (step_base) and everything else is an immediate on top of it.
@@ -242,23 +281,35 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(Prefill
   };
   const uint32_t ks_store = lds0 + 2 * (ld_r * kVsPitch + 8 * ld_c);
   const uint32_t vs_store = ks_store + 2 * 2 * kVsHalves;
-  u32x4 stg[4];
-  auto load_piece = [&](uint32_t kt, int i) {  // kt (relative to kt0) must be wave-uniform to the compiler
+  Piece<E4M3> stg[4];
+  const uint64_t k_scale_u = E4M3 ? uniform64(p.k_scale + plane_at / kHeadDim) : 0, v_scale_u = E4M3 ? uniform64(p.v_scale + plane_at / kHeadDim) : 0;
+  // kt (relative to kt0) must be wave-uniform to the compiler
+  auto load_piece = [&](auto group, uint32_t kt, int i) __attribute__((always_inline)) {
     const uint64_t off = (uint64_t)(kt0 + kt) * tile_bytes;
     const uint32_t left = bytes_left(valid_bytes, off);
     const __amdgpu_buffer_rsrc_t rsrc =
         __builtin_amdgcn_make_buffer_rsrc((void*)(plane_u + off), 0, left, kBufferFlags);
-    stg[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, piece_off[i], 0, 0);
+    if constexpr (E4M3) {
+      const uint32_t rows = rows_left(left), row = piece_off[i] / kHeadDim;
+      stg[i].codes = __builtin_amdgcn_raw_buffer_load_b64(rsrc, piece_off[i], 0, 0);
+      if (!group)
+        stg[i].k_scale = __builtin_amdgcn_raw_buffer_load_b8(
+            __builtin_amdgcn_make_buffer_rsrc((void*)(k_scale_u + off / kHeadDim), 0, rows, kBufferFlags), row, 0, 0);
+      stg[i].v_scale = __builtin_amdgcn_raw_buffer_load_b8(
+          __builtin_amdgcn_make_buffer_rsrc((void*)(v_scale_u + off / kHeadDim), 0, rows, kBufferFlags), row, 0, 0);
+    } else {
+      stg[i].rows = __builtin_amdgcn_raw_buffer_load_b128(rsrc, piece_off[i], 0, 0);
+    }
   };
   // (the group comes as a compile-time constant where the caller runs behind the scalar
   // branch on the group, as the run-time value in the prologue)
   // base: step_base of this lane's place in the destination buffer
-  auto store_piece = [&](uint32_t base, int i) {
-    *(LdsU32x4*)(base + 2 * 16 * i * kVsPitch) = stg[i];
+  auto store_piece = [&](auto group, uint32_t base, int i) __attribute__((always_inline)) {
+    *(LdsU32x4*)(base + 2 * 16 * i * kVsPitch) = group ? staged<T, false>(stg[i]) : staged<T, true>(stg[i]);
   };
   auto load_tile = [&](uint32_t kt) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_piece(kt, i);
+    for (int i = 0; i < 4; ++i) load_piece(grp, kt, i);
   };
   auto store_base = [&](auto group, int buf) {
     return step_base((group ? vs_store : ks_store) + 2 * buf * kVsHalves);
@@ -266,7 +317,7 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(Prefill
   auto store_tile = [&](int buf) {
     const uint32_t base = store_base(grp, buf);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) store_piece(base, i);
+    for (int i = 0; i < 4; ++i) store_piece(grp, base, i);
   };
 
   const uint32_t wave_lds = lds0 + 4 * 2 * kHeadDim * ((uint32_t)__builtin_amdgcn_readfirstlane(wave) & 3);
@@ -314,7 +365,7 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(Prefill
   } else {
     if (grp) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) stg[i] = u32x4{0u, 0u, 0u, 0u};
+      for (int i = 0; i < 4; ++i) stg[i] = Piece<E4M3>{};
       store_tile(2);
     }
     load_tile(0);
@@ -397,8 +448,8 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(Prefill
       if (n + kLdsAhead < 32) ring[n % kLdsAhead] = stream_operand(ks, vs, n + kLdsAhead);
       // staging last: the loads issued at the end of the previous matrix step have had
       // almost a whole iteration (~2 us) to arrive before their registers are stored
-      if (!DIRECT && n >= 24 && n < 28) store_piece(store_at, n - 24);
-      if (!DIRECT && n >= 28 && n < 32) load_piece(kt + 2, n - 28);
+      if (!DIRECT && n >= 24 && n < 28) store_piece(group, store_at, n - 24);
+      if (!DIRECT && n >= 28 && n < 32) load_piece(group, kt + 2, n - 28);
       __builtin_amdgcn_sched_barrier(0);
     }
     // the barrier that follows carries no wait of its own: wait here for the LDS stores
@@ -553,7 +604,7 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(Prefill
 // 16x16x32 form / this one (us, in turn on one board): 1030 tokens on 1000, 32 / 4 heads, bf16 52.0 / 48.0, 1200 on 1400
 // 64.0 / 58.8, 1480 tokens 41.0 / 37.9; 520 on 2000, 64 / 8, f16 62.2 / 56.8; 120 x 9 on 1200, 32 / 4, bf16 38.4 / 36.0.
 // ---------------------------------------------------------------------------
-template <typename T, bool SPLIT>
+template <typename T, bool SPLIT, bool E4M3 = false>
 __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong32_kernel(PrefillKernelArgs p) {
   // K tiles [2][64][kKsPitch] then V tiles [3][64][kVsPitch]
   __shared__ __attribute__((aligned(16))) uint16_t smem[2 * kKsHalves + 3 * kVsHalves];
@@ -608,19 +659,20 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong32_kernel(Prefi
   const float c = p.c;
 
   const size_t plane_at = seq_plane_offset(p.seq_offsets, p.kv_stride_seq, seq) + kvh * p.kv_stride_head;
-  const uint16_t* kplane = p.k + plane_at;
-  const uint16_t* vplane = p.v + plane_at;
+  constexpr uint32_t kElem = kElemBytes[E4M3];
+  const char* kplane = (const char*)p.k + plane_at * kElem;
+  const char* vplane = (const char*)p.v + plane_at * kElem;
 
   const int st_tid = tid & 255;
   const int ld_c = st_tid & 15, ld_r = st_tid >> 4;
-  const uint16_t* plane = grp ? vplane : kplane;                  // wave-uniform
+  const char* plane = grp ? vplane : kplane;                  // wave-uniform
   const uint32_t stride_pos = (uint32_t)p.kv_stride_pos;
   const uint64_t plane_u = uniform64(plane);
-  const uint32_t tile_bytes = kBK * stride_pos * 2;   // (API bound: 64 rows span < 2^32 bytes)
-  const uint64_t valid_bytes = uniform_u64(((uint64_t)kmax * stride_pos + kHeadDim) * 2);
+  const uint32_t tile_bytes = kBK * stride_pos * kElem;   // (API bound: 64 rows span < 2^32 bytes)
+  const uint64_t valid_bytes = uniform_u64(((uint64_t)kmax * stride_pos + kHeadDim) * kElem);
   uint32_t piece_off[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) piece_off[i] = ((ld_r + 16 * i) * stride_pos + 8 * ld_c) * 2;
+  for (int i = 0; i < 4; ++i) piece_off[i] = ((ld_r + 16 * i) * stride_pos + 8 * ld_c) * kElem;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(LdsHalf*)smem;
   auto step_base = [](uint32_t addr) {
     asm volatile("" : "+v"(addr));  // opaque: keeps the compiler from folding the sum another way
@@ -628,20 +680,32 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong32_kernel(Prefi
   };
   const uint32_t ks_store = lds0 + 2 * (ld_r * kKsPitch + 8 * ld_c);
   const uint32_t vs_store = lds0 + 2 * (2 * kKsHalves + ld_r * kVsPitch + 8 * ld_c);
-  u32x4 stg[4];
-  auto load_piece = [&](uint32_t kt, int i) {  // kt (relative to kt0) must be wave-uniform to the compiler
+  Piece<E4M3> stg[4];
+  const uint64_t k_scale_u = E4M3 ? uniform64(p.k_scale + plane_at / kHeadDim) : 0, v_scale_u = E4M3 ? uniform64(p.v_scale + plane_at / kHeadDim) : 0;
+  // kt (relative to kt0) must be wave-uniform to the compiler
+  auto load_piece = [&](auto group, uint32_t kt, int i) __attribute__((always_inline)) {
     const uint64_t off = (uint64_t)(kt0 + kt) * tile_bytes;
     const uint32_t left = bytes_left(valid_bytes, off);
     const __amdgpu_buffer_rsrc_t rsrc =
         __builtin_amdgcn_make_buffer_rsrc((void*)(plane_u + off), 0, left, kBufferFlags);
-    stg[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, piece_off[i], 0, 0);
+    if constexpr (E4M3) {
+      const uint32_t rows = rows_left(left), row = piece_off[i] / kHeadDim;
+      stg[i].codes = __builtin_amdgcn_raw_buffer_load_b64(rsrc, piece_off[i], 0, 0);
+      if (!group)
+        stg[i].k_scale = __builtin_amdgcn_raw_buffer_load_b8(
+            __builtin_amdgcn_make_buffer_rsrc((void*)(k_scale_u + off / kHeadDim), 0, rows, kBufferFlags), row, 0, 0);
+      stg[i].v_scale = __builtin_amdgcn_raw_buffer_load_b8(
+          __builtin_amdgcn_make_buffer_rsrc((void*)(v_scale_u + off / kHeadDim), 0, rows, kBufferFlags), row, 0, 0);
+    } else {
+      stg[i].rows = __builtin_amdgcn_raw_buffer_load_b128(rsrc, piece_off[i], 0, 0);
+    }
   };
-  auto store_piece = [&](auto group, uint32_t base, int i) {
-    *(LdsU32x4*)(base + 2 * 16 * i * (group ? kVsPitch : kKsPitch)) = stg[i];
+  auto store_piece = [&](auto group, uint32_t base, int i) __attribute__((always_inline)) {
+    *(LdsU32x4*)(base + 2 * 16 * i * (group ? kVsPitch : kKsPitch)) = group ? staged<T, false>(stg[i]) : staged<T, true>(stg[i]);
   };
   auto load_tile = [&](uint32_t kt) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_piece(kt, i);
+    for (int i = 0; i < 4; ++i) load_piece(grp, kt, i);
   };
   auto store_base = [&](auto group, int buf) {
     return step_base(group ? vs_store + 2 * buf * kVsHalves : ks_store + 2 * buf * kKsHalves);
@@ -665,7 +729,7 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong32_kernel(Prefi
 
   if (grp) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) stg[i] = u32x4{0u, 0u, 0u, 0u};
+    for (int i = 0; i < 4; ++i) stg[i] = Piece<E4M3>{};
     store_tile(2);
   }
   load_tile(0);
@@ -723,7 +787,7 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong32_kernel(Prefi
       }
       if (n + kLdsAhead < 32) ring[n % kLdsAhead] = stream_operand(ks, vs, n + kLdsAhead);
       if (n >= 24 && n < 28) store_piece(group, store_at, n - 24);
-      if (n >= 28 && n < 32) load_piece(kt + 2, n - 28);
+      if (n >= 28 && n < 32) load_piece(group, kt + 2, n - 28);
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
@@ -859,7 +923,7 @@ constexpr int kStDepth = 2;
 // WAVES = 4, 8 or 12 waves of 32 query rows each: up to 128, 256 or 384 rows of a plane (16, 32
 // or 48 tokens of a sequence with eight heads a group).  Four waves leave room for two
 // workgroups a compute unit; eight and twelve fill a unit with one.
-template <typename T, int WAVES>
+template <typename T, int WAVES, bool E4M3 = false>
 __global__ __launch_bounds__(WAVES * kWave, WAVES == 4 ? 2 : 1) void chunk_stream_kernel(PrefillKernelArgs p) {
   constexpr int DEPTH = kStDepth;
   constexpr int kThreads = WAVES * kWave;
@@ -912,8 +976,9 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 4 ? 2 : 1) void chunk_strea
   const float c = p.c;
 
   const size_t plane_at = seq_plane_offset(p.seq_offsets, p.kv_stride_seq, seq) + kvh * p.kv_stride_head;
-  const uint16_t* kplane = p.k + plane_at;
-  const uint16_t* vplane = p.v + plane_at;
+  constexpr uint32_t kElem = kElemBytes[E4M3];
+  const char* kplane = (const char*)p.k + plane_at * kElem;
+  const char* vplane = (const char*)p.v + plane_at * kElem;
   const uint32_t stride_pos = (uint32_t)p.kv_stride_pos;
   // staging: the first 256 or 512 threads move one 32 x 128 chunk of K and one of V, two or one
   // 16-byte pieces of each (rows ld_r + 16 i or row ld_r, columns 8 ld_c ..), through buffer loads
@@ -921,31 +986,39 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 4 ? 2 : 1) void chunk_strea
   const bool stager = kThreads == kStagers || __builtin_amdgcn_readfirstlane(wave) < kStagers / kWave;
   const int ld_c = tid & 15, ld_r = (tid >> 4) & (kPieceRows - 1);
   const uint64_t kplane_u = uniform64(kplane), vplane_u = uniform64(vplane);
-  const uint32_t chunk_bytes = kCK * stride_pos * 2;
-  const uint64_t valid_bytes = uniform_u64(((uint64_t)kmax * stride_pos + kHeadDim) * 2);
-  const uint32_t piece_off0 = (ld_r * stride_pos + 8 * ld_c) * 2;
-  const uint32_t piece_step = kPieceRows * stride_pos * 2;
-  u32x4 stg[DEPTH][2 * kPieces];
-  auto load_chunk = [&](uint32_t ck, u32x4 (&st)[2 * kPieces]) {  // ck relative to this split's first chunk; wave-uniform
+  const uint32_t chunk_bytes = kCK * stride_pos * kElem;
+  const uint64_t valid_bytes = uniform_u64(((uint64_t)kmax * stride_pos + kHeadDim) * kElem);
+  const uint32_t piece_off0 = (ld_r * stride_pos + 8 * ld_c) * kElem;
+  const uint32_t piece_step = kPieceRows * stride_pos * kElem;
+  Piece<E4M3> stg[DEPTH][2 * kPieces];   // (E4M3: a K piece carries both scales)
+  auto load_chunk = [&](uint32_t ck, Piece<E4M3> (&st)[2 * kPieces]) __attribute__((always_inline)) {  // ck relative to this split's first chunk; wave-uniform
     if (!stager) return;
-    const uint64_t off = (uint64_t)k0 * stride_pos * 2 + (uint64_t)ck * chunk_bytes;
+    const uint64_t off = (uint64_t)k0 * stride_pos * kElem + (uint64_t)ck * chunk_bytes;
     const uint32_t left = bytes_left(valid_bytes, off);
     const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kplane_u + off), 0, left, kBufferFlags);
     const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vplane_u + off), 0, left, kBufferFlags);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-      st[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, piece_off0 + i * piece_step, 0, 2);   // 2: non-temporal, read once
-      st[kPieces + i] = __builtin_amdgcn_raw_buffer_load_b128(vr, piece_off0 + i * piece_step, 0, 2);
+      const uint32_t at = piece_off0 + i * piece_step;
+      if constexpr (E4M3) {
+        st[i].codes = __builtin_amdgcn_raw_buffer_load_b64(kr, at, 0, 2);   // 2: non-temporal, read once
+        st[kPieces + i].codes = __builtin_amdgcn_raw_buffer_load_b64(vr, at, 0, 2);
+        load_scales(p, plane_at + off, left, at, st[i]);
+      } else {
+        st[i].rows = __builtin_amdgcn_raw_buffer_load_b128(kr, at, 0, 2);
+        st[kPieces + i].rows = __builtin_amdgcn_raw_buffer_load_b128(vr, at, 0, 2);
+      }
     }
   };
   const uint32_t lds0 = (uint32_t)(uintptr_t)(LdsHalf*)smem;
   const uint32_t ks_store = lds0 + 2 * (ld_r * kVsPitch + 8 * ld_c), vs_store = ks_store + 2 * 2 * kStHalves;
-  auto store_chunk = [&](uint32_t buf, const u32x4 (&st)[2 * kPieces]) {
+  auto store_chunk = [&](uint32_t buf, Piece<E4M3> (&st)[2 * kPieces]) __attribute__((always_inline)) {
     if (!stager) return;
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-      *(LdsU32x4*)(ks_store + 2 * (buf * kStHalves + kPieceRows * i * kVsPitch)) = st[i];
-      *(LdsU32x4*)(vs_store + 2 * (buf * kStHalves + kPieceRows * i * kVsPitch)) = st[kPieces + i];
+      if constexpr (E4M3) st[kPieces + i].v_scale = st[i].v_scale;
+      *(LdsU32x4*)(ks_store + 2 * (buf * kStHalves + kPieceRows * i * kVsPitch)) = staged<T, true>(st[i]);
+      *(LdsU32x4*)(vs_store + 2 * (buf * kStHalves + kPieceRows * i * kVsPitch)) = staged<T, false>(st[kPieces + i]);
     }
   };
   // operand addresses: as in the kernel above (K rows as the A operand of S^T = K.Q^T, V through
@@ -1113,7 +1186,7 @@ constexpr int kShKsHalves = kSK * kKsPitch, kShVsHalves = kSK * kVsPitch;
 constexpr int kShTileHalves = kShKsHalves + kShVsHalves;
 constexpr int kShRedPitch = kHeadDim + 4;   // floats per row of the merge
 
-template <typename T, int WR, int WK>
+template <typename T, int WR, int WK, bool E4M3 = false>
 __global__ __launch_bounds__(WR* WK* kWave, 2) void short_prompt_kernel(PrefillKernelArgs p) {
   constexpr int kThreads = WR * WK * kWave;
   constexpr int kBufs = WR == 1 ? 1 : 2;        // one wave: its LDS accesses are in order, no second buffer
@@ -1154,22 +1227,37 @@ __global__ __launch_bounds__(WR* WK* kWave, 2) void short_prompt_kernel(PrefillK
   const uint32_t wave_first_pos = P0 + wave_row0 / p.group, wave_last_pos = P0 + wave_row1 / p.group;
 
   const size_t plane_at = seq_plane_offset(p.seq_offsets, p.kv_stride_seq, seq) + kvh * p.kv_stride_head;
-  const uint64_t kplane_u = uniform64(p.k + plane_at), vplane_u = uniform64(p.v + plane_at);
+  constexpr uint32_t kElem = kElemBytes[E4M3];
+  const uint64_t kplane_u = uniform64((const char*)p.k + plane_at * kElem), vplane_u = uniform64((const char*)p.v + plane_at * kElem);
   const uint32_t stride_pos = (uint32_t)p.kv_stride_pos;
-  const uint32_t chunk_bytes = kSK * stride_pos * 2;
-  const uint64_t valid_bytes = uniform_u64(((uint64_t)kmax * stride_pos + kHeadDim) * 2);
+  const uint32_t chunk_bytes = kSK * stride_pos * kElem;
+  const uint64_t valid_bytes = uniform_u64(((uint64_t)kmax * stride_pos + kHeadDim) * kElem);
   const int ld_c = lane & 15, ld_r = 4 * rw + (lane >> 4);   // rows ld_r + 4 WR i of a tile
-  const uint32_t piece_off0 = (ld_r * stride_pos + 8 * ld_c) * 2, piece_step = 4 * WR * stride_pos * 2;
-  u32x4 kst[kPieces], vst[kPieces];
-  auto load_chunk = [&](uint32_t ck) {
+  const uint32_t piece_off0 = (ld_r * stride_pos + 8 * ld_c) * kElem, piece_step = 4 * WR * stride_pos * kElem;
+  Piece<E4M3> kst[kPieces], vst[kPieces];   // (E4M3: a K piece carries both scales)
+  auto load_chunk = [&](uint32_t ck) __attribute__((always_inline)) {
     const uint64_t off = (uint64_t)ck * chunk_bytes;
     const uint32_t left = bytes_left(valid_bytes, off);
     const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kplane_u + off), 0, left, kBufferFlags);
     const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vplane_u + off), 0, left, kBufferFlags);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) kst[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, piece_off0 + i * piece_step, 0, 0);
+    for (int i = 0; i < kPieces; ++i) {
+      const uint32_t at = piece_off0 + i * piece_step;
+      if constexpr (E4M3) {
+        kst[i].codes = __builtin_amdgcn_raw_buffer_load_b64(kr, at, 0, 0);
+        load_scales(p, plane_at + off, left, at, kst[i]);
+      } else {
+        kst[i].rows = __builtin_amdgcn_raw_buffer_load_b128(kr, at, 0, 0);
+      }
+    }
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) vst[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, piece_off0 + i * piece_step, 0, 0);
+    for (int i = 0; i < kPieces; ++i) {
+      const uint32_t at = piece_off0 + i * piece_step;
+      if constexpr (E4M3)
+        vst[i].codes = __builtin_amdgcn_raw_buffer_load_b64(vr, at, 0, 0);
+      else
+        vst[i].rows = __builtin_amdgcn_raw_buffer_load_b128(vr, at, 0, 0);
+    }
   };
   if ((uint32_t)kg < n_chunks) load_chunk(kg);
   u32x4 qreg[8];
@@ -1185,11 +1273,12 @@ __global__ __launch_bounds__(WR* WK* kWave, 2) void short_prompt_kernel(PrefillK
   const uint32_t lds0 = (uint32_t)(uintptr_t)(LdsHalf*)smem + 2 * kg * kBufs * kShTileHalves;
   const uint32_t ks_store = lds0 + 2 * (ld_r * kKsPitch + 8 * ld_c);
   const uint32_t vs_store = lds0 + 2 * (kShKsHalves + ld_r * kVsPitch + 8 * ld_c);
-  auto store_chunk = [&](uint32_t buf) {
+  auto store_chunk = [&](uint32_t buf) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-      *(LdsU32x4*)(ks_store + 2 * (buf * kShTileHalves + 4 * WR * i * kKsPitch)) = kst[i];
-      *(LdsU32x4*)(vs_store + 2 * (buf * kShTileHalves + 4 * WR * i * kVsPitch)) = vst[i];
+      if constexpr (E4M3) vst[i].v_scale = kst[i].v_scale;
+      *(LdsU32x4*)(ks_store + 2 * (buf * kShTileHalves + 4 * WR * i * kKsPitch)) = staged<T, true>(kst[i]);
+      *(LdsU32x4*)(vs_store + 2 * (buf * kShTileHalves + 4 * WR * i * kVsPitch)) = staged<T, false>(vst[i]);
     }
   };
   // operand addresses as in the kernels above
@@ -1415,33 +1504,42 @@ hipError_t launch_chunk(const AttnArgs& a, hipStream_t stream) {
   p.c = c > 0.0f ? c : 1e-37f;
   p.part_o = a.prefill_part_o;
   p.part_ml = a.prefill_part_ml;
+  p.k_scale = a.k_scale;
+  p.v_scale = a.v_scale;
 
   const dim3 grid(plan.n_wg, plan.n_split);
   auto go = [&](auto kernel, uint32_t threads) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, stream, p); };
-  if (plan.kernel == kChunkShort) {
-    if (plan.row_blocks == 2)
-      go(short_prompt_kernel<T, 2, 2>, 4 * kWave);
-    else
-      go(short_prompt_kernel<T, 1, 4>, 4 * kWave);
-  } else if (plan.kernel == kChunkStream) {
-    if (plan.waves == 4)
-      go(chunk_stream_kernel<T, 4>, 4 * kWave);
-    else if (plan.waves == 8)
-      go(chunk_stream_kernel<T, 8>, 8 * kWave);
-    else
-      go(chunk_stream_kernel<T, 12>, 12 * kWave);
-  } else if (plan.n_split == 1) {
-    if (plan.form == kPingpongDirect)
-      go(prefill_pingpong_kernel<T, false, true>, kPpThreads);
-    else if (plan.form == kPingpongWide)
-      go(prefill_pingpong32_kernel<T, false>, kPpThreads);
-    else
-      go(prefill_pingpong_kernel<T, false, false>, kPpThreads);
-  } else if (plan.form == kPingpongWide) {
-    go(prefill_pingpong32_kernel<T, true>, kPpThreads);
-  } else {
-    go(prefill_pingpong_kernel<T, true, false>, kPpThreads);
-  }
+  auto launch = [&](auto e4m3) {
+    constexpr bool E4M3 = decltype(e4m3)::value;
+    if (plan.kernel == kChunkShort) {
+      if (plan.row_blocks == 2)
+        go(short_prompt_kernel<T, 2, 2, E4M3>, 4 * kWave);
+      else
+        go(short_prompt_kernel<T, 1, 4, E4M3>, 4 * kWave);
+    } else if (plan.kernel == kChunkStream) {
+      if (plan.waves == 4)
+        go(chunk_stream_kernel<T, 4, E4M3>, 4 * kWave);
+      else if (plan.waves == 8)
+        go(chunk_stream_kernel<T, 8, E4M3>, 8 * kWave);
+      else
+        go(chunk_stream_kernel<T, 12, E4M3>, 12 * kWave);
+    } else if (plan.n_split == 1) {
+      if (plan.form == kPingpongDirect && !E4M3)
+        go(prefill_pingpong_kernel<T, false, !E4M3, E4M3>, kPpThreads);
+      else if (plan.form == kPingpongWide)
+        go(prefill_pingpong32_kernel<T, false, E4M3>, kPpThreads);
+      else
+        go(prefill_pingpong_kernel<T, false, false, E4M3>, kPpThreads);
+    } else if (plan.form == kPingpongWide) {
+      go(prefill_pingpong32_kernel<T, true, E4M3>, kPpThreads);
+    } else {
+      go(prefill_pingpong_kernel<T, true, false, E4M3>, kPpThreads);
+    }
+  };
+  if (a.k_scale)
+    launch(std::true_type{});
+  else
+    launch(std::false_type{});
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || plan.n_split == 1) return e;
 

@@ -585,17 +585,6 @@ __global__ __launch_bounds__(256) void shaped_merge_kernel(ShapedKernelArgs p) {
 }
 
 template <typename T>
-hipError_t launch_merge(const ShapedKernelArgs& p, hipStream_t stream) {
-  const size_t quads = (size_t)p.interval * p.batch * p.n_q_heads * (kHeadDim / 4);
-  if (p.n_part > 8) {
-    hipLaunchKernelGGL((shaped_merge_kernel<T, 8>), dim3((uint32_t)((quads * 8 + 255) / 256)), dim3(256), 0, stream, p);
-  } else {
-    hipLaunchKernelGGL((shaped_merge_kernel<T, 1>), dim3((uint32_t)((quads + 255) / 256)), dim3(256), 0, stream, p);
-  }
-  return hipGetLastError();
-}
-
-template <typename T>
 hipError_t launch(const ShapedKernelArgs& p, bool cap, bool slopes, bool merge, hipStream_t stream) {
   const dim3 grid(p.own_wgs + p.prefix_tiles * p.prefix_split * p.n_kv_heads), block(kThreads);
   if (cap && slopes)
@@ -606,15 +595,18 @@ hipError_t launch(const ShapedKernelArgs& p, bool cap, bool slopes, bool merge, 
     hipLaunchKernelGGL((shaped_tile_kernel<T, false, true>), grid, block, 0, stream, p);
   else
     hipLaunchKernelGGL((shaped_tile_kernel<T, false, false>), grid, block, 0, stream, p);
-  const hipError_t e = hipGetLastError();
-  return e != hipSuccess || p.whole || !merge ? e : launch_merge<T>(p, stream);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.whole || !merge) return e;
+  const size_t quads = (size_t)p.interval * p.batch * p.n_q_heads * (kHeadDim / 4);
+  if (p.n_part > 8) {
+    hipLaunchKernelGGL((shaped_merge_kernel<T, 8>), dim3((uint32_t)((quads * 8 + 255) / 256)), dim3(256), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL((shaped_merge_kernel<T, 1>), dim3((uint32_t)((quads + 255) / 256)), dim3(256), 0, stream, p);
+  }
+  return hipGetLastError();
 }
 
 }  // namespace
-
-hipError_t launch_shaped_merge(const ShapedKernelArgs& p, int dtype, hipStream_t stream) {
-  return dtype == 0 ? launch_merge<F16>(p, stream) : launch_merge<BF16>(p, stream);
-}
 
 ShapedKernelArgs shaped_kernel_args(const ShapedArgs& args) {
   const AttnArgs& a = args.a;

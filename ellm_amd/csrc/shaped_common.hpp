@@ -41,8 +41,6 @@ struct ShapedKernelArgs {
 
 // The arguments of a call that its plan has no part in.
 ShapedKernelArgs shaped_kernel_args(const ShapedArgs& args);
-// Joins the n_part partial results of every row of a call and finishes the rows.
-hipError_t launch_shaped_merge(const ShapedKernelArgs& p, int dtype, hipStream_t stream);
 
 namespace {
 
