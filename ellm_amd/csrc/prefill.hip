@@ -70,29 +70,11 @@ struct PrefillKernelArgs {
   const uint8_t* v_scale;
 };
 
-// Rows on their way from memory to LDS, eight elements a lane and piece.  E4M3 (the template argument of the kernels below):
-// planes of rows in 8 bits (e4m3.hpp), strides in codes.  Eight codes are eight bytes to load, and their row's scale one
-// more; they are converted between the load's registers and LDS, once for all the rows that read the tile, so that
-// nothing else of a kernel changes.  (A lane of K takes the value row's scale as well: key_scale.)
-template <bool E4M3>
-struct Piece {
-  u32x4 rows;
-};
-template <>
-struct Piece<true> {
-  u32x2 codes;
-  uint32_t k_scale, v_scale;
-};
+// E4M3 (the template argument of the kernels below): planes of rows in 8 bits (e4m3.hpp), strides in codes.  A lane loads sixteen
+// codes at a time and converts them between the load's registers and LDS, once for all the rows that read the tile, so that
+// nothing else of a kernel changes: half the bytes, half the loads, one for a row's scales more, sixteen conversions a lane and tile of 32
+// rows.
 constexpr uint32_t kElemBytes[2] = {2, 1};   // of a plane's element: [E4M3]
-// What a piece is in LDS: of a key row (KEYS) or a value row.
-template <typename T, bool KEYS>
-__device__ __forceinline__ u32x4 staged(const Piece<false>& x) {
-  return x.rows;
-}
-template <typename T, bool KEYS>
-__device__ __forceinline__ u32x4 staged(const Piece<true>& x) {
-  return values8<T>(x.codes, KEYS ? key_scale(x.k_scale, x.v_scale) : value_scale(x.v_scale));
-}
 
 // ---------------------------------------------------------------------------
 // Ping-pong kernel: 8 waves, two per SIMD.  Waves 0-3 and waves 4-7 run the
@@ -147,6 +129,12 @@ typedef __attribute__((address_space(3))) u32x4 LdsU32x4;
 typedef __attribute__((address_space(3))) u32x2 LdsU32x2;
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4 LdsI16x4;
+// Sixteen codes as 16-bit values to LDS address `at`.
+template <typename T>
+__device__ __forceinline__ void store_codes16(uint32_t at, u32x4 codes, uint32_t scale) {
+  *(LdsU32x4*)at = values8<T>(u32x2{codes[0], codes[1]}, scale);
+  *(LdsU32x4*)(at + 16) = values8<T>(u32x2{codes[2], codes[3]}, scale);
+}
 // V rows in LDS: 288 B apart, so that the four rows a 16-lane block of a
 // transposing read touches (32 B of each) fall into disjoint banks
 constexpr int kVsPitch = kHeadDim + 16;
@@ -165,11 +153,11 @@ constexpr int kBufferFlags = 0x00020000;  // raw buffer of 32-bit data, no swizz
 __device__ __forceinline__ uint32_t rows_left(uint32_t left) { return left / kHeadDim + (left % kHeadDim ? 1u : 0u); }
 // The scales of a key row and its value row: of the row that holds byte `at` from byte `off` of the cache's layer on, of which `left`
 // bytes may be read (rows past those: 0).
-__device__ __forceinline__ void load_scales(const PrefillKernelArgs& p, uint64_t off, uint32_t left, uint32_t at, Piece<true>& x) {
+__device__ __forceinline__ void load_scales(const PrefillKernelArgs& p, uint64_t off, uint32_t left, uint32_t at, uint32_t& k, uint32_t& v) {
   const uint32_t rows = rows_left(left);
   const uint64_t ks = uniform64(p.k_scale + off / kHeadDim), vs = uniform64(p.v_scale + off / kHeadDim);
-  x.k_scale = __builtin_amdgcn_raw_buffer_load_b8(__builtin_amdgcn_make_buffer_rsrc((void*)ks, 0, rows, kBufferFlags), at / kHeadDim, 0, 0);
-  x.v_scale = __builtin_amdgcn_raw_buffer_load_b8(__builtin_amdgcn_make_buffer_rsrc((void*)vs, 0, rows, kBufferFlags), at / kHeadDim, 0, 0);
+  k = __builtin_amdgcn_raw_buffer_load_b8(__builtin_amdgcn_make_buffer_rsrc((void*)ks, 0, rows, kBufferFlags), at / kHeadDim, 0, 0);
+  v = __builtin_amdgcn_raw_buffer_load_b8(__builtin_amdgcn_make_buffer_rsrc((void*)vs, 0, rows, kBufferFlags), at / kHeadDim, 0, 0);
 }
 
 // 16 bytes a lane from memory straight to LDS address lds_at + 16 x lane.  Written as asm: the compiler's
@@ -252,8 +240,8 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(Prefill
   // each (rows ld_r + 16 i, columns 8 ld_c ..), K and V alike: V sits in LDS row by
   // row as it does in memory and is transposed by the LDS read (ds_read_b64_tr_b16).
   const int st_tid = tid & 255;
-  const int ld_r = st_tid >> 4;
-  const int ld_c = DIRECT ? (st_tid & 15) ^ (grp ? 2 * (ld_r & 7) : ld_r) : st_tid & 15;
+  const int ld_r = E4M3 ? st_tid >> 3 : st_tid >> 4;
+  const int ld_c = E4M3 ? st_tid & 7 : DIRECT ? (st_tid & 15) ^ (grp ? 2 * (ld_r & 7) : ld_r) : st_tid & 15;
   const char* plane = grp ? vplane : kplane;                  // wave-uniform
   const uint32_t stride_pos = (uint32_t)p.kv_stride_pos;
   // Tiles are fetched with buffer loads: the descriptor (base of tile kt, bytes
@@ -270,7 +258,7 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(Prefill
   const uint64_t valid_bytes = uniform_u64(((uint64_t)kmax * stride_pos + kHeadDim) * kElem);
   uint32_t piece_off[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) piece_off[i] = ((ld_r + 16 * i) * stride_pos + 8 * ld_c) * kElem;
+  for (int i = 0; i < 4; ++i) piece_off[i] = E4M3 ? (ld_r + 32 * i) * stride_pos + 16 * ld_c : ((ld_r + 16 * i) * stride_pos + 8 * ld_c) * 2;
   // LDS addresses are kept as byte offsets: the buffers span more than the 64 KB an
   // instruction's immediate offset reaches, so each step forms one base register
   // per tile (step_base) and everything else is an immediate on top of it.
@@ -279,9 +267,11 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(Prefill
     asm volatile("" : "+v"(addr));  // opaque: keeps the compiler from folding the sum another way
     return addr;
   };
-  const uint32_t ks_store = lds0 + 2 * (ld_r * kVsPitch + 8 * ld_c);
+  const uint32_t ks_store = lds0 + 2 * (ld_r * kVsPitch + (E4M3 ? 16 : 8) * ld_c);
   const uint32_t vs_store = ks_store + 2 * 2 * kVsHalves;
-  Piece<E4M3> stg[4];
+  // E4M3: sixteen codes a load (rows ld_r + 32 i, codes 16 ld_c ..), two pieces of LDS each
+  u32x4 stg[4];   // (E4M3: codes of two rows)
+  uint32_t k_scales[2], v_scales[2];
   const uint64_t k_scale_u = E4M3 ? uniform64(p.k_scale + plane_at / kHeadDim) : 0, v_scale_u = E4M3 ? uniform64(p.v_scale + plane_at / kHeadDim) : 0;
   // kt (relative to kt0) must be wave-uniform to the compiler
   auto load_piece = [&](auto group, uint32_t kt, int i) __attribute__((always_inline)) {
@@ -290,34 +280,43 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(Prefill
     const __amdgpu_buffer_rsrc_t rsrc =
         __builtin_amdgcn_make_buffer_rsrc((void*)(plane_u + off), 0, left, kBufferFlags);
     if constexpr (E4M3) {
-      const uint32_t rows = rows_left(left), row = piece_off[i] / kHeadDim;
-      stg[i].codes = __builtin_amdgcn_raw_buffer_load_b64(rsrc, piece_off[i], 0, 0);
-      if (!group)
-        stg[i].k_scale = __builtin_amdgcn_raw_buffer_load_b8(
-            __builtin_amdgcn_make_buffer_rsrc((void*)(k_scale_u + off / kHeadDim), 0, rows, kBufferFlags), row, 0, 0);
-      stg[i].v_scale = __builtin_amdgcn_raw_buffer_load_b8(
-          __builtin_amdgcn_make_buffer_rsrc((void*)(v_scale_u + off / kHeadDim), 0, rows, kBufferFlags), row, 0, 0);
+      if (i < 2) {
+        stg[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, piece_off[i], 0, 0);
+        return;
+      }
+      const uint32_t rows = rows_left(left), row = piece_off[i - 2] / kHeadDim;
+      const __amdgpu_buffer_rsrc_t ks = __builtin_amdgcn_make_buffer_rsrc((void*)(k_scale_u + off / kHeadDim), 0, rows, kBufferFlags),
+                                   vs = __builtin_amdgcn_make_buffer_rsrc((void*)(v_scale_u + off / kHeadDim), 0, rows, kBufferFlags);
+      if (!group) k_scales[i - 2] = __builtin_amdgcn_raw_buffer_load_b8(ks, row, 0, 0);
+      v_scales[i - 2] = __builtin_amdgcn_raw_buffer_load_b8(vs, row, 0, 0);
     } else {
-      stg[i].rows = __builtin_amdgcn_raw_buffer_load_b128(rsrc, piece_off[i], 0, 0);
+      stg[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, piece_off[i], 0, 0);
     }
   };
   // (the group comes as a compile-time constant where the caller runs behind the scalar
   // branch on the group, as the run-time value in the prologue)
   // base: step_base of this lane's place in the destination buffer
   auto store_piece = [&](auto group, uint32_t base, int i) __attribute__((always_inline)) {
-    *(LdsU32x4*)(base + 2 * 16 * i * kVsPitch) = group ? staged<T, false>(stg[i]) : staged<T, true>(stg[i]);
+    const uint32_t pitch = 2 * (uint32_t)kVsPitch;
+    if constexpr (E4M3) {
+      const u32x4& x = stg[i >> 1];
+      *(LdsU32x4*)(base + 32 * (i >> 1) * pitch + 16 * (i & 1)) =
+          values8<T>(u32x2{x[2 * (i & 1)], x[2 * (i & 1) + 1]}, group ? value_scale(v_scales[i >> 1]) : key_scale(k_scales[i >> 1], v_scales[i >> 1]));
+    } else {
+      *(LdsU32x4*)(base + 16 * i * pitch) = stg[i];
+    }
   };
-  auto load_tile = [&](uint32_t kt) {
+  auto load_tile = [&](auto group, uint32_t kt) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_piece(grp, kt, i);
+    for (int i = 0; i < 4; ++i) load_piece(group, kt, i);
   };
   auto store_base = [&](auto group, int buf) {
     return step_base((group ? vs_store : ks_store) + 2 * buf * kVsHalves);
   };
-  auto store_tile = [&](int buf) {
-    const uint32_t base = store_base(grp, buf);
+  auto store_tile = [&](auto group, int buf) __attribute__((always_inline)) {
+    const uint32_t base = store_base(group, buf);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) store_piece(grp, base, i);
+    for (int i = 0; i < 4; ++i) store_piece(group, base, i);
   };
 
   const uint32_t wave_lds = lds0 + 4 * 2 * kHeadDim * ((uint32_t)__builtin_amdgcn_readfirstlane(wave) & 3);
@@ -363,14 +362,24 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(Prefill
     for (int kt = 0; kt < kPpAhead; ++kt) load_direct(grp, kt);
     asm volatile("s_waitcnt vmcnt(8)" ::: "memory");   // 4 (kPpAhead - 1): tile 0 is there
   } else {
-    if (grp) {
+    auto begin = [&](auto group) __attribute__((always_inline)) {
+      if (group) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) stg[i] = Piece<E4M3>{};
-      store_tile(2);
+        for (int i = 0; i < 4; ++i) stg[i] = u32x4{0u, 0u, 0u, 0u};
+        store_tile(group, 2);
+      }
+      load_tile(group, 0);
+      store_tile(group, 0);
+      load_tile(group, 1);
+    };
+    if constexpr (E4M3) {   // (its loads differ between the groups)
+      if (__builtin_amdgcn_readfirstlane(grp))
+        begin(std::integral_constant<int, 1>{});
+      else
+        begin(std::integral_constant<int, 0>{});
+    } else {
+      begin(grp);
     }
-    load_tile(0);
-    store_tile(0);
-    load_tile(1);
   }
   __syncthreads();
 
@@ -664,7 +673,7 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong32_kernel(Prefi
   const char* vplane = (const char*)p.v + plane_at * kElem;
 
   const int st_tid = tid & 255;
-  const int ld_c = st_tid & 15, ld_r = st_tid >> 4;
+  const int ld_c = E4M3 ? st_tid & 7 : st_tid & 15, ld_r = E4M3 ? st_tid >> 3 : st_tid >> 4;
   const char* plane = grp ? vplane : kplane;                  // wave-uniform
   const uint32_t stride_pos = (uint32_t)p.kv_stride_pos;
   const uint64_t plane_u = uniform64(plane);
@@ -672,15 +681,18 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong32_kernel(Prefi
   const uint64_t valid_bytes = uniform_u64(((uint64_t)kmax * stride_pos + kHeadDim) * kElem);
   uint32_t piece_off[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) piece_off[i] = ((ld_r + 16 * i) * stride_pos + 8 * ld_c) * kElem;
+  for (int i = 0; i < 4; ++i) piece_off[i] = E4M3 ? (ld_r + 32 * i) * stride_pos + 16 * ld_c : ((ld_r + 16 * i) * stride_pos + 8 * ld_c) * 2;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(LdsHalf*)smem;
   auto step_base = [](uint32_t addr) {
     asm volatile("" : "+v"(addr));  // opaque: keeps the compiler from folding the sum another way
     return addr;
   };
-  const uint32_t ks_store = lds0 + 2 * (ld_r * kKsPitch + 8 * ld_c);
-  const uint32_t vs_store = lds0 + 2 * (2 * kKsHalves + ld_r * kVsPitch + 8 * ld_c);
-  Piece<E4M3> stg[4];
+  constexpr int kLoad = E4M3 ? 16 : 8;   // elements
+  const uint32_t ks_store = lds0 + 2 * (ld_r * kKsPitch + kLoad * ld_c);
+  const uint32_t vs_store = lds0 + 2 * (2 * kKsHalves + ld_r * kVsPitch + kLoad * ld_c);
+  // E4M3: sixteen codes a load (rows ld_r + 32 i, codes 16 ld_c ..), two pieces of LDS each
+  u32x4 stg[4];   // (E4M3: codes of two rows)
+  uint32_t k_scales[2], v_scales[2];
   const uint64_t k_scale_u = E4M3 ? uniform64(p.k_scale + plane_at / kHeadDim) : 0, v_scale_u = E4M3 ? uniform64(p.v_scale + plane_at / kHeadDim) : 0;
   // kt (relative to kt0) must be wave-uniform to the compiler
   auto load_piece = [&](auto group, uint32_t kt, int i) __attribute__((always_inline)) {
@@ -689,31 +701,40 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong32_kernel(Prefi
     const __amdgpu_buffer_rsrc_t rsrc =
         __builtin_amdgcn_make_buffer_rsrc((void*)(plane_u + off), 0, left, kBufferFlags);
     if constexpr (E4M3) {
-      const uint32_t rows = rows_left(left), row = piece_off[i] / kHeadDim;
-      stg[i].codes = __builtin_amdgcn_raw_buffer_load_b64(rsrc, piece_off[i], 0, 0);
-      if (!group)
-        stg[i].k_scale = __builtin_amdgcn_raw_buffer_load_b8(
-            __builtin_amdgcn_make_buffer_rsrc((void*)(k_scale_u + off / kHeadDim), 0, rows, kBufferFlags), row, 0, 0);
-      stg[i].v_scale = __builtin_amdgcn_raw_buffer_load_b8(
-          __builtin_amdgcn_make_buffer_rsrc((void*)(v_scale_u + off / kHeadDim), 0, rows, kBufferFlags), row, 0, 0);
+      if (i < 2) {
+        stg[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, piece_off[i], 0, 0);
+        return;
+      }
+      const uint32_t rows = rows_left(left), row = piece_off[i - 2] / kHeadDim;
+      const __amdgpu_buffer_rsrc_t ks = __builtin_amdgcn_make_buffer_rsrc((void*)(k_scale_u + off / kHeadDim), 0, rows, kBufferFlags),
+                                   vs = __builtin_amdgcn_make_buffer_rsrc((void*)(v_scale_u + off / kHeadDim), 0, rows, kBufferFlags);
+      if (!group) k_scales[i - 2] = __builtin_amdgcn_raw_buffer_load_b8(ks, row, 0, 0);
+      v_scales[i - 2] = __builtin_amdgcn_raw_buffer_load_b8(vs, row, 0, 0);
     } else {
-      stg[i].rows = __builtin_amdgcn_raw_buffer_load_b128(rsrc, piece_off[i], 0, 0);
+      stg[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, piece_off[i], 0, 0);
     }
   };
   auto store_piece = [&](auto group, uint32_t base, int i) __attribute__((always_inline)) {
-    *(LdsU32x4*)(base + 2 * 16 * i * (group ? kVsPitch : kKsPitch)) = group ? staged<T, false>(stg[i]) : staged<T, true>(stg[i]);
+    const uint32_t pitch = 2 * (uint32_t)(group ? kVsPitch : kKsPitch);
+    if constexpr (E4M3) {
+      const u32x4& x = stg[i >> 1];
+      *(LdsU32x4*)(base + 32 * (i >> 1) * pitch + 16 * (i & 1)) =
+          values8<T>(u32x2{x[2 * (i & 1)], x[2 * (i & 1) + 1]}, group ? value_scale(v_scales[i >> 1]) : key_scale(k_scales[i >> 1], v_scales[i >> 1]));
+    } else {
+      *(LdsU32x4*)(base + 16 * i * pitch) = stg[i];
+    }
   };
-  auto load_tile = [&](uint32_t kt) {
+  auto load_tile = [&](auto group, uint32_t kt) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_piece(grp, kt, i);
+    for (int i = 0; i < 4; ++i) load_piece(group, kt, i);
   };
   auto store_base = [&](auto group, int buf) {
     return step_base(group ? vs_store + 2 * buf * kVsHalves : ks_store + 2 * buf * kKsHalves);
   };
-  auto store_tile = [&](int buf) {
-    const uint32_t base = store_base(grp, buf);
+  auto store_tile = [&](auto group, int buf) __attribute__((always_inline)) {
+    const uint32_t base = store_base(group, buf);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) store_piece(grp, base, i);
+    for (int i = 0; i < 4; ++i) store_piece(group, base, i);
   };
 
   float m_run = -INFINITY, l_run = 0.0f;
@@ -727,14 +748,24 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong32_kernel(Prefi
 #pragma unroll
   for (int cc = 0; cc < 4; ++cc) pk[cc] = u32x4{0u, 0u, 0u, 0u};  // P(-1) = 0
 
-  if (grp) {
+  auto begin = [&](auto group) __attribute__((always_inline)) {
+    if (group) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) stg[i] = Piece<E4M3>{};
-    store_tile(2);
+      for (int i = 0; i < 4; ++i) stg[i] = u32x4{0u, 0u, 0u, 0u};
+      store_tile(group, 2);
+    }
+    load_tile(group, 0);
+    store_tile(group, 0);
+    load_tile(group, 1);
+  };
+  if constexpr (E4M3) {   // (its loads differ between the groups)
+    if (__builtin_amdgcn_readfirstlane(grp))
+      begin(std::integral_constant<int, 1>{});
+    else
+      begin(std::integral_constant<int, 0>{});
+  } else {
+    begin(grp);
   }
-  load_tile(0);
-  store_tile(0);
-  load_tile(1);
   __syncthreads();
 
   // A operand of P.V (rows = 32 dims, 16 keys): lane (dim j, key half g) holds keys {4g..4g+3, 8+4g..8+4g+3} of the
@@ -990,35 +1021,49 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 4 ? 2 : 1) void chunk_strea
   const uint64_t valid_bytes = uniform_u64(((uint64_t)kmax * stride_pos + kHeadDim) * kElem);
   const uint32_t piece_off0 = (ld_r * stride_pos + 8 * ld_c) * kElem;
   const uint32_t piece_step = kPieceRows * stride_pos * kElem;
-  Piece<E4M3> stg[DEPTH][2 * kPieces];   // (E4M3: a K piece carries both scales)
-  auto load_chunk = [&](uint32_t ck, Piece<E4M3> (&st)[2 * kPieces]) __attribute__((always_inline)) {  // ck relative to this split's first chunk; wave-uniform
+  // (E4M3: sixteen codes a load, a chunk of K or of V in 256 of them: a thread moves a load of each, or, where twice as many threads
+  // move them, one of either)
+  constexpr bool kOneEach = E4M3 && kStagers == kStStagersMax;
+  const bool moves_v = kOneEach && __builtin_amdgcn_readfirstlane(wave) >= 4;
+  const int ld_r8 = (tid >> 3) & 31, ld_x8 = tid & 7;
+  struct Staged {
+    u32x4 rows[E4M3 ? (kOneEach ? 1 : 2) : 2 * kPieces];
+    uint32_t k_scale, v_scale;
+  };
+  Staged stg[DEPTH];
+  auto load_chunk = [&](uint32_t ck, Staged& st) __attribute__((always_inline)) {  // ck relative to this split's first chunk; wave-uniform
     if (!stager) return;
     const uint64_t off = (uint64_t)k0 * stride_pos * kElem + (uint64_t)ck * chunk_bytes;
     const uint32_t left = bytes_left(valid_bytes, off);
     const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kplane_u + off), 0, left, kBufferFlags);
     const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vplane_u + off), 0, left, kBufferFlags);
+    if constexpr (E4M3) {   // (2: non-temporal, read once)
+      const uint32_t at = ld_r8 * stride_pos + 16 * ld_x8;
+      if (!moves_v) st.rows[0] = __builtin_amdgcn_raw_buffer_load_b128(kr, at, 0, 2);
+      if (!kOneEach || moves_v) st.rows[kOneEach ? 0 : 1] = __builtin_amdgcn_raw_buffer_load_b128(vr, at, 0, 2);
+      load_scales(p, plane_at + off, left, at, st.k_scale, st.v_scale);
+    } else {
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const uint32_t at = piece_off0 + i * piece_step;
-      if constexpr (E4M3) {
-        st[i].codes = __builtin_amdgcn_raw_buffer_load_b64(kr, at, 0, 2);   // 2: non-temporal, read once
-        st[kPieces + i].codes = __builtin_amdgcn_raw_buffer_load_b64(vr, at, 0, 2);
-        load_scales(p, plane_at + off, left, at, st[i]);
-      } else {
-        st[i].rows = __builtin_amdgcn_raw_buffer_load_b128(kr, at, 0, 2);
-        st[kPieces + i].rows = __builtin_amdgcn_raw_buffer_load_b128(vr, at, 0, 2);
+      for (int i = 0; i < kPieces; ++i) {
+        st.rows[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, piece_off0 + i * piece_step, 0, 2);   // 2: non-temporal, read once
+        st.rows[kPieces + i] = __builtin_amdgcn_raw_buffer_load_b128(vr, piece_off0 + i * piece_step, 0, 2);
       }
     }
   };
   const uint32_t lds0 = (uint32_t)(uintptr_t)(LdsHalf*)smem;
-  const uint32_t ks_store = lds0 + 2 * (ld_r * kVsPitch + 8 * ld_c), vs_store = ks_store + 2 * 2 * kStHalves;
-  auto store_chunk = [&](uint32_t buf, Piece<E4M3> (&st)[2 * kPieces]) __attribute__((always_inline)) {
+  const uint32_t ks_store = lds0 + 2 * (E4M3 ? ld_r8 * kVsPitch + 16 * ld_x8 : ld_r * kVsPitch + 8 * ld_c), vs_store = ks_store + 2 * 2 * kStHalves;
+  auto store_chunk = [&](uint32_t buf, const Staged& st) __attribute__((always_inline)) {
     if (!stager) return;
+    if constexpr (E4M3) {
+      const uint32_t k_scale = key_scale(st.k_scale, st.v_scale), v_scale = value_scale(st.v_scale);
+      if (!moves_v) store_codes16<T>(ks_store + 2 * buf * kStHalves, st.rows[0], k_scale);
+      if (!kOneEach || moves_v) store_codes16<T>(vs_store + 2 * buf * kStHalves, st.rows[kOneEach ? 0 : 1], v_scale);
+    } else {
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      if constexpr (E4M3) st[kPieces + i].v_scale = st[i].v_scale;
-      *(LdsU32x4*)(ks_store + 2 * (buf * kStHalves + kPieceRows * i * kVsPitch)) = staged<T, true>(st[i]);
-      *(LdsU32x4*)(vs_store + 2 * (buf * kStHalves + kPieceRows * i * kVsPitch)) = staged<T, false>(st[kPieces + i]);
+      for (int i = 0; i < kPieces; ++i) {
+        *(LdsU32x4*)(ks_store + 2 * (buf * kStHalves + kPieceRows * i * kVsPitch)) = st.rows[i];
+        *(LdsU32x4*)(vs_store + 2 * (buf * kStHalves + kPieceRows * i * kVsPitch)) = st.rows[kPieces + i];
+      }
     }
   };
   // operand addresses: as in the kernel above (K rows as the A operand of S^T = K.Q^T, V through
@@ -1234,30 +1279,23 @@ __global__ __launch_bounds__(WR* WK* kWave, 2) void short_prompt_kernel(PrefillK
   const uint64_t valid_bytes = uniform_u64(((uint64_t)kmax * stride_pos + kHeadDim) * kElem);
   const int ld_c = lane & 15, ld_r = 4 * rw + (lane >> 4);   // rows ld_r + 4 WR i of a tile
   const uint32_t piece_off0 = (ld_r * stride_pos + 8 * ld_c) * kElem, piece_step = 4 * WR * stride_pos * kElem;
-  Piece<E4M3> kst[kPieces], vst[kPieces];   // (E4M3: a K piece carries both scales)
+  // (E4M3: sixteen codes a load, rows ld_r8 + 8 WR i of a tile; lane l of a wave fetches the scales of the tile's row l % 32, which
+  // lane exchanges hand to those that need them)
+  constexpr int kLoads = E4M3 ? kPieces / 2 : kPieces;
+  const int ld_r8 = 8 * rw + (lane >> 3), ld_x8 = lane & 7;
+  u32x4 kst[kLoads], vst[kLoads];
+  uint32_t k_scale, v_scale;
   auto load_chunk = [&](uint32_t ck) __attribute__((always_inline)) {
     const uint64_t off = (uint64_t)ck * chunk_bytes;
     const uint32_t left = bytes_left(valid_bytes, off);
     const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kplane_u + off), 0, left, kBufferFlags);
     const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vplane_u + off), 0, left, kBufferFlags);
+    const uint32_t at = E4M3 ? ld_r8 * stride_pos + 16 * ld_x8 : piece_off0, step = E4M3 ? 8 * WR * stride_pos : piece_step;
+    if constexpr (E4M3) load_scales(p, plane_at + off, left, (lane & 31) * stride_pos, k_scale, v_scale);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const uint32_t at = piece_off0 + i * piece_step;
-      if constexpr (E4M3) {
-        kst[i].codes = __builtin_amdgcn_raw_buffer_load_b64(kr, at, 0, 0);
-        load_scales(p, plane_at + off, left, at, kst[i]);
-      } else {
-        kst[i].rows = __builtin_amdgcn_raw_buffer_load_b128(kr, at, 0, 0);
-      }
-    }
+    for (int i = 0; i < kLoads; ++i) kst[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, at + i * step, 0, 0);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const uint32_t at = piece_off0 + i * piece_step;
-      if constexpr (E4M3)
-        vst[i].codes = __builtin_amdgcn_raw_buffer_load_b64(vr, at, 0, 0);
-      else
-        vst[i].rows = __builtin_amdgcn_raw_buffer_load_b128(vr, at, 0, 0);
-    }
+    for (int i = 0; i < kLoads; ++i) vst[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, at + i * step, 0, 0);
   };
   if ((uint32_t)kg < n_chunks) load_chunk(kg);
   u32x4 qreg[8];
@@ -1271,14 +1309,23 @@ __global__ __launch_bounds__(WR* WK* kWave, 2) void short_prompt_kernel(PrefillK
   }
   const float c = p.c;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(LdsHalf*)smem + 2 * kg * kBufs * kShTileHalves;
-  const uint32_t ks_store = lds0 + 2 * (ld_r * kKsPitch + 8 * ld_c);
-  const uint32_t vs_store = lds0 + 2 * (kShKsHalves + ld_r * kVsPitch + 8 * ld_c);
+  const uint32_t ks_store = lds0 + 2 * (E4M3 ? ld_r8 * kKsPitch + 16 * ld_x8 : ld_r * kKsPitch + 8 * ld_c);
+  const uint32_t vs_store = lds0 + 2 * (kShKsHalves + (E4M3 ? ld_r8 * kVsPitch + 16 * ld_x8 : ld_r * kVsPitch + 8 * ld_c));
   auto store_chunk = [&](uint32_t buf) __attribute__((always_inline)) {
+    if constexpr (E4M3) {
+      const int ks = (int)key_scale(k_scale, v_scale), vs = (int)value_scale(v_scale);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      if constexpr (E4M3) vst[i].v_scale = kst[i].v_scale;
-      *(LdsU32x4*)(ks_store + 2 * (buf * kShTileHalves + 4 * WR * i * kKsPitch)) = staged<T, true>(kst[i]);
-      *(LdsU32x4*)(vs_store + 2 * (buf * kShTileHalves + 4 * WR * i * kVsPitch)) = staged<T, false>(vst[i]);
+      for (int i = 0; i < kLoads; ++i) {
+        const int row = ld_r8 + 8 * WR * i;
+        store_codes16<T>(ks_store + 2 * (buf * kShTileHalves + 8 * WR * i * kKsPitch), kst[i], (uint32_t)__shfl(ks, row));
+        store_codes16<T>(vs_store + 2 * (buf * kShTileHalves + 8 * WR * i * kVsPitch), vst[i], (uint32_t)__shfl(vs, row));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        *(LdsU32x4*)(ks_store + 2 * (buf * kShTileHalves + 4 * WR * i * kKsPitch)) = kst[i];
+        *(LdsU32x4*)(vs_store + 2 * (buf * kShTileHalves + 4 * WR * i * kVsPitch)) = vst[i];
+      }
     }
   };
   // operand addresses as in the kernels above
