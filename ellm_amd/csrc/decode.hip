@@ -181,7 +181,7 @@ hipError_t launch_decode(const AttnArgs& a, hipStream_t stream, const ShapedStat
   p.split_len = a.split_len;
   p.n_split = a.n_split;
   p.batch = a.batch;
-  p.scale_log2 = a.scale * kLog2e;
+  p.scale_log2 = a.k_scale ? scale_log2_e4m3(a.scale) : a.scale * kLog2e;
   p.pend = a.pending;
   p.k_scale = a.k_scale;
   p.v_scale = a.v_scale;

@@ -330,7 +330,7 @@ hipError_t launch_decode_balanced(const AttnArgs& a, uint32_t wgs, hipStream_t s
   p.n_split = 0;
   p.batch = a.batch;
   p.wgs_one = a.n_cu ? a.n_cu : wgs;
-  p.scale_log2 = a.scale * kLog2e;
+  p.scale_log2 = a.k_scale ? scale_log2_e4m3(a.scale) : a.scale * kLog2e;
   // cluster slots (the kernel's cslot0 + cluster stays below this): the planes' own counters follow
   const uint32_t planes = a.batch * a.n_kv_heads * p.head_groups;
   p.n_cluster_max = balanced_cluster_slots(wgs, planes);

@@ -21,6 +21,13 @@ namespace dec {
 
 constexpr int kChunk8 = 32;   // keys per wave step
 
+// The scale of the scores in log2 units.  (A score that is hidden is an infinity times this: a scale of zero is taken as one that no
+// finite product feels.)
+inline float scale_log2_e4m3(float scale) {
+  const float x = scale * kLog2e;
+  return x >= 1e-37f || x <= -1e-37f || !(x == x) ? x : 1e-37f;
+}
+
 // Query heads of a group as the B operand that goes with the keys' own order of dims: lane (head c, group g) holds
 // q[head][64 (s >> 1) + 16 g + 8 (s & 1) + 0..7] for s = 0..3; heads past the group's end are zero.
 __device__ __forceinline__ void load_queries8(const uint16_t* q_rows, const Lane& t, uint32_t heads_here, u32x4 (&qreg)[4]) {
@@ -38,6 +45,12 @@ struct Chunk8 {
   uint32_t scale;
 };
 
+__device__ __forceinline__ uint32_t scalar(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+__device__ __forceinline__ uint64_t scalar64(uint64_t x) {
+  return ((uint64_t)scalar((uint32_t)(x >> 32)) << 32) | (uint64_t)scalar((uint32_t)x);
+}
+constexpr int kNonTemporal = 2;   // cache policy of a buffer load: streamed, not kept
+
 // One wave's share of keys [k_begin, k_end) of a plane, as stream_keys; acc[b][r] of lane (head c, group g) is column
 // 32 g + 8 r + b.  k_end is the plane's end (pos + 1) or a multiple of kChunk8 from k_begin on.
 template <typename T>
@@ -45,36 +58,44 @@ __device__ __forceinline__ void stream_keys8(const DecodeKernelArgs& p, size_t p
                                              uint32_t pos, const u32x4 (&qreg)[4], uint16_t* smem, const Lane& t,
                                              uint32_t rot_seed, float& m_out, float& l_out, f32x4 (&acc)[8]) {
   const int g = t.g, c = t.c;
-  uint8_t* const scales = (uint8_t*)smem + t.wave * (2 * kChunk8);   // [keys' 32][values' 32]
-  const uint8_t* const kp = (const uint8_t*)p.k + plane + 16 * g;
-  const uint8_t* const vp = (const uint8_t*)p.v + plane + 8 * c;
+  const uint32_t wave = scalar(t.wave);
+  uint8_t* const scales = (uint8_t*)smem + wave * (2 * kChunk8);   // [keys' 32][values' 32]
+  // Rows are fetched through buffer descriptors that begin with the chunk and end with the plane's last row (rows past it read as
+  // zeros, and weigh nothing): scalar arithmetic, the lanes' own offsets never change.
+  const uint64_t at_plane = scalar64(plane), kp = scalar64((uint64_t)p.k + at_plane), vp = scalar64((uint64_t)p.v + at_plane);
+  const uint32_t pitch = (uint32_t)p.kv_stride_pos, scale_pitch = pitch / kHeadDim;
+  const uint32_t k_off = c * pitch + 16 * g;
+  uint32_t v_off[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v_off[e] = (16 * (e >> 2) + 4 * g + (e & 3)) * pitch + 8 * c;
   const uint8_t* const sp = (t.lane < kChunk8 ? p.k_scale : p.v_scale) + plane / kHeadDim;
-  const size_t pitch = p.kv_stride_pos, scale_pitch = pitch / kHeadDim;
 
   const uint32_t n_chunks = (k_end - k_begin + kChunk8 - 1) / kChunk8;
-  const uint32_t my_chunks = n_chunks > (uint32_t)t.wave ? (n_chunks - t.wave + kDecWaves - 1) / kDecWaves : 0;
-  const uint32_t rot = rot_seed % max(my_chunks, 1u);
+  const uint32_t my_chunks = n_chunks > wave ? (n_chunks - wave + kDecWaves - 1) / kDecWaves : 0;
+  const uint32_t rot = scalar(rot_seed % max(my_chunks, 1u));
   auto first_key = [&](uint32_t it) {
     uint32_t r = it + rot;
     if (r >= my_chunks) r -= my_chunks;
-    return k_begin + (t.wave + r * kDecWaves) * kChunk8;
+    return scalar(k_begin + (wave + r * kDecWaves) * kChunk8);
   };
-  // (rows past the last key are clamped onto it: always in bounds, and their weights are zero)
   auto fetch = [&](Chunk8& x, uint32_t it) __attribute__((always_inline)) {
     const uint32_t kb = first_key(it);
-    x.scale = sp[min(kb + (t.lane & (kChunk8 - 1)), pos) * scale_pitch];
+    const uint64_t off = (uint64_t)kb * pitch, left = (uint64_t)(pos - kb) * pitch + kHeadDim;
+    const uint32_t bytes = scalar(left >> 32 ? 0xffffffffu : (uint32_t)left);
+    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kp + off), 0, bytes, 0x00020000);
+    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vp + off), 0, bytes, 0x00020000);
+    x.scale = sp[(size_t)min(kb + (t.lane & (kChunk8 - 1)), pos) * scale_pitch];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const uint8_t* row = kp + min(kb + 16 * b + c, pos) * pitch;
-      x.k[b][0] = load16_once(row);
-      x.k[b][1] = load16_once(row + 64);
-    }
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      x.v[e] = __builtin_nontemporal_load((const u32x2*)(vp + min(kb + 16 * (e >> 2) + 4 * g + (e & 3), pos) * pitch));
+      for (int h = 0; h < 2; ++h)
+        x.k[b][h] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_off + 16 * b * pitch + 64 * h, 0, kNonTemporal);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x.v[e] = __builtin_amdgcn_raw_buffer_load_b64(vr, v_off[e], 0, kNonTemporal);
   };
 
   float m_run = -INFINITY, l_run = 0.0f;
+  const float hidden = p.scale_log2 < 0.0f ? INFINITY : -INFINITY;   // (a product that comes out as -inf)
 #pragma unroll
   for (int b = 0; b < 8; ++b) acc[b] = f32x4{0, 0, 0, 0};
 
@@ -85,50 +106,52 @@ __device__ __forceinline__ void stream_keys8(const DecodeKernelArgs& p, size_t p
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const float scale = scale_of(scales[16 * b + c]);
-      st[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         const u32x2 lo = values4<T>(x.k[b][s >> 1][2 * (s & 1)], scale), hi = values4<T>(x.k[b][s >> 1][2 * (s & 1) + 1], scale);
-        st[b] = Mfma<T>::m16x16x32(u32x4{lo[0], lo[1], hi[0], hi[1]}, qreg[s], st[b]);
+        st[b] = Mfma<T>::m16x16x32(u32x4{lo[0], lo[1], hi[0], hi[1]}, qreg[s], s ? st[b] : f32x4{0, 0, 0, 0});
       }
     }
-    float y[8], top = -INFINITY;
+    if (kb + kChunk8 - 1 > pos) {   // (uniform: the plane's last chunk)
+      const int32_t seen = (int32_t)(pos - kb) - 4 * g;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      y[e] = kb + 16 * (e >> 2) + 4 * g + (e & 3) <= pos ? st[e >> 2][e & 3] * p.scale_log2 : -INFINITY;
-      top = fmaxf(top, y[e]);
+      for (int e = 0; e < 8; ++e) st[e >> 2][e & 3] = 16 * (e >> 2) + (e & 3) <= seen ? st[e >> 2][e & 3] : hidden;
     }
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, st[e >> 2][e & 3] * p.scale_log2);
     top = max_with_partner_half(top);
     float a = top, b16 = top;
     swap_rows16(a, b16);
-    const float m_new = fmaxf(m_run, fmaxf(a, b16));   // (finite: key kb is always valid)
-    const float alpha = fast_exp2(m_run - m_new);
-    float sum = 0.0f;
+    const float m_new = fmaxf(m_run, fmaxf(a, b16));   // (key kb is always valid: finite, unless its row is NaN)
+    if (__any(m_new != m_run)) {
+      const float alpha = fast_exp2(m_run - m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int b = 0; b < 8; ++b) acc[b] *= alpha;
+      m_run = m_new;
+    }
+    float y[8], sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      y[e] = fast_exp2(y[e] - m_new);
+      y[e] = fast_exp2(__builtin_fmaf(st[e >> 2][e & 3], p.scale_log2, -m_new));
       sum += y[e];
     }
-    l_run = l_run * alpha + sum;
-    m_run = m_new;
+    l_run += sum;
     u32x4 pb;
 #pragma unroll
     for (int w = 0; w < 4; ++w) pb[w] = Mfma<T>::pack2(y[2 * w], y[2 * w + 1]);
     const uint32_t s0 = *(const uint32_t*)(scales + kChunk8 + 4 * g), s1 = *(const uint32_t*)(scales + kChunk8 + 16 + 4 * g);
     u32x4 value[8];   // of key e: dims 8 c .. 8 c + 7
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float scale = scale_of(((e < 4 ? s0 : s1) >> (8 * (e & 3))) & 255u);
-      const u32x2 lo = values4<T>(x.v[e][0], scale), hi = values4<T>(x.v[e][1], scale);
-      value[e] = u32x4{lo[0], lo[1], hi[0], hi[1]};
-    }
+    for (int e = 0; e < 8; ++e) value[e] = values8<T>(x.v[e], ((e < 4 ? s0 : s1) >> (8 * (e & 3))) & 255u);
 #pragma unroll
     for (int b = 0; b < 8; ++b) {
       u32x4 col;
 #pragma unroll
       for (int w = 0; w < 4; ++w)
         col[w] = __builtin_amdgcn_perm(value[2 * w + 1][b >> 1], value[2 * w][b >> 1], (b & 1) ? 0x07060302u : 0x05040100u);
-      acc[b] = Mfma<T>::m16x16x32(col, pb, acc[b] * alpha);
+      acc[b] = Mfma<T>::m16x16x32(col, pb, acc[b]);
     }
     __builtin_amdgcn_wave_barrier();
   };
