@@ -885,7 +885,7 @@ static int kv_append_attn(ellm_kv_cache* c, size_t layer, ellm_attn* a, const vo
   args.position_interval = 1;
   args.batch = (uint32_t)batch_size;
   args.positions = positions;
-  if (a->shaped.active() || a->k_scale) {   // those kernels read finished rows: the two calls one after the other
+  if (a->shaped.active()) {   // the kernels for shaped scores read finished rows: the two calls one after the other
     const int st = ellm_kv_append_norm_rope(c, layer, position_index, 1, batch_size, k_src, v_src, batch_size, rope,
                                             rope_positions, eps, positions, max_position, stream);
     return st != ELLM_OK ? st : ellm::attn_run_single_token(a, &args, (uint32_t)first, (hipStream_t)stream);

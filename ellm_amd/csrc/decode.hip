@@ -70,7 +70,15 @@ __global__ __launch_bounds__(kDecThreads, PENDING || E4M3 ? 2 : 4) void decode_s
   u32x4 qreg[4];
   float m_run, l_run;
   f32x4 acc[8];
-  if constexpr (PENDING) {
+  if constexpr (E4M3) {
+    load_queries8(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
+    Stream8<T, PENDING != kPendNone> stream;
+    stream.open(p, plane, k_begin, k_end, pos, t, split * 7u + blockIdx.y * 3u + seq * 5u);
+    // the split that holds the plane's last key takes the new row; one workgroup of a group writes it
+    NewRow8 fresh;
+    if constexpr (PENDING) fresh = new_row8(p, plane, seq, kvh, pos, hgrp == 0);
+    stream.run(p, qreg, smem, t, m_run, l_run, acc, &fresh);
+  } else if constexpr (PENDING) {
     PendingQueries queries;   // requested first: the stream's own loads follow
     if constexpr (PENDING == kPendSums) queries.fetch(p.pend, seq, head0, pos, t, heads_here);
     // the split that holds the plane's last key takes the new row; one workgroup of a group writes it
@@ -86,10 +94,6 @@ __global__ __launch_bounds__(kDecThreads, PENDING || E4M3 ? 2 : 4) void decode_s
     if constexpr (PENDING == kPendSums) {
       if (fresh.present) store_queries(const_cast<uint16_t*>(p.q) + (size_t)row0 * kHeadDim, t, heads_here, qreg);
     }
-  } else if constexpr (E4M3) {
-    load_queries8(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
-    stream_keys8<T>(p, plane, k_begin, k_end, pos, qreg, smem, t, split * 7u + blockIdx.y * 3u + seq * 5u, m_run, l_run, acc);
-    order_columns8(acc);
   } else {
     load_queries(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
     stream_keys<T>(planes_of<SHAPE>(p, plane, kvh, range), k_begin, k_end, pos, qreg, smem, t,
@@ -99,13 +103,19 @@ __global__ __launch_bounds__(kDecThreads, PENDING || E4M3 ? 2 : 4) void decode_s
   auto final_row = [&](uint32_t h, uint32_t dq, const f32x4& a, float l, float m) {
     emit_joined<T, SHAPE>(p, row0 + h, dq, a, l, m);
   };
-  merge_waves<E4M3 ? 4 : 16, E4M3 ? 32 : 4>(
-      smem, t, heads_here, m_run, l_run, acc, [&](uint32_t h, uint32_t dq, const f32x4& a, float l, float m) {
-        if (p.n_split == 1)
-          final_row(h, dq, a, l, m);
-        else
-          store_partial(p.ws_acc, p.ws_ml, (size_t)((row0 + h) * p.n_split + split), dq, a, l, m);
-      });
+  auto emit = [&](uint32_t h, uint32_t dq, const f32x4& a, float l, float m) {
+    if (p.n_split == 1)
+      final_row(h, dq, a, l, m);
+    else
+      store_partial(p.ws_acc, p.ws_ml, (size_t)((row0 + h) * p.n_split + split), dq, a, l, m);
+  };
+  if constexpr (E4M3) {
+    put_waves8(smem, t, heads_here, m_run, l_run, acc);
+    __syncthreads();
+    join_waves(smem, t, heads_here, emit);
+  } else {
+    merge_waves(smem, t, heads_here, m_run, l_run, acc, emit);
+  }
   if (p.n_split == 1) return;
 
   // ---- the last workgroup to arrive merges: two levels, 16 partials each -----
@@ -188,11 +198,11 @@ hipError_t launch_decode(const AttnArgs& a, hipStream_t stream, const ShapedStat
 
   dim3 grid(a.n_split, a.n_kv_heads * p.head_groups, a.batch);
   dim3 block(kDecThreads);
-  if (a.k_scale) {
-    if (a.dtype == 0)
-      hipLaunchKernelGGL((decode_split_kernel<F16, kPendNone, kShapeNone, true>), grid, block, 0, stream, p);
-    else
-      hipLaunchKernelGGL((decode_split_kernel<BF16, kPendNone, kShapeNone, true>), grid, block, 0, stream, p);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, p); };
+  if (a.k_scale && a.pending.k_rows) {
+    a.dtype == 0 ? go(decode_split_kernel<F16, kPendRows, kShapeNone, true>) : go(decode_split_kernel<BF16, kPendRows, kShapeNone, true>);
+  } else if (a.k_scale) {
+    a.dtype == 0 ? go(decode_split_kernel<F16, kPendNone, kShapeNone, true>) : go(decode_split_kernel<BF16, kPendNone, kShapeNone, true>);
   } else if (shape) {
     const int kind = fill_shape(*shape, a, &p.shape);
     if (a.dtype == 0)

@@ -45,7 +45,7 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
   __shared__ uint32_t prefix[kMaxBatch + 1];   // units of the sequences before sequence b (per plane)
   __shared__ uint32_t s_pos[kMaxBatch];        // last position of every sequence
   __shared__ uint32_t s_last, s_umax, s_umin;
-  const Lane t;
+  Lane t;
   const uint32_t B = p.batch;
 
   // the last row of a sequence's keys, counted from its first (-1: no keys)
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
     if (total_units == 0) return;
   }
   // Units without keys in front of every plane's first (decode_shares.hpp).
-  const uint32_t charge = balanced_charge(umax_all, umin_all, total_units, B);
+  const uint32_t charge = balanced_charge(umax_all, umin_all, total_units, B, E4M3 ? kBalancedChargeE4m3 : kBalancedCharge);
   r_units += charge;
   r_incl += charge * (t.lane + 1);
   total_units += charge * B;
@@ -142,7 +142,9 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
   // its own start-up that a second workgroup on the unit hides (400 planes of 100-4096 keys).
   // (decode_shares.hpp: balanced_workgroups, also walked by the CPU tests)
   const uint32_t planes_all = PL * B;
-  const uint32_t W = balanced_workgroups(gridDim.x, p.wgs_one, U, umax_all + charge, umin_all + charge, planes_all);
+  const uint32_t one_each =
+      E4M3 ? balanced_one_each_e4m3(gridDim.x, p.wgs_one, U, umax_all == umin_all, planes_all) : p.wgs_one;
+  const uint32_t W = balanced_workgroups(gridDim.x, one_each, U, umax_all + charge, umin_all + charge, planes_all);
   // Workgroups are dealt to the eight XCDs by their id modulo 8.  Each XCD takes one contiguous
   // eighth of the shares, so that no two of them walk the same stretch of memory side by side
   // (with shares numbered like the workgroups and as many pieces per plane as XCDs, every XCD
@@ -162,6 +164,8 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
   uint32_t x = share_begin(w);
   const uint32_t x_end = share_begin(w + 1);
   while (x < x_end) {
+    // (what follows from a lane's number is formed where it is needed: kept around the loop it would spill)
+    if constexpr (E4M3) asm volatile("" : "+v"(t.tid), "+v"(t.lane), "+v"(t.g), "+v"(t.c));
     // the sequence that holds unit x: the last b with PL prefix[b] <= x
     // (every thread computes the same values; readfirstlane tells the compiler so)
     uint32_t seq, u_seq, seq_start, pos;
@@ -215,7 +219,15 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
     u32x4 qreg[4];
     float m_run, l_run;
     f32x4 acc[8];
-    if constexpr (PENDING) {
+    if constexpr (E4M3) {
+      load_queries8(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
+      Stream8<T, PENDING != kPendNone> stream;
+      stream.open(p, plane, k_begin, k_end, pos, t, w * 7u + pl * 3u + seq * 5u);
+      // the piece that holds the plane's last key takes the new row; one workgroup of a group writes it
+      NewRow8 fresh;
+      if constexpr (PENDING) fresh = new_row8(p, plane, seq, kvh, pos, hgrp == 0);
+      stream.run(p, qreg, smem, t, m_run, l_run, acc, &fresh);
+    } else if constexpr (PENDING) {
       PendingQueries queries;   // requested first: the stream's own loads follow
       if constexpr (PENDING == kPendSums) queries.fetch(p.pend, seq, head0, pos, t, heads_here);
       // the piece that holds the plane's last key takes the new row; one workgroup of a group writes it
@@ -230,10 +242,6 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
       if constexpr (PENDING == kPendSums) {
         if (fresh.present) store_queries(const_cast<uint16_t*>(p.q) + (size_t)row0 * kHeadDim, t, heads_here, qreg);
       }
-    } else if constexpr (E4M3) {
-      load_queries8(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
-      stream_keys8<T>(p, plane, k_begin, k_end, pos, qreg, smem, t, w * 7u + pl * 3u + seq * 5u, m_run, l_run, acc);
-      order_columns8(acc);
     } else {
       load_queries(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
       stream_keys<T>(planes_of<SHAPE>(p, plane, kvh, range), k_begin, k_end, pos, qreg, smem, t,
@@ -243,13 +251,19 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
     auto final_row = [&](uint32_t h, uint32_t dq, const f32x4& av, float l, float m) {
       emit_joined<T, SHAPE>(p, (size_t)(row0 + h), dq, av, l, m);
     };
-    merge_waves<E4M3 ? 4 : 16, E4M3 ? 32 : 4>(
-        smem, t, heads_here, m_run, l_run, acc, [&](uint32_t h, uint32_t dq, const f32x4& av, float l, float m) {
-          if (n_pieces == 1)
-            final_row(h, dq, av, l, m);
-          else
-            store_partial(p.ws_acc, p.ws_ml, (size_t)((slot0 + piece) * G + h), dq, av, l, m);
-        });
+    auto emit = [&](uint32_t h, uint32_t dq, const f32x4& av, float l, float m) {
+      if (n_pieces == 1)
+        final_row(h, dq, av, l, m);
+      else
+        store_partial(p.ws_acc, p.ws_ml, (size_t)((slot0 + piece) * G + h), dq, av, l, m);
+    };
+    if constexpr (E4M3) {
+      put_waves8(smem, t, heads_here, m_run, l_run, acc);
+      __syncthreads();
+      join_waves(smem, t, heads_here, emit);
+    } else {
+      merge_waves(smem, t, heads_here, m_run, l_run, acc, emit);
+    }
     if (n_pieces > 1) {
       const uint32_t n_clusters = (n_pieces + kMergeFan - 1) / kMergeFan;
       const uint32_t cluster = piece / kMergeFan;
@@ -285,7 +299,7 @@ bool decode_balanced_takes(const DecodeWorkspace& w, uint32_t batch, uint32_t n_
   const uint64_t head_groups = (group + kMaxHeadsPerGroup - 1) / kMaxHeadsPerGroup;
   const uint64_t planes = (uint64_t)batch * n_kv_heads * head_groups;
   const uint64_t units = planes * ((max_len + kUnitKeys - 1) / kUnitKeys);
-  if (units < 8ull * wgs || units + kBalancedCharge * planes + wgs >= (1ull << 31) || wgs >= (1u << 16)) return false;
+  if (units < 8ull * wgs || units + kBalancedChargeE4m3 * planes + wgs >= (1ull << 31) || wgs >= (1u << 16)) return false;
   const uint64_t G = group < (uint32_t)kMaxHeadsPerGroup ? group : (uint32_t)kMaxHeadsPerGroup;
   const uint64_t slots = balanced_slots(wgs, (uint32_t)planes), cslots = balanced_cluster_slots(wgs, (uint32_t)planes);
   return slots * G <= w.rows && cslots * G <= w.rows2 && cslots + planes <= w.counters;
@@ -339,11 +353,11 @@ hipError_t launch_decode_balanced(const AttnArgs& a, uint32_t wgs, hipStream_t s
   p.k_scale = a.k_scale;
   p.v_scale = a.v_scale;
   const dim3 grid(wgs), block(kDecThreads);
-  if (a.k_scale) {
-    if (a.dtype == 0)
-      hipLaunchKernelGGL((decode_balanced_kernel<F16, kPendNone, kShapeNone, true>), grid, block, 0, stream, p);
-    else
-      hipLaunchKernelGGL((decode_balanced_kernel<BF16, kPendNone, kShapeNone, true>), grid, block, 0, stream, p);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, p); };
+  if (a.k_scale && a.pending.k_rows) {
+    a.dtype == 0 ? go(decode_balanced_kernel<F16, kPendRows, kShapeNone, true>) : go(decode_balanced_kernel<BF16, kPendRows, kShapeNone, true>);
+  } else if (a.k_scale) {
+    a.dtype == 0 ? go(decode_balanced_kernel<F16, kPendNone, kShapeNone, true>) : go(decode_balanced_kernel<BF16, kPendNone, kShapeNone, true>);
   } else if (shape) {
     const int kind = fill_shape(*shape, a, &p.shape);
     if (a.dtype == 0)

@@ -581,11 +581,11 @@ __device__ __forceinline__ void stream_keys(const Planes& planes, uint32_t k_beg
 // buffers).  Afterwards a thread owns four consecutive columns of one head (an item; eight heads
 // make 256 items, one per thread, sixteen heads two per thread) and hands them to
 // emit(h, dq, a[4], sum, max): columns 4 dq .. 4 dq + 3 of head h of the group.  acc[b] of lane (head, g): columns
-// QUAD_B b + QUAD_G g .. + 3.
-template <int QUAD_B = 16, int QUAD_G = 4, typename Emit>
-__device__ __forceinline__ void merge_waves(uint16_t* smem, const Lane& t, uint32_t heads_here, float m_run,
-                                            float l_run, const f32x4 (&acc)[8], Emit emit) {
-  __syncthreads();
+// QUAD_B b + QUAD_G g .. + 3.  In two steps: put_waves, each wave a part of its own, and behind a barrier join_waves.
+constexpr int kRedBytes = kDecWaves * kMaxHeadsPerGroup * kRedPitch * 4;
+template <int QUAD_B = 16, int QUAD_G = 4>
+__device__ __forceinline__ void put_waves(uint16_t* smem, const Lane& t, uint32_t heads_here, float m_run, float l_run,
+                                          const f32x4 (&acc)[8]) {
   float* red = (float*)smem;
   if ((uint32_t)t.c < heads_here) {
     float* row = red + (t.wave * kMaxHeadsPerGroup + t.c) * kRedPitch;
@@ -593,7 +593,10 @@ __device__ __forceinline__ void merge_waves(uint16_t* smem, const Lane& t, uint3
     for (int b = 0; b < 8; ++b) *(f32x4*)(row + QUAD_B * b + QUAD_G * t.g) = acc[b];
     if (t.g == 0) *(f32x2*)(row + kHeadDim) = f32x2{m_run, l_run};
   }
-  __syncthreads();
+}
+template <typename Emit>
+__device__ __forceinline__ void join_waves(const uint16_t* smem, const Lane& t, uint32_t heads_here, Emit emit) {
+  const float* red = (const float*)smem;
   const uint32_t n_items = heads_here * kQuads;
 #pragma unroll
   for (int n = 0; n < kItems; ++n) {
@@ -621,6 +624,14 @@ __device__ __forceinline__ void merge_waves(uint16_t* smem, const Lane& t, uint3
     }
     emit(h, dq, a, lsum, mmax);
   }
+}
+template <typename Emit>
+__device__ __forceinline__ void merge_waves(uint16_t* smem, const Lane& t, uint32_t heads_here, float m_run,
+                                            float l_run, const f32x4 (&acc)[8], Emit emit) {
+  __syncthreads();
+  put_waves(smem, t, heads_here, m_run, l_run, acc);
+  __syncthreads();
+  join_waves(smem, t, heads_here, emit);
 }
 
 // Columns 4 dq .. of output row `row` (sequence x query heads + head), normalised; the row's

@@ -60,8 +60,13 @@ ELLM_SHARES_FN uint32_t balanced_min_share(uint32_t longest_plane_units) {
 // on average: a start is below half a per cent of one, and the launch as often longer as shorter (32 of 1024-131072, two draws,
 // 662 / 657 and 488.5 / 491.7; below, 48 of 1000-30000 210.6 / 207.6, 10 of 1000-60000 184.2 / 183.0).
 constexpr uint32_t kBalancedCharge = 2;
-ELLM_SHARES_FN uint32_t balanced_charge(uint32_t umax, uint32_t umin, uint32_t total, uint32_t sequences) {
-  return umax == umin || total > 512u * sequences ? 0 : kBalancedCharge;
+// Rows in 8 bits, whose units are half the bytes: three (us, two / three / four units a start; bfloat16, 32 / 4 heads: 300 of 64-2000
+// keys 68.7 / 67.9 / 67.2, 28 of 115-3918 19.3 / 19.1 / 18.4, 16 of 64-8000 17.5 / 16.9 / 16.8, 200 of 1-600 26.7 / 26.4 / 26.3;
+// but 100 of 100-4096 48.8 / 48.1 / 49.4, 32 of 300-16000, 64 / 8 heads, 82.3 / 82.8 / 83.9, 63 of 2048 and one of 1901 30.8 / 30.9 / 31.5).
+constexpr uint32_t kBalancedChargeE4m3 = 3;
+ELLM_SHARES_FN uint32_t balanced_charge(uint32_t umax, uint32_t umin, uint32_t total, uint32_t sequences,
+                                        uint32_t start = kBalancedCharge) {
+  return umax == umin || total > 512u * sequences ? 0 : start;
 }
 // Workgroups that take part out of `limit`: at most one per unit of work and few enough for
 // balanced_min_share; with planes of equal length a whole number per plane (so that shares end
@@ -88,6 +93,14 @@ ELLM_SHARES_FN uint32_t balanced_workgroups(uint32_t launched, uint32_t one_each
     if (100u * fewer >= 47u * W) W = fewer;
   }
   return W;
+}
+// What balanced_workgroups takes as `one_each` where rows are in 8 bits: a workgroup of those has more to compute for a byte, and two
+// on a unit fill each other's waits.  One on a unit only for planes of equal length, whose partial results count, and for few short
+// shares of few planes (us, one / two a unit: 32 of 300-16000, 64 / 8 heads, 112 / 103; 64 of 100-2000, 32 / 4, 24.0 / 22.3; 15 of 8192
+// and one of 8101 30.5 / 28.5; 24 of 1000-60000 131.2 / 129.8; but 64 of 2048 23.1 / 26.9, 16 of 64-8000 17.7 / 19.0).
+ELLM_SHARES_FN uint32_t balanced_one_each_e4m3(uint32_t launched, uint32_t one_each, uint32_t U, bool equal_planes,
+                                               uint32_t planes) {
+  return equal_planes || (2u * planes <= one_each && U < 12u * launched) ? one_each : launched;
 }
 // The share workgroup `id` takes: each XCD (id % 8) one contiguous eighth when W allows.
 ELLM_SHARES_FN uint32_t balanced_share_of(uint32_t id, uint32_t W) {

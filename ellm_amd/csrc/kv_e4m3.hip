@@ -28,37 +28,6 @@ struct WriteArgs {
   float eps;
 };
 
-template <typename T>
-__device__ __forceinline__ void unpack8(u32x4 raw, float (&x)[8]) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    x[2 * e] = Mfma<T>::to_float((uint16_t)(raw[e] & 0xffffu));
-    x[2 * e + 1] = Mfma<T>::to_float((uint16_t)(raw[e] >> 16));
-  }
-}
-
-// The key row that lane c of sixteen holds eight elements of, normalised and rotated: the formulas of norm_rope_row16
-// (common.hpp) in binary32, one rounding an operation, but the squares added as a tree (a lane's eight in order, then
-// across lanes 1, 2, 4, 8 apart) and the results not rounded: the codes are taken of them as they are.
-template <typename T>
-__device__ __forceinline__ void norm_rope8(float (&x)[8], u32x4 turn, float eps) {
-#pragma clang fp contract(off)
-  float sum = 0.0f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) sum = sum + x[e] * x[e];
-#pragma unroll
-  for (int m = 1; m < 16; m <<= 1) sum = sum + __shfl_xor(sum, m, 16);
-  const float rrms = 1.0f / (sqrtf(sum / (float)kHeadDim) + eps);
-  float w[8];
-  unpack8<T>(turn, w);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float a = x[2 * e] * rrms, b = x[2 * e + 1] * rrms;
-    x[2 * e] = a * w[2 * e] - b * w[2 * e + 1];
-    x[2 * e + 1] = a * w[2 * e + 1] + b * w[2 * e];
-  }
-}
-
 template <typename T, bool NORM>
 __global__ __launch_bounds__(kThreads) void kv_append_e4m3_kernel(WriteArgs p) {
   const uint32_t c = threadIdx.x & 15;
