@@ -2,6 +2,7 @@
 // validation, the operator handle, the K/V cache object, error reporting.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -804,9 +805,18 @@ int ellm_kv_read_e4m3(const ellm_kv_cache* c, size_t layer, size_t first_sequenc
     return fail(ELLM_ERR_INVALID_ARGUMENT, "destinations must be 16-byte aligned");
   const size_t extent[3] = {n_tokens, batch_size, c->desc.kv_head_num};
   for (int i = 0; i < 3; ++i)
-    if (dst_strides[i] % 8 != 0 || (extent[i] > 1 && dst_strides[i] < 128))
+    if (extent[i] > 1 && (dst_strides[i] % 8 != 0 || dst_strides[i] < 128))
       return fail(ELLM_ERR_INVALID_ARGUMENT, "dst_strides[%d] = %zu must be a multiple of 8 elements, and 128 at least", i,
                   dst_strides[i]);
+  // no row onto another: from the narrowest axis up, each must step over what the ones below it span
+  int axis[3] = {0, 1, 2};
+  std::sort(axis, axis + 3, [&](int a, int b) { return dst_strides[a] < dst_strides[b]; });
+  size_t span = 128;
+  for (int i : axis) {
+    if (extent[i] <= 1) continue;
+    if (dst_strides[i] < span) return fail(ELLM_ERR_INVALID_ARGUMENT, "dst_strides[%d] = %zu puts rows onto one another", i, dst_strides[i]);
+    span += (extent[i] - 1) * dst_strides[i];
+  }
   if (layer >= c->desc.layers) return fail(ELLM_ERR_OUT_OF_RANGE, "layer %zu of %zu", layer, c->desc.layers);
   if (first_sequence >= c->desc.sequences || batch_size > c->desc.sequences - first_sequence)
     return fail(ELLM_ERR_OUT_OF_RANGE, "sequences [%zu, %zu) of %zu", first_sequence, first_sequence + batch_size,

@@ -64,6 +64,28 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
   return top >= 0x7f800000u ? kScaleNan : b > 9 ? b - 8 : 1;
 }
 
+// x of the lane 1, 2, 4 or 8 apart, in a row of sixteen lanes of which the lanes that STEP's earlier ones joined hold the same x:
+// there lane 7 - i stands for i ^ 4, and 15 - i for i ^ 8.  No trip through LDS, as an exchange of any two lanes is.
+template <int STEP>
+__device__ __forceinline__ uint32_t from_partner16(uint32_t x) {
+  constexpr int kCtrl = STEP == 1 ? 0xb1 : STEP == 2 ? 0x4e : STEP == 4 ? 0x141 : 0x140;   // quad_perm 1 0 3 2, 2 3 0 1; mirrors
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kCtrl, 0xf, 0xf, true);
+}
+__device__ __forceinline__ float sum16(float x) {
+  auto with = [&](uint32_t y) { x = x + __builtin_bit_cast(float, y); };
+  with(from_partner16<1>(__builtin_bit_cast(uint32_t, x)));
+  with(from_partner16<2>(__builtin_bit_cast(uint32_t, x)));
+  with(from_partner16<4>(__builtin_bit_cast(uint32_t, x)));
+  with(from_partner16<8>(__builtin_bit_cast(uint32_t, x)));
+  return x;
+}
+__device__ __forceinline__ uint32_t max16(uint32_t x) {
+  x = max(x, from_partner16<1>(x));
+  x = max(x, from_partner16<2>(x));
+  x = max(x, from_partner16<4>(x));
+  return max(x, from_partner16<8>(x));
+}
+
 template <typename T>
 __device__ __forceinline__ void unpack8(u32x4 raw, float (&x)[8]) {
 #pragma unroll
@@ -82,8 +104,7 @@ __device__ __forceinline__ void norm_rope8(float (&x)[8], u32x4 turn, float eps)
   float sum = 0.0f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum = sum + x[e] * x[e];
-#pragma unroll
-  for (int m = 1; m < 16; m <<= 1) sum = sum + __shfl_xor(sum, m, 16);
+  sum = sum16(sum);
   const float rrms = 1.0f / (sqrtf(sum / (float)kHeadDim) + eps);
   float w[8];
   unpack8<T>(turn, w);
@@ -101,9 +122,7 @@ __device__ __forceinline__ u32x2 row_codes16(const float (&x)[8], uint32_t& byte
   uint32_t top = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) top = max(top, __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffffu);
-#pragma unroll
-  for (int m = 1; m < 16; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, 16));
-  byte = scale_byte(top);
+  byte = scale_byte(max16(top));
   const float scale = scale_of(byte);
   u32x2 codes;
 #pragma unroll

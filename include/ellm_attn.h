@@ -350,8 +350,9 @@ int ellm_attn_create_ragged(const ellm_attn_desc* desc, const ellm_kv_seq_table*
  * and a row that holds an infinity or a NaN reads as NaN as a whole (scale 255, codes 0).  What is read back is a value of
  * the 16-bit type as it stands, and attention over the cache is attention over those values.
  * desc->dtype: the type of the rows that are written and read back.  The other calls for caches take such a cache too:
- * ellm_kv_append, ellm_kv_append_norm_rope (key rows are normalised and rotated in binary32 and rounded once, to e4m3),
- * ellm_kv_append_attn_run*, ellm_kv_destroy; ellm_kv_layer and ellm_kv_layer_ragged refuse it.  No counterpart in the
+ * ellm_kv_append, ellm_kv_append_norm_rope (key rows are normalised and rotated in binary32 and rounded once, to e4m3; of
+ * several tokens that a sequence's capacity clamps to its last row the last one is kept), ellm_kv_append_attn_run*,
+ * ellm_kv_destroy; ellm_kv_layer and ellm_kv_layer_ragged refuse it.  No counterpart in the
  * reference, whose caches hold the element type of the graph (src/memory/cache.rs:23).
  */
 int ellm_kv_create_e4m3(const ellm_kv_desc* desc, ellm_kv_cache** out_cache);
@@ -367,8 +368,8 @@ int ellm_kv_layer_e4m3(const ellm_kv_cache* cache, size_t layer, size_t first_se
  * [first_sequence, first_sequence + batch_size).  The row of token t, sequence s, head h (counted from 0) goes to
  * k_dst + t * dst_strides[0] + s * dst_strides[1] + h * dst_strides[2] (elements, multiples of 8, at least 128 along axes
  * longer than one), v_dst likewise: {batch_size * kv_head_num * 128, kv_head_num * 128, 128} is the order ellm_kv_append
- * takes rows in, {128, kv_strides[0], kv_strides[1]} that of a 16-bit cache.  Destinations are 16-byte aligned and outside
- * the cache. */
+ * takes rows in, {128, kv_strides[0], kv_strides[1]} that of a 16-bit cache; every axis longer than one steps over all that
+ * the axes of smaller strides span.  Destinations are 16-byte aligned and outside the cache. */
 int ellm_kv_read_e4m3(const ellm_kv_cache* cache, size_t layer, size_t first_sequence, size_t position_index,
                       size_t n_tokens, size_t batch_size, void* k_dst, void* v_dst, const size_t dst_strides[3],
                       void* stream);

@@ -1,0 +1,245 @@
+"""Steps over caches in 8 bits where one launch writes the new rows and attends over them: the cache bit for bit as the write
+alone leaves it, and the attention of the cache as it then stands."""
+import math
+
+import pytest
+import torch
+
+import ellm_amd
+from e4m3_util import CODE, D, LARGEST, hold, rope_table, rows, values
+from shaped_util import check, reference
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+SCALE = 1.0 / math.sqrt(D)
+
+
+class Layer:
+    """A cache whose rows are random codes (no NaN among them) and scales 2^-9 .. 2^-6, and a handle over it."""
+
+    def __init__(self, seed, dtype, hq, hkv, capacities, uniform=False, scale=SCALE, layers=1, interval=1):
+        self.dtype, self.hq, self.hkv, self.caps, self.uniform, self.layers = dtype, hq, hkv, capacities, uniform, layers
+        batch = len(capacities)
+        if uniform:
+            self.cache = ellm_amd.KVCache(layers, batch, hkv, capacities[0], CODE[dtype], e4m3=True)
+        else:
+            self.cache = ellm_amd.KVCache.ragged(layers, capacities, hkv, CODE[dtype], e4m3=True)
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        for codes, byte in self.tensors():
+            codes.copy_(torch.randint(0, 256, codes.shape, generator=gen, device="cuda").to(torch.uint8))
+            codes[(codes & 127) == 127] = 0
+            byte.copy_(torch.randint(118, 122, byte.shape, generator=gen, device="cuda").to(torch.uint8))
+        view = self.cache.layer_e4m3(layers - 1)
+        k, v, ks, vs = self.cache.layer_e4m3_tensors(layers - 1)
+        self.q = torch.randn((interval, batch, hq, D), generator=gen, device="cuda").to(dtype)
+        self.out, self.lse = torch.full_like(self.q, 7.0), torch.full(self.q.shape[:3], 7.0, device="cuda")
+        self.op = ellm_amd.Attention(self.q, k, v, self.out, batch, hq, hkv, D, view.strides, scale, lse=self.lse,
+                                     sequence_capacity=max(capacities), max_position_interval=interval,
+                                     seq_table=None if uniform else view, kv_scales=(ks, vs))
+        self.scale = scale
+
+    def tensors(self):
+        k, v, ks, vs = (t.view(torch.uint8) for t in self.cache.layer_e4m3_tensors(self.layers - 1))
+        return (k, ks), (v, vs)
+
+    def plane(self, s):
+        """K and V of sequence s as the cache holds them, [1, heads, capacity, 128] in 32 bits (exact)."""
+        at = sum(self.caps[:s])
+        part = (lambda t: t[s]) if self.uniform else (lambda t: t[:, at:at + self.caps[s]])
+        return [values(part(c), part(b)).float()[None] for c, b in self.tensors()]
+
+    def check(self, positions, what=""):
+        torch.cuda.synchronize()
+        for s, p in enumerate(positions):
+            k, v = self.plane(s)
+            n = p + self.q.shape[0]
+            want = reference(self.q[:, s:s + 1], k[:, :, :n], v[:, :, :n], [p], self.scale)
+            check(self.out[:, s:s + 1], self.lse[:, s:s + 1], want, f"{what} sequence {s}")
+
+
+def _new(seed, batch, hkv, dtype, tokens=1):
+    gen = torch.Generator().manual_seed(seed)
+    return [rows(gen, (tokens, batch, hkv), dtype, 0.5).cuda() for _ in range(2)]
+
+
+def _same_bits(a, b):
+    torch.cuda.synchronize()
+    return all(torch.equal(x, y) for m, n in zip(a.tensors(), b.tensors()) for x, y in zip(m, n))
+
+
+CASES = [
+    (4, 1, [1], [0]),                                    # the first token
+    (8, 8, [3, 1, 40], [0, 0, 0]),
+    (5, 1, [33, 34, 32, 65], [32, 33, 31, 64]),          # the new key begins a chunk, or ends one
+    (40, 2, [400, 129, 1, 300], [399, 128, 0, 7]),       # twenty heads a group
+    (16, 1, [6000], [5777]),                             # many workgroups to a plane
+    (17, 1, [6000, 40], [5999, 39]),
+    (64, 8, [3000, 100, 7], [2999, 5, 6]),
+    (8, 4, [9000 - 200 * i for i in range(16)], [8990 - 500 * i for i in range(16)]),   # shares of different planes
+    (32, 4, [9000] * 16, [8999] * 16),
+    (40, 2, [9000] * 9, [8700, 31, 0, 8999, 8000, 1, 8992, 8991, 100]),
+]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hq,hkv,capacities,positions", CASES)
+def test_a_step_with_positions_of_their_own(dtype, hq, hkv, capacities, positions):
+    batch, most = len(capacities), max(positions)
+    step, apart = (Layer(50, dtype, hq, hkv, capacities, layers=2) for _ in range(2))
+    k, v = _new(51, batch, hkv, dtype)
+    rope = rope_table(most + 1, dtype).cuda()
+    at = torch.tensor(positions, dtype=torch.int32, device="cuda")
+    step.cache.append_norm_rope_with_attention(1, step.op, 0, k, v, rope, positions=at, max_position=most)
+    apart.cache.append_norm_rope(1, 0, k, v, rope, positions=at, max_position=most)
+    assert _same_bits(step, apart)
+    step.check(positions)
+
+
+def test_the_cases_reach_both_kernels():
+    paths = {Layer(50, F16, hq, hkv, capacities).op.ragged_path(max(positions), len(capacities))
+             for hq, hkv, capacities, positions in CASES}
+    assert paths == {0, 1}
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hq,hkv,batch,position", [(4, 1, 1, 0), (8, 2, 3, 31), (8, 2, 3, 32), (34, 2, 2, 1000), (16, 1, 1, 5999),
+                                                   (64, 8, 16, 3000)])
+def test_a_step_at_one_position(dtype, hq, hkv, batch, position):
+    step, apart = (Layer(52, dtype, hq, hkv, [position + 2] * batch, uniform=True) for _ in range(2))
+    k, v = _new(53, batch, hkv, dtype)
+    rope = rope_table(position + 1, dtype).cuda()
+    step.cache.append_norm_rope_with_attention(0, step.op, position, k, v, rope)
+    apart.cache.append_norm_rope(0, position, k, v, rope)
+    assert _same_bits(step, apart)
+    step.check([position] * batch)
+
+
+@pytest.mark.parametrize("batch,position", [(3, 100), (16, 8999)])
+def test_new_rows_that_are_not_finite(batch, position):
+    """They read as NaN from then on, in their own sequence and group of heads only."""
+    hq, hkv = 8, 4
+    step, apart = (Layer(54, BF16, hq, hkv, [9000] * batch, uniform=True) for _ in range(2))
+    k, v = _new(55, batch, hkv, BF16)
+    k[0, 0, 1, 5], v[0, 2, 3, 100] = float("inf"), float("nan")
+    rope = rope_table(position + 1, BF16).cuda()
+    step.cache.append_norm_rope_with_attention(0, step.op, position, k, v, rope)
+    apart.cache.append_norm_rope(0, position, k, v, rope)
+    assert _same_bits(step, apart)
+    bad = torch.zeros(1, batch, hq, dtype=torch.bool, device="cuda")
+    bad[0, 0, 2:4] = bad[0, 2, 6:8] = True
+    assert torch.equal(torch.isnan(step.out).all(dim=-1), bad) and torch.equal(torch.isnan(step.out).any(dim=-1), bad)
+
+
+def test_rows_behind_the_last_sequence_stay():
+    step = Layer(56, F16, 8, 2, [50] * 4, uniform=True)
+    before = [t.clone() for pair in step.tensors() for t in pair]
+    k, v = _new(57, 2, 2, F16)
+    step.cache.append_norm_rope_with_attention(0, step.op, 20, k, v, rope_table(21, F16).cuda(), batch_size=2)
+    torch.cuda.synchronize()
+    assert (step.out[:, 2:] == 7.0).all() and (step.lse[:, 2:] == 7.0).all()
+    for was, now in zip(before, (t for pair in step.tensors() for t in pair)):
+        assert torch.equal(was[2:], now[2:]) and torch.equal(was[:, :, :20], now[:, :, :20])
+        assert torch.equal(was[:, :, 21:], now[:, :, 21:])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("scale", [0.0, -0.07, 1e-40])
+@pytest.mark.parametrize("interval,batch,keys", [(1, 2, 100), (1, 16, 9000), (20, 2, 60), (40, 1, 300)])
+def test_scales_of_zero_and_below(dtype, scale, interval, batch, keys):
+    t = Layer(58, dtype, 8, 4, [keys] * batch, uniform=True, scale=scale, interval=interval)
+    first = keys - interval - (1 if interval == 1 else 0)   # (a last chunk that is not whole)
+    if interval == 1:
+        t.op.run_ragged(torch.full((batch,), first, dtype=torch.int32, device="cuda"), first, batch)
+    else:
+        t.op.run(first, interval, batch)
+    t.check([first] * batch)
+
+
+def test_two_recorded_steps_of_one_handle():
+    """Recorded twice with different rows to write, replayed in turn with eager runs between: each as the eager call."""
+    dtype, caps = BF16, [9000] * 16
+    step, eager = (Layer(60, dtype, 8, 4, caps) for _ in range(2))
+    rope = rope_table(9000, dtype).cuda()
+    at = torch.tensor([8000 - 450 * i for i in range(16)], dtype=torch.int32, device="cuda")
+    moving = [at.clone(), at.clone() + 1]
+    new = [_new(61 + i, 16, 4, dtype) for i in range(2)]
+    stream, graphs = torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+    for i in range(2):
+        with torch.cuda.stream(stream), ellm_amd.StepGraph(stream) as graph:
+            step.cache.append_norm_rope_with_attention(0, step.op, 0, *new[i], rope, positions=moving[i], max_position=8999, stream=stream)
+            ellm_amd.positions_advance(moving[i], 2, stream=stream)
+        graphs.append(graph)
+    stream.synchronize()
+    for turn in range(6):
+        graphs[turn % 2].launch(stream)
+        stream.synchronize()
+        eager.cache.append_norm_rope_with_attention(0, eager.op, 0, *new[turn % 2], rope, positions=at + turn, max_position=8999)
+        torch.cuda.synchronize()
+        assert torch.equal(step.out, eager.out) and torch.equal(step.lse, eager.lse)
+        assert _same_bits(step, eager)
+        step.op.run_ragged(at, 8999, 16)   # eager work of the same handle and workspace in between
+        torch.cuda.synchronize()
+    for graph in graphs:
+        graph.close()
+
+
+def test_on_a_stream_of_the_callers():
+    """Rows that arrive late on a side stream: the write and the run wait for them there."""
+    step, apart = (Layer(64, F16, 8, 2, [700] * 3, uniform=True) for _ in range(2))
+    k, v = _new(65, 3, 2, F16)
+    rope = rope_table(700, F16).cuda()
+    late_k, late_v = torch.zeros_like(k), torch.zeros_like(v)
+    stream = torch.cuda.Stream()
+    work = torch.randn(2048, 2048, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for _ in range(20):
+            work = torch.mm(work, work).clamp(-1, 1)
+        late_k.copy_(k), late_v.copy_(v)
+        step.cache.append_norm_rope_with_attention(0, step.op, 600, late_k, late_v, rope)   # (the current stream)
+    stream.synchronize()
+    apart.cache.append_norm_rope(0, 600, k, v, rope)
+    assert _same_bits(step, apart)
+    step.check([600] * 3)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_several_tokens_that_are_clamped_to_one_row_leave_the_last(dtype):
+    t = Layer(66, dtype, 2, 2, [4, 30, 9])
+    before = [[x.clone() for x in pair] for pair in t.tensors()]
+    k, v = _new(67, 3, 2, dtype, tokens=5)
+    rope = rope_table(30, dtype)
+    at = torch.tensor([2, 20, 25], dtype=torch.int32)
+    t.cache.append_norm_rope(0, 0, k, v, rope.cuda(), positions=at.cuda(), max_position=25)
+    torch.cuda.synchronize()
+    written = {0: [(2, 0), (3, 4)], 1: [(20 + i, i) for i in range(5)], 2: [(8, 4)]}   # sequence -> (row, token)
+    start = [0, 4, 34]
+    codes, byte = t.tensors()[1]
+    want_codes, want_byte = before[1]
+    c, b = hold(v.cpu(), LARGEST[dtype])
+    for s, pairs in written.items():
+        for row, token in pairs:
+            want_codes[:, start[s] + row], want_byte[:, start[s] + row] = c[token, s].cuda(), b[token, s].cuda()
+    assert torch.equal(codes, want_codes) and torch.equal(byte, want_byte)
+    codes, byte = t.tensors()[0]   # the keys: only those rows changed, and none is a mixture
+    alone = Layer(66, dtype, 2, 2, [4, 30, 9])
+    for token in range(5):         # one token a call, in order
+        alone.cache.append_norm_rope(0, 0, k[token:token + 1], v[token:token + 1], rope.cuda(), positions=(at + token).cuda(),
+                                     max_position=29)
+    assert _same_bits(t, alone)
+
+
+def test_rows_read_onto_one_another_are_refused():
+    cache = ellm_amd.KVCache(1, 3, 2, 8, CODE[F16], e4m3=True)
+    flat = torch.zeros(40 * D, dtype=F16, device="cuda")
+
+    def views(strides, shape=(4, 3, 2)):
+        return [flat.as_strided((*shape, D), (*strides, 1)) for _ in range(2)]
+
+    for strides in ((D, D, D), (6 * D, 2 * D, D // 2), (3 * D, 2 * D, D), (D, 4 * D, 4 * D)):
+        with pytest.raises(ellm_amd.EllmError):
+            cache.read(0, 0, *views(strides))
+    cache.read(0, 0, *views((D, 8 * D, 4 * D)))
+    cache.read(0, 0, *views((5, 3, D), (1, 1, 2)))   # (strides of axes of length one mean nothing)
+    torch.cuda.synchronize()
