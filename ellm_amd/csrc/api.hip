@@ -435,7 +435,8 @@ int ellm::attn_run_single_token(ellm_attn* h, ellm::AttnArgs* a, uint32_t max_po
     if (e != hipSuccess) return fail_hip(e, "single-token attention launch");
     return ELLM_OK;
   }
-  const ellm::DecodePlan plan = ellm::decode_plan(longest, a->batch, a->n_kv_heads, (uint32_t)h->n_cu);
+  const ellm::DecodePlan plan = ellm::decode_plan(longest, a->batch, a->n_kv_heads, (uint32_t)h->n_cu,
+                                                  a->k_scale ? ellm::kDecodeStepKeysE4m3 : ellm::kDecodeStepKeys);
   a->split_len = plan.split_len;
   a->n_split = plan.n_split;
   if (!ellm::decode_plan_fits(h->ws, a->batch, a->n_q_heads, a->n_kv_heads, a->group, a->n_split))

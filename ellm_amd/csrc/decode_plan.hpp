@@ -10,6 +10,7 @@ namespace ellm {
 
 // Keys handled by one workgroup step of the single-token kernel.
 constexpr uint32_t kDecodeStepKeys = 64;
+constexpr uint32_t kDecodeStepKeysE4m3 = 128;   // ... of rows in 8 bits: the same bytes
 // Partials folded per merge step and query heads of a GQA group that one workgroup serves
 // (decode_common.hpp asserts that its own constants equal these).
 constexpr uint32_t kPlanMergeFan = 16;
@@ -28,7 +29,8 @@ struct DecodeWorkspace {
   size_t counters;  // uint32 arrival counters
 };
 
-inline DecodePlan decode_plan(uint32_t max_len, uint32_t batch, uint32_t n_kv_heads, uint32_t n_cu) {
+inline DecodePlan decode_plan(uint32_t max_len, uint32_t batch, uint32_t n_kv_heads, uint32_t n_cu,
+                              uint32_t step = kDecodeStepKeys) {
   // Every plane is cut into the same number of splits.  Each workgroup has fixed costs (query
   // load, wave merge, partial write, arrival) that more, shorter workgroups pay more often, and
   // one workgroup alone on a compute unit streams a little faster than each of two that share
@@ -43,8 +45,7 @@ inline DecodePlan decode_plan(uint32_t max_len, uint32_t batch, uint32_t n_kv_he
   const uint64_t planes = (uint64_t)batch * n_kv_heads;
   // both merge levels fold at most 16 partials: at most 16 * 16 splits per plane
   const uint32_t floor_len =
-      ((max_len + kPlanMergeFan * kPlanMergeFan - 1) / (kPlanMergeFan * kPlanMergeFan) + kDecodeStepKeys - 1) /
-      kDecodeStepKeys * kDecodeStepKeys;
+      ((max_len + kPlanMergeFan * kPlanMergeFan - 1) / (kPlanMergeFan * kPlanMergeFan) + step - 1) / step * step;
   // Never shorter than four 64-key steps, except where even such splits leave at least half of
   // the units without a workgroup (one sequence of a few hundred keys, a handful of a thousand):
   // there a wave's chunks, fetched one after the other, are a chain of trips to memory, and one
@@ -52,14 +53,18 @@ inline DecodePlan decode_plan(uint32_t max_len, uint32_t batch, uint32_t n_kv_he
   // (1 x 512 keys: 9.4 -> 6.7 us, 4 x 1024: 10.0 -> 8.5, 1 x 2048: 8.4; folds of at most 8 or 4
   // partials, i.e. longer splits, measured the same or slower).
   const bool tiny = planes * ((max_len + 4 * kDecodeStepKeys - 1) / (4 * kDecodeStepKeys)) * 2 <= n_cu;
-  const uint32_t one_fold_len = ((max_len + kPlanMergeFan - 1) / kPlanMergeFan + kDecodeStepKeys - 1) /
-                                kDecodeStepKeys * kDecodeStepKeys;
-  const uint32_t min_len = tiny ? one_fold_len : 4 * kDecodeStepKeys;
+  const uint32_t one_fold_len = ((max_len + kPlanMergeFan - 1) / kPlanMergeFan + step - 1) / step * step;
+  // Rows in 8 bits: planes of up to four steps are not cut at all, four trips of a wave's chunks being a shorter chain than a
+  // second split and the fold (us, one split / cut as above, 4 heads: 1 x 200 keys 4.7 / 6.5, 1 x 400 6.2 / 6.6, 1 x 512 6.2 / 6.65,
+  // 30 x 500 7.9 / 9.4; eight steps: 4 x 1024 9.9 / 7.6); beyond, steps of 128 keys leave no wave idle (1 x 900 6.8, with steps
+  // of 64 7.0; 4 x 1024 7.6 / 8.3).
+  const bool whole = step == kDecodeStepKeysE4m3 && max_len <= 4 * step;
+  const uint32_t min_len = whole ? 4 * step : tiny ? one_fold_len : 4 * kDecodeStepKeys;
   auto plan_for = [&](uint32_t per_cu, uint64_t* cost) {
     const uint32_t target = n_cu * per_cu;
     const uint32_t want = target / planes > 0 ? (uint32_t)(target / planes) : 1;
     uint32_t split_len = (max_len + want - 1) / want;
-    split_len = (split_len + kDecodeStepKeys - 1) / kDecodeStepKeys * kDecodeStepKeys;
+    split_len = (split_len + step - 1) / step * step;
     if (split_len < min_len) split_len = min_len;
     if (split_len < floor_len) split_len = floor_len;
     DecodePlan plan;
