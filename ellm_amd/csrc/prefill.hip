@@ -160,6 +160,20 @@ __device__ __forceinline__ void load_scales(const PrefillKernelArgs& p, uint64_t
   v = __builtin_amdgcn_raw_buffer_load_b8(__builtin_amdgcn_make_buffer_rsrc((void*)vs, 0, rows, kBufferFlags), at / kHeadDim, 0, 0);
 }
 
+// x of lane i of the lane's four
+template <int I>
+__device__ __forceinline__ uint32_t of_four(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x55 * I, 0xf, 0xf, true);   // quad_perm i i i i
+}
+// f(0), f(1), .. f(N - 1), of constants
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void each(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    each<N, I + 1>(f);
+  }
+}
+
 // 16 bytes a lane from memory straight to LDS address lds_at + 16 x lane.  Written as asm: the compiler's
 // own form of this load makes it wait for every outstanding one before each later LDS read (it cannot see
 // that the two touch different buffers).  M0 carries the address; one wait state between its write and the
@@ -1279,8 +1293,8 @@ __global__ __launch_bounds__(WR* WK* kWave, 2) void short_prompt_kernel(PrefillK
   const uint64_t valid_bytes = uniform_u64(((uint64_t)kmax * stride_pos + kHeadDim) * kElem);
   const int ld_c = lane & 15, ld_r = 4 * rw + (lane >> 4);   // rows ld_r + 4 WR i of a tile
   const uint32_t piece_off0 = (ld_r * stride_pos + 8 * ld_c) * kElem, piece_step = 4 * WR * stride_pos * kElem;
-  // (E4M3: sixteen codes a load, rows ld_r8 + 8 WR i of a tile; lane l of a wave fetches the scales of the tile's row l % 32, which
-  // lane exchanges hand to those that need them)
+  // (E4M3: sixteen codes a load, rows ld_r8 + 8 WR i of a tile; the lanes of four fetch the scales of one of those rows each, and
+  // have them from one another by DPP: through LDS, 33 x 5 tokens on 777 took 12.5 us for 12.0)
   constexpr int kLoads = E4M3 ? kPieces / 2 : kPieces;
   const int ld_r8 = 8 * rw + (lane >> 3), ld_x8 = lane & 7;
   u32x4 kst[kLoads], vst[kLoads];
@@ -1291,7 +1305,7 @@ __global__ __launch_bounds__(WR* WK* kWave, 2) void short_prompt_kernel(PrefillK
     const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kplane_u + off), 0, left, kBufferFlags);
     const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vplane_u + off), 0, left, kBufferFlags);
     const uint32_t at = E4M3 ? ld_r8 * stride_pos + 16 * ld_x8 : piece_off0, step = E4M3 ? 8 * WR * stride_pos : piece_step;
-    if constexpr (E4M3) load_scales(p, plane_at + off, left, (lane & 31) * stride_pos, k_scale, v_scale);
+    if constexpr (E4M3) load_scales(p, plane_at + off, left, (ld_r8 + 8 * WR * (lane % kLoads)) * stride_pos, k_scale, v_scale);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) kst[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, at + i * step, 0, 0);
 #pragma unroll
@@ -1313,13 +1327,11 @@ __global__ __launch_bounds__(WR* WK* kWave, 2) void short_prompt_kernel(PrefillK
   const uint32_t vs_store = lds0 + 2 * (kShKsHalves + (E4M3 ? ld_r8 * kVsPitch + 16 * ld_x8 : ld_r * kVsPitch + 8 * ld_c));
   auto store_chunk = [&](uint32_t buf) __attribute__((always_inline)) {
     if constexpr (E4M3) {
-      const int ks = (int)key_scale(k_scale, v_scale), vs = (int)value_scale(v_scale);
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int row = ld_r8 + 8 * WR * i;
-        store_codes16<T>(ks_store + 2 * (buf * kShTileHalves + 8 * WR * i * kKsPitch), kst[i], (uint32_t)__shfl(ks, row));
-        store_codes16<T>(vs_store + 2 * (buf * kShTileHalves + 8 * WR * i * kVsPitch), vst[i], (uint32_t)__shfl(vs, row));
-      }
+      const uint32_t ks = key_scale(k_scale, v_scale), vs = value_scale(v_scale);
+      each<kLoads>([&](auto i) __attribute__((always_inline)) {
+        store_codes16<T>(ks_store + 2 * (buf * kShTileHalves + 8 * WR * i * kKsPitch), kst[i], of_four<i>(ks));
+        store_codes16<T>(vs_store + 2 * (buf * kShTileHalves + 8 * WR * i * kVsPitch), vst[i], of_four<i>(vs));
+      });
     } else {
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
