@@ -243,3 +243,40 @@ def test_rows_read_onto_one_another_are_refused():
     cache.read(0, 0, *views((D, 8 * D, 4 * D)))
     cache.read(0, 0, *views((5, 3, D), (1, 1, 2)))   # (strides of axes of length one mean nothing)
     torch.cuda.synchronize()
+
+
+def test_positions_past_a_sequences_capacity_write_its_last_row():
+    caps, at = [3, 40, 9], [30, 39, 9]
+    step, apart = (Layer(68, BF16, 8, 2, caps) for _ in range(2))
+    k, v = _new(69, 3, 2, BF16)
+    rope = rope_table(40, BF16).cuda()
+    where = torch.tensor(at, dtype=torch.int32, device="cuda")
+    step.cache.append_norm_rope_with_attention(0, step.op, 0, k, v, rope, positions=where, max_position=39)
+    apart.cache.append_norm_rope(0, 0, k, v, rope, positions=where, max_position=39)
+    assert _same_bits(step, apart)
+    step.check([min(p, c - 1) for p, c in zip(at, caps)])
+
+
+@pytest.mark.parametrize("interval,first", [(1, 299), (1, 256), (40, 250), (3, 290)])
+def test_rows_as_far_apart_as_the_handle_takes(interval, first):
+    """Rows 2^24 codes apart: offsets of codes pass 2^32 inside a plane, and in the middle of a tile."""
+    hkv, hq, n, pitch = 2, 8, 300, 1 << 24
+    gen = torch.Generator(device="cuda").manual_seed(70)
+    codes = torch.empty(n * pitch, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(n * pitch // D, dtype=torch.uint8, device="cuda")
+    planes, scale_planes, held = [], [], []
+    for at in (0, 1024):   # keys and values of a position in the same stretch
+        plane = codes.as_strided((1, hkv, n, D), (n * pitch, 256, pitch, 1), at)
+        plane.copy_(torch.randint(0, 120, plane.shape, generator=gen, device="cuda").to(torch.uint8))
+        byte = scales.as_strided((1, hkv, n), (n * pitch // D, 2, pitch // D), at // D)
+        byte.copy_(torch.randint(118, 122, byte.shape, generator=gen, device="cuda").to(torch.uint8))
+        planes.append(codes[at:].view(torch.float8_e4m3fn))
+        scale_planes.append(scales[at // D:].view(torch.float8_e8m0fnu))
+        held.append(values(plane, byte).float())
+    q = torch.randn((interval, 1, hq, D), generator=gen, device="cuda").to(F16)
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:3], 7.0, device="cuda")
+    op = ellm_amd.Attention(q, *planes, out, 1, hq, hkv, D, (n * pitch, 256, pitch, 1), SCALE, lse=lse, sequence_capacity=n,
+                            kv_scales=scale_planes)
+    op.run(first, interval, 1)
+    torch.cuda.synchronize()
+    check(out, lse, reference(q, *held, [first], SCALE))
