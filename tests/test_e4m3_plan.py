@@ -1,10 +1,13 @@
 """How single-token calls over planes in 8 bits are cut (ellm_amd/csrc/decode_plan.hpp and decode_shares.hpp, host code):
 invariants over a sweep of shapes, and the plans of some shapes."""
 import os
+import re
 import shutil
 import subprocess
 
 import pytest
+
+from test_build_invariants import _listing
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "ellm_amd", "csrc")
@@ -75,3 +78,9 @@ def test_shares_of_planes_of_different_lengths(lines):
     found = {line.split()[0]: [int(x) for x in line.split()[1:]] for line in lines if not line[0].isdigit()}
     assert found["shares"] == [256, 256, 512, 512, 256]
     assert found["charge"] == [0, 3, 0, 2]
+
+
+def test_write_and_read_kernels_stay_in_registers(tmp_path):
+    text = _listing("kv_e4m3.hip", tmp_path)
+    assert set(re.findall(r"\.private_segment_fixed_size:\s*(\d+)", text)) == {"0"}
+    assert set(re.findall(r"\.[sv]gpr_spill_count:\s*(\d+)", text)) == {"0"}
