@@ -280,3 +280,49 @@ def test_rows_as_far_apart_as_the_handle_takes(interval, first):
     op.run(first, interval, 1)
     torch.cuda.synchronize()
     check(out, lse, reference(q, *held, [first], SCALE))
+
+
+def test_a_layer_with_projections():
+    """Two layers whose projections write 16-bit rows into one buffer that all layers share, from there into each layer's cache in
+    8 bits; attention over that cache; output projection and residual.  A prompt in two chunks, then single tokens."""
+    dtype, batch, hq, hkv, hidden, capacity, layers = F16, 3, 8, 2, 256, 128, 2
+    gen = torch.Generator(device="cuda").manual_seed(71)
+
+    def normal(*shape, scale=1.0):
+        return (torch.randn(shape, generator=gen, device="cuda") * scale).to(dtype)
+
+    rope = rope_table(capacity, dtype).cuda()
+    cache = ellm_amd.KVCache(layers, batch, hkv, capacity, CODE[dtype], e4m3=True)
+    k_rows, v_rows = (torch.zeros((capacity, batch, hkv, D), dtype=dtype, device="cuda") for _ in range(2))
+    shared = (hkv * D, D, batch * hkv * D, 1)   # (sequence, head, position) strides of that buffer
+    x = torch.zeros((32, batch, hidden), dtype=dtype, device="cuda")
+    q = torch.zeros((32, batch, hq, D), dtype=dtype, device="cuda")
+    att, out = torch.zeros_like(q), torch.zeros_like(x)
+    stack = []
+    for layer in range(layers):
+        wq, wk, wv = (normal(n * D, hidden, scale=hidden ** -0.5) for n in (hq, hkv, hkv))
+        wo = normal(hidden, hq * D, scale=(hq * D) ** -0.5)
+        k, v, ks, vs = cache.layer_e4m3_tensors(layer)
+        stack.append((ellm_amd.MatMul3(x, wq, q, wk, k_rows, wv, v_rows, rope, D, batch, hq, hkv, shared, capacity),
+                      ellm_amd.Attention(q, k, v, att, batch, hq, hkv, D, cache.layer_e4m3(layer).strides, SCALE,
+                                         sequence_capacity=capacity, kv_scales=(ks, vs)),
+                      ellm_amd.MatMulAdd(att.view(32, batch, hq * D), wo, x, out), wo, (k, v, ks, vs)))
+    for first, n in ellm_amd.schedule_calls(0, 52, 32, 55):
+        for layer, (project, attend, finish, wo, (k, v, ks, vs)) in enumerate(stack):
+            x[:n] = normal(n, batch, hidden)
+            project.run(first, n, batch)
+            cache.append(layer, first, k_rows[first:first + n], v_rows[first:first + n])
+            attend.run(first, n, batch)
+            finish.run(0, n, batch)
+            torch.cuda.synchronize()
+            for got, byte, rows_ in ((k, ks, k_rows), (v, vs, v_rows)):
+                codes, want_byte = hold(rows_[first:first + n].cpu(), LARGEST[dtype])
+                assert torch.equal(byte.view(torch.uint8)[:, :, first:first + n].cpu(), want_byte.permute(1, 2, 0))
+                assert torch.equal(got.view(torch.uint8)[:, :, first:first + n].cpu(), codes.permute(1, 2, 0, 3))
+            planes = [values(c.view(torch.uint8), b.view(torch.uint8)).float() for c, b in ((k, ks), (v, vs))]
+            check(att[:n], None, reference(q[:n], *planes, [first] * batch, SCALE), f"layer {layer}, {n} at {first}")
+            a, w = att[:n].reshape(-1, hq * D).double(), wo.double()
+            want = a @ w.T + x[:n].reshape(-1, hidden).double()
+            # the result rounded once, and a binary32 sum of hq * 128 products and the residual
+            bound = 2.0 ** -11 * want.abs() + (hq * D + 1) * 2.0 ** -24 * (a.abs() @ w.abs().T + x[:n].reshape(-1, hidden).double().abs())
+            assert ((out[:n].reshape(-1, hidden).double() - want).abs() <= bound * (1 + 2.0 ** -10)).all()
