@@ -26,6 +26,7 @@ namespace {
 
 constexpr uint32_t kUnitKeys = kDecodeStepKeys;   // 64: one step of the four waves
 constexpr uint32_t kMaxBatch = 1024;              // lengths are scanned in LDS
+constexpr uint32_t kSeqsThread = kMaxBatch / kDecThreads;
 static_assert(kBalancedFan == (uint32_t)kMergeFan, "decode_shares.hpp numbers the slots for this fan");
 
 // (the compiler cannot see that a value every lane computes alike is wave-uniform)
@@ -37,6 +38,21 @@ __device__ __forceinline__ uint32_t uni(uint32_t v) { return (uint32_t)__builtin
 // clusters of 16 pieces take cluster slots p + slot0 / 16 + c, which are distinct for the same
 // reason (1 + floor(n / 16) >= ceil(n / 16)).
 
+// op over the lanes below and this one; `none` is op's neutral value.  By DPP: within rows of sixteen lanes, then the rows' last
+// lanes into the rows behind them.
+template <typename Op>
+__device__ __forceinline__ uint32_t scan_lanes(uint32_t none, uint32_t v, Op op) {
+#define ELLM_DPP(ctrl, rows) (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, ctrl, rows, 0xf, false)
+  v = op(v, ELLM_DPP(0x111, 0xf));   // row_shr 1, 2, 4, 8
+  v = op(v, ELLM_DPP(0x112, 0xf));
+  v = op(v, ELLM_DPP(0x114, 0xf));
+  v = op(v, ELLM_DPP(0x118, 0xf));
+  v = op(v, ELLM_DPP(0x142, 0xa));   // row_bcast 15 into rows 1 and 3, 31 into rows 2 and 3
+  v = op(v, ELLM_DPP(0x143, 0xc));
+#undef ELLM_DPP
+  return v;
+}
+
 // PENDING: the launch of a fused step, as in decode.hip.  SHAPE: shaped scores (decode_common.hpp); lengths are then those
 // of the key ranges.  E4M3: planes of rows in 8 bits (decode_e4m3.hpp).
 template <typename T, int PENDING, int SHAPE = kShapeNone, bool E4M3 = false>
@@ -44,7 +60,7 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
   __shared__ __attribute__((aligned(16))) uint16_t smem[kDecWaves * kWaveLdsHalves];
   __shared__ uint32_t prefix[kMaxBatch + 1];   // units of the sequences before sequence b (per plane)
   __shared__ uint32_t s_pos[kMaxBatch];        // last position of every sequence
-  __shared__ uint32_t s_last, s_umax, s_umin;
+  __shared__ uint32_t s_last, s_units[kDecWaves], s_umax[kDecWaves], s_umin[kDecWaves];   // (of a wave's sequences)
   Lane t;
   const uint32_t B = p.batch;
 
@@ -58,26 +74,15 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
   auto units_of = [&](uint32_t pos) { return SHAPE != kShapeNone && pos == 0xffffffffu ? 0u : pos / kUnitKeys + 1; };
   // Units per sequence and their running sum.  Up to 64 sequences: every wave keeps them in
   // registers, sequence b in lane b (no LDS, no barrier, and the look-up below is a ballot);
-  // more: wave 0 scans them into LDS, 64 at a time.
-  auto wave_scan = [&](uint32_t v) {   // inclusive sum over the lanes below and this one
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const uint32_t below = __shfl_up(v, d, kWave);
-      if (t.lane >= d) v += below;
-    }
-    return v;
-  };
+  // more: four a thread, scanned into LDS.
+  auto lane_value = [&](uint32_t v, uint32_t l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)l); };
+  auto wave_scan = [&](uint32_t v) { return scan_lanes(0u, v, [](uint32_t a, uint32_t b) { return a + b; }); };
   auto wave_max = [&](uint32_t v) {
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) v = max(v, (uint32_t)__shfl_xor(v, d, kWave));
-    return v;
+    return lane_value(scan_lanes(0u, v, [](uint32_t a, uint32_t b) { return max(a, b); }), kWave - 1);
   };
   auto wave_min = [&](uint32_t v) {
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) v = min(v, (uint32_t)__shfl_xor(v, d, kWave));
-    return v;
+    return lane_value(scan_lanes(0xffffffffu, v, [](uint32_t a, uint32_t b) { return min(a, b); }), kWave - 1);
   };
-  auto lane_value = [&](uint32_t v, uint32_t l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)l); };
   const bool in_registers = B <= (uint32_t)kWave;   // (uniform)
   uint32_t r_pos = 0, r_units = 0, r_incl = 0, total_units, umax_all, umin_all;
   if (in_registers) {
@@ -86,32 +91,51 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
     r_units = live ? units_of(r_pos) : 0u;
     r_incl = wave_scan(r_units);
     total_units = lane_value(r_incl, kWave - 1);
-    umax_all = uni(wave_max(r_units));
-    umin_all = uni(wave_min(live ? r_units : 0xffffffffu));
+    umax_all = wave_max(r_units);
+    umin_all = wave_min(live ? r_units : 0xffffffffu);
   } else {
-    if (t.wave == 0) {
-      uint32_t carry = 0, umax = 0, umin = 0xffffffffu;
-      for (uint32_t base = 0; base < B; base += kWave) {
-        const bool live = base + t.lane < B;
-        const uint32_t pos_b = live ? position_of(base + t.lane) : 0u;
-        if (live) s_pos[base + t.lane] = pos_b;
-        const uint32_t u = live ? units_of(pos_b) : 0u;
-        const uint32_t incl = wave_scan(u);
-        if (live) prefix[base + t.lane + 1] = carry + incl;
-        carry += __shfl(incl, kWave - 1, kWave);
-        umax = max(umax, wave_max(u));
-        umin = min(umin, wave_min(live ? u : 0xffffffffu));
+    uint32_t own[kSeqsThread], sum = 0, umax = 0, umin = 0xffffffffu;
+#pragma unroll
+    for (uint32_t i = 0; i < kSeqsThread; ++i) {
+      const uint32_t b = kSeqsThread * t.tid + i;
+      own[i] = 0;
+      if (b < B) {
+        const uint32_t pos_b = position_of(b);
+        s_pos[b] = pos_b;
+        own[i] = units_of(pos_b);
+        umin = min(umin, own[i]);
       }
-      if (t.lane == 0) {
-        prefix[0] = 0;
-        s_umax = umax;
-        s_umin = umin;
-      }
+      sum += own[i];
+      umax = max(umax, own[i]);
+    }
+    const uint32_t incl = wave_scan(sum);
+    umax = wave_max(umax);
+    umin = wave_min(umin);
+    if (t.lane == kWave - 1) {
+      s_units[t.wave] = incl;
+      s_umax[t.wave] = umax;
+      s_umin[t.wave] = umin;
     }
     __syncthreads();
+    uint32_t before = incl - sum;
+    for (int w = 0; w < t.wave; ++w) before += s_units[w];
+    if (t.tid == 0) prefix[0] = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kSeqsThread; ++i) {
+      const uint32_t b = kSeqsThread * t.tid + i;
+      before += own[i];
+      if (b < B) prefix[b + 1] = before;
+    }
+    umax_all = umin_all = 0;
+#pragma unroll
+    for (int w = 0; w < kDecWaves; ++w) {
+      umax_all = max(umax_all, s_umax[w]);
+      umin_all = w ? min(umin_all, s_umin[w]) : s_umin[w];
+    }
+    umax_all = uni(umax_all);
+    umin_all = uni(umin_all);
+    __syncthreads();
     total_units = uni(prefix[B]);
-    umax_all = uni(s_umax);
-    umin_all = uni(s_umin);
   }
 
   if constexpr (SHAPE != kShapeNone) {
@@ -221,12 +245,12 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
     f32x4 acc[8];
     if constexpr (E4M3) {
       load_queries8(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
-      Stream8<T, PENDING != kPendNone> stream;
+      Stream8<T, PENDING != kPendNone, true> stream;
       stream.open(p, plane, k_begin, k_end, pos, t, w * 7u + pl * 3u + seq * 5u);
       // the piece that holds the plane's last key takes the new row; one workgroup of a group writes it
       NewRow8 fresh;
       if constexpr (PENDING) fresh = new_row8(p, plane, seq, kvh, pos, hgrp == 0);
-      stream.run(p, qreg, smem, t, m_run, l_run, acc, &fresh);
+      stream.run(p, qreg, smem, t, m_run, l_run, acc, &fresh, blockIdx.x >= p.wgs_one);
     } else if constexpr (PENDING) {
       PendingQueries queries;   // requested first: the stream's own loads follow
       if constexpr (PENDING == kPendSums) queries.fetch(p.pend, seq, head0, pos, t, heads_here);

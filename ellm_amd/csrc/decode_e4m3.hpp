@@ -87,7 +87,8 @@ __device__ __forceinline__ NewRow8 new_row8(const DecodeKernelArgs& p, size_t pl
 // One wave's share of keys [k_begin, k_end) of a plane, as stream_keys: open() sends for the first of them, run() takes them.
 // k_end is the plane's end (pos + 1) or a multiple of kChunk8 from k_begin on.  PENDING: the last key may be one that the cache
 // does not hold yet (NewRow8); the wave with the fewest chunks makes its row, writes it and takes it as a chunk of one key.
-template <typename T, bool PENDING = false>
+// TURNS: two workgroups share a unit (run).
+template <typename T, bool PENDING = false, bool TURNS = false>
 struct Stream8 {
   uint64_t kp, vp;             // the plane's codes
   const uint8_t* sp;           // the lane's scales: keys' or values'
@@ -143,10 +144,15 @@ struct Stream8 {
     if (my_chunks) fetch(first, 0, t);
   }
 
+  // TURNS: of two workgroups on a unit the first one's waves are older and are served first: they end 8 us ahead of the second's on
+  // shares of 85 us.  So the two (`second`) take turns, four chunks each, at the higher priority (us: 32 of 300-16000, 64 / 8 heads, 82.6 ->
+  // 81.8; 100 of 100-4096 48.1 -> 47.4, 64 of 100-2000 21.8 -> 20.7, 10 of 1000-60000 64.6 -> 63.8; every chunk 81.7, 47.6, 21.2, 63.6).
+  // Not where planes are cut alike (64 x 500 14.0 / 14.4).
+  //
   // The wave's reference (log2 units), its sum, and its sums of values: acc[b][r] of lane (head c, group g) is column
   // 32 g + 8 r + b.
-  __device__ __forceinline__ void run(const DecodeKernelArgs& p, const u32x4 (&qreg)[4], uint16_t* smem, const Lane& t,
-                                      float& m_out, float& l_out, f32x4 (&acc)[8], const NewRow8* fresh = nullptr) {
+  __device__ __forceinline__ void run(const DecodeKernelArgs& p, const u32x4 (&qreg)[4], uint16_t* smem, const Lane& t, float& m_out,
+                                      float& l_out, f32x4 (&acc)[8], const NewRow8* fresh = nullptr, bool second = false) {
     const int g = t.g, c = t.c;
     uint8_t* const scales = (uint8_t*)smem + kRedBytes + wave * (2 * kChunk8);   // [keys' 32][values' 32]
     float m_run = -INFINITY, l_run = 0.0f;
@@ -251,7 +257,16 @@ struct Stream8 {
         consume(one, new_pos, new_pos, 0);
       }
     }
-    for (uint32_t it = 0; it < my_chunks; ++it) consume(first, first_key(it), pos, it + 1 < my_chunks ? it + 1 : 0);
+    for (uint32_t it = 0; it < my_chunks; ++it) {
+      if constexpr (TURNS) {
+        if (((it >> 2) & 1) != (uint32_t)second)
+          __builtin_amdgcn_s_setprio(1);
+        else
+          __builtin_amdgcn_s_setprio(0);
+      }
+      consume(first, first_key(it), pos, it + 1 < my_chunks ? it + 1 : 0);
+    }
+    if constexpr (TURNS) __builtin_amdgcn_s_setprio(0);
 
     l_run += xor_shuffle(l_run, 16);
     l_run += xor_shuffle(l_run, 32);
