@@ -223,12 +223,14 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
     }
     const uint32_t a_end = a + (stop - x) - charge;   // units of keys
     // the workgroups that hold the plane's first and last unit (this one, when the piece starts
-    // or ends with the plane: no look-up then)
-    const uint32_t first_w = x <= S_keys ? w : holder(S_keys);
-    const uint32_t last_w = stop == E ? w : holder(E - 1);
-    const uint32_t n_pieces = last_w - first_w + 1, piece = w - first_w;
+    // or ends with the plane: no look-up then); E4M3: looked up with the first keys on their way
+    uint32_t first_w, last_w;
+    auto look_up = [&]() __attribute__((always_inline)) {
+      first_w = x <= S_keys ? w : holder(S_keys);
+      last_w = stop == E ? w : holder(E - 1);
+    };
+    if constexpr (!E4M3) look_up();
     const uint32_t plane_id = seq * PL + pl;
-    const uint32_t slot0 = balanced_slot0(first_w, plane_id);
 
     const uint32_t k_begin = (max(a, charge) - charge) * kUnitKeys;
     const uint32_t k_end = min(pos + 1, a_end * kUnitKeys);
@@ -247,6 +249,8 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
       load_queries8(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
       Stream8<T, PENDING != kPendNone, true> stream;
       stream.open(p, plane, k_begin, k_end, pos, t, w * 7u + pl * 3u + seq * 5u);
+      __builtin_amdgcn_sched_barrier(0);
+      look_up();
       // the piece that holds the plane's last key takes the new row; one workgroup of a group writes it
       NewRow8 fresh;
       if constexpr (PENDING) fresh = new_row8(p, plane, seq, kvh, pos, hgrp == 0);
@@ -272,6 +276,8 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
                      w * 7u + pl * 3u + seq * 5u, score, m_run, l_run, acc);
     }
 
+    const uint32_t n_pieces = last_w - first_w + 1, piece = w - first_w;
+    const uint32_t slot0 = balanced_slot0(first_w, plane_id);
     auto final_row = [&](uint32_t h, uint32_t dq, const f32x4& av, float l, float m) {
       emit_joined<T, SHAPE>(p, (size_t)(row0 + h), dq, av, l, m);
     };
