@@ -166,9 +166,9 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
   // its own start-up that a second workgroup on the unit hides (400 planes of 100-4096 keys).
   // (decode_shares.hpp: balanced_workgroups, also walked by the CPU tests)
   const uint32_t planes_all = PL * B;
-  const uint32_t one_each =
-      E4M3 ? balanced_one_each_e4m3(gridDim.x, p.wgs_one, U, umax_all == umin_all, planes_all) : p.wgs_one;
-  const uint32_t W = balanced_workgroups(gridDim.x, one_each, U, umax_all + charge, umin_all + charge, planes_all);
+  const uint32_t W =
+      E4M3 ? balanced_workgroups_e4m3(gridDim.x, p.wgs_one, U, umax_all + charge, umin_all + charge, planes_all, umax_all)
+           : balanced_workgroups(gridDim.x, p.wgs_one, U, umax_all + charge, umin_all + charge, planes_all);
   // Workgroups are dealt to the eight XCDs by their id modulo 8.  Each XCD takes one contiguous
   // eighth of the shares, so that no two of them walk the same stretch of memory side by side
   // (with shares numbered like the workgroups and as many pieces per plane as XCDs, every XCD

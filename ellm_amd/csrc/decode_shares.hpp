@@ -94,13 +94,20 @@ ELLM_SHARES_FN uint32_t balanced_workgroups(uint32_t launched, uint32_t one_each
   }
   return W;
 }
-// What balanced_workgroups takes as `one_each` where rows are in 8 bits: a workgroup of those has more to compute for a byte, and two
-// on a unit fill each other's waits.  One on a unit only for planes of equal length, whose partial results count, and for few short
-// shares of few planes (us, one / two a unit: 32 of 300-16000, 64 / 8 heads, 112 / 103; 64 of 100-2000, 32 / 4, 24.0 / 22.3; 15 of 8192
-// and one of 8101 30.5 / 28.5; 24 of 1000-60000 131.2 / 129.8; but 64 of 2048 23.1 / 26.9, 16 of 64-8000 17.7 / 19.0).
-ELLM_SHARES_FN uint32_t balanced_one_each_e4m3(uint32_t launched, uint32_t one_each, uint32_t U, bool equal_planes,
-                                               uint32_t planes) {
-  return equal_planes || (2u * planes <= one_each && U < 12u * launched) ? one_each : launched;
+// The same where rows are in 8 bits: a workgroup of those has more to compute for a byte, and two on a unit fill each other's waits.  One
+// on a unit all the same for planes of equal length, whose partial results count (us, one / two a unit, bfloat16: 64 of 2048 keys, 32 / 4
+// heads, 22.9 / 26.0); where two would cut the longest plane (`longest` units of keys) into more pieces than one fold takes and one would
+// not (4 of 5742-11482, 40 / 8 heads, 19.8 / 21.9; 9 of 376-18764, 32 / 4, 23.6 / 25.3); and for long shares, whose starts count for little
+// (10 of 4599-45981, 32 / 4, 47.0 / 49.5; 28 of 6377-12753, 64 / 8, 88.2 / 90.7).  Else two: 32 of 228-2279, 32 / 4, 15.7 / 14.1;
+// 7 of 2993-5985, 40 / 8, 18.9 / 18.0; 4 of 32257-35841, 32 / 4, 33.3 / 30.9; 18 of 206-10269, 64 / 8, 40.8 / 39.2.  Over 46 drawn calls
+// the choice is the better one but for ties of a per cent.
+ELLM_SHARES_FN uint32_t balanced_workgroups_e4m3(uint32_t launched, uint32_t one_each, uint32_t U, uint32_t umax,
+                                                 uint32_t umin, uint32_t planes, uint32_t longest) {
+  if (umax == umin) return balanced_workgroups(launched, one_each, U, umax, umin, planes);
+  const uint64_t fold = (uint64_t)kBalancedFan * U;
+  const bool folds = (uint64_t)longest * one_each <= fold && (uint64_t)longest * launched > fold;
+  const bool one = planes <= one_each && (folds || U >= 25u * launched);
+  return balanced_takers(one ? one_each : launched, U, balanced_min_share(umax), false, planes);
 }
 // The share workgroup `id` takes: each XCD (id % 8) one contiguous eighth when W allows.
 ELLM_SHARES_FN uint32_t balanced_share_of(uint32_t id, uint32_t W) {

@@ -32,10 +32,13 @@ int main() {
                    (int)decode_plan_fits(w, batch, h[0], h[1], h[0] / h[1], p.n_split));
           }
       }
-  // workgroups a launch of 512 keeps as "one each" of 256: equal planes, few short ones, many or long ones
-  printf("shares %u %u %u %u %u\n", balanced_one_each_e4m3(512, 256, 512 * 9, true, 256),
-         balanced_one_each_e4m3(512, 256, 512 * 11, false, 64), balanced_one_each_e4m3(512, 256, 512 * 11, false, 256),
-         balanced_one_each_e4m3(512, 256, 512 * 12, false, 64), balanced_one_each_e4m3(512, 256, 512 * 40, true, 16));
+  // workgroups out of 512 and 256: equal planes; a longest plane of 22 pieces on 512 and 11 on 256, of 12 and 6, of 44 and 22; more planes
+  // than units; long shares; the largest call, whose longest plane is all of it: 254 pieces are the most that two folds take, 248 the multiple of 8
+  const uint32_t U = 512 * 9;
+  printf("shares %u %u %u %u %u %u %u\n", balanced_workgroups_e4m3(512, 256, 64 * 36, 36, 36, 64, 36),
+         balanced_workgroups_e4m3(512, 256, U, 201, 9, 40, 198), balanced_workgroups_e4m3(512, 256, U, 111, 9, 60, 108),
+         balanced_workgroups_e4m3(512, 256, U, 399, 9, 20, 396), balanced_workgroups_e4m3(512, 256, 512 * 40, 201, 9, 257, 198),
+         balanced_workgroups_e4m3(512, 256, 512 * 25, 53, 9, 256, 50), balanced_workgroups_e4m3(512, 256, 0x7fffffffu, 0x7ffffffeu, 4, 2, 0x7ffffffbu));
   // what a plane's start is charged with: nothing for equal or long planes
   printf("charge %u %u %u %u\n", balanced_charge(10, 10, 100, 10, kBalancedChargeE4m3), balanced_charge(10, 9, 100, 10, kBalancedChargeE4m3),
          balanced_charge(900, 9, 5130, 10, kBalancedChargeE4m3), balanced_charge(10, 9, 100, 10));
@@ -76,7 +79,7 @@ def test_plans_are_well_formed_and_fit_the_workspace(lines):
 
 def test_shares_of_planes_of_different_lengths(lines):
     found = {line.split()[0]: [int(x) for x in line.split()[1:]] for line in lines if not line[0].isdigit()}
-    assert found["shares"] == [256, 256, 512, 512, 256]
+    assert found["shares"] == [256, 256, 512, 512, 512, 256, 248]
     assert found["charge"] == [0, 3, 0, 2]
 
 
