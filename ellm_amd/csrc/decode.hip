@@ -73,11 +73,11 @@ __global__ __launch_bounds__(kDecThreads, PENDING || E4M3 ? 2 : 4) void decode_s
   if constexpr (E4M3) {
     load_queries8(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
     Stream8<T, PENDING != kPendNone> stream;
-    stream.open(p, plane, k_begin, k_end, pos, t, split * 7u + blockIdx.y * 3u + seq * 5u);
     // the split that holds the plane's last key takes the new row; one workgroup of a group writes it
     NewRow8 fresh;
     if constexpr (PENDING) fresh = new_row8(p, plane, seq, kvh, pos, hgrp == 0);
-    stream.run(p, qreg, smem, t, m_run, l_run, acc, &fresh);
+    stream.open(p, plane, k_begin, k_end, pos, t, split * 7u + blockIdx.y * 3u + seq * 5u, fresh);
+    stream.run(p, qreg, smem, t, m_run, l_run, acc, fresh);
   } else if constexpr (PENDING) {
     PendingQueries queries;   // requested first: the stream's own loads follow
     if constexpr (PENDING == kPendSums) queries.fetch(p.pend, seq, head0, pos, t, heads_here);

@@ -167,7 +167,8 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
   // (decode_shares.hpp: balanced_workgroups, also walked by the CPU tests)
   const uint32_t planes_all = PL * B;
   const uint32_t W =
-      E4M3 ? balanced_workgroups_e4m3(gridDim.x, p.wgs_one, U, umax_all + charge, umin_all + charge, planes_all, umax_all)
+      E4M3 ? balanced_workgroups_e4m3(gridDim.x, p.wgs_one, U, umax_all + charge, umin_all + charge, planes_all, umax_all,
+                                      PENDING != kPendNone)
            : balanced_workgroups(gridDim.x, p.wgs_one, U, umax_all + charge, umin_all + charge, planes_all);
   // Workgroups are dealt to the eight XCDs by their id modulo 8.  Each XCD takes one contiguous
   // eighth of the shares, so that no two of them walk the same stretch of memory side by side
@@ -248,13 +249,13 @@ __global__ __launch_bounds__(kDecThreads, 2) void decode_balanced_kernel(DecodeK
     if constexpr (E4M3) {
       load_queries8(p.q + (size_t)row0 * kHeadDim, t, heads_here, qreg);
       Stream8<T, PENDING != kPendNone, true> stream;
-      stream.open(p, plane, k_begin, k_end, pos, t, w * 7u + pl * 3u + seq * 5u);
-      __builtin_amdgcn_sched_barrier(0);
-      look_up();
       // the piece that holds the plane's last key takes the new row; one workgroup of a group writes it
       NewRow8 fresh;
       if constexpr (PENDING) fresh = new_row8(p, plane, seq, kvh, pos, hgrp == 0);
-      stream.run(p, qreg, smem, t, m_run, l_run, acc, &fresh, blockIdx.x >= p.wgs_one);
+      stream.open(p, plane, k_begin, k_end, pos, t, w * 7u + pl * 3u + seq * 5u, fresh);
+      __builtin_amdgcn_sched_barrier(0);
+      look_up();
+      stream.run(p, qreg, smem, t, m_run, l_run, acc, fresh, blockIdx.x >= p.wgs_one);
     } else if constexpr (PENDING) {
       PendingQueries queries;   // requested first: the stream's own loads follow
       if constexpr (PENDING == kPendSums) queries.fetch(p.pend, seq, head0, pos, t, heads_here);

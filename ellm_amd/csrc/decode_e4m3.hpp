@@ -95,6 +95,7 @@ struct Stream8 {
   uint32_t pitch, pos, k_begin, my_chunks, rot, wave;
   bool take_new;               // (PENDING) this wave takes the new row ...
   uint32_t new_pos;            // ... of this position
+  u32x4 k_new, v_new, turn;    // ... and has its source rows
   Chunk8 first;
 
   __device__ __forceinline__ uint32_t first_key(uint32_t it) const {
@@ -122,7 +123,7 @@ struct Stream8 {
   }
 
   __device__ __forceinline__ void open(const DecodeKernelArgs& p, size_t plane, uint32_t begin, uint32_t end, uint32_t last,
-                                       const Lane& t, uint32_t rot_seed) {
+                                       const Lane& t, uint32_t rot_seed, const NewRow8& fresh) {
     wave = scalar(t.wave);
     const uint64_t at = scalar64(plane);
     kp = scalar64((uint64_t)p.k + at);
@@ -141,6 +142,13 @@ struct Stream8 {
     take_new = with_new && wave == n_chunks % kDecWaves;   // (uniform over the wave)
     my_chunks = n_chunks > wave ? (n_chunks - wave + kDecWaves - 1) / kDecWaves : 0;
     rot = scalar(rot_seed % max(my_chunks, 1u));
+    if constexpr (PENDING) {   // ahead of the wave's first chunk, which arrives while the row is made
+      if (take_new) {
+        k_new = load16(fresh.k_row + 8 * t.c);
+        v_new = load16(fresh.v_row + 8 * t.c);
+        turn = load16(fresh.rope_row + 8 * t.c);
+      }
+    }
     if (my_chunks) fetch(first, 0, t);
   }
 
@@ -152,7 +160,7 @@ struct Stream8 {
   // The wave's reference (log2 units), its sum, and its sums of values: acc[b][r] of lane (head c, group g) is column
   // 32 g + 8 r + b.
   __device__ __forceinline__ void run(const DecodeKernelArgs& p, const u32x4 (&qreg)[4], uint16_t* smem, const Lane& t, float& m_out,
-                                      float& l_out, f32x4 (&acc)[8], const NewRow8* fresh = nullptr, bool second = false) {
+                                      float& l_out, f32x4 (&acc)[8], const NewRow8& fresh, bool second = false) {
     const int g = t.g, c = t.c;
     uint8_t* const scales = (uint8_t*)smem + kRedBytes + wave * (2 * kChunk8);   // [keys' 32][values' 32]
     float m_run = -INFINITY, l_run = 0.0f;
@@ -224,11 +232,9 @@ struct Stream8 {
 
     if constexpr (PENDING) {
       if (take_new) {
-        // (behind the wave's first chunk: both trips to memory run side by side)
-        const u32x4 k_new = load16(fresh->k_row + 8 * c), v_new = load16(fresh->v_row + 8 * c), turn = load16(fresh->rope_row + 8 * c);
         float x[8];
         unpack8<T>(k_new, x);
-        norm_rope8<T>(x, turn, fresh->eps);
+        norm_rope8<T>(x, turn, fresh.eps);
         uint32_t kb, vb;
         const u32x2 k = row_codes16<T>(x, kb);
         unpack8<T>(v_new, x);
@@ -237,12 +243,12 @@ struct Stream8 {
         if (g == 0) {
           *(u32x2*)(rows + 8 * c) = k;
           *(u32x2*)(rows + kHeadDim + 8 * c) = v;
-          if (fresh->store) {
-            *(u32x2*)(fresh->k_dst + 8 * c) = k;
-            *(u32x2*)(fresh->v_dst + 8 * c) = v;
+          if (fresh.store) {
+            *(u32x2*)(fresh.k_dst + 8 * c) = k;
+            *(u32x2*)(fresh.v_dst + 8 * c) = v;
             if (c == 0) {
-              *fresh->k_scale = (uint8_t)kb;
-              *fresh->v_scale = (uint8_t)vb;
+              *fresh.k_scale = (uint8_t)kb;
+              *fresh.v_scale = (uint8_t)vb;
             }
           }
         }

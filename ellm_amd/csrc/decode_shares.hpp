@@ -96,17 +96,18 @@ ELLM_SHARES_FN uint32_t balanced_workgroups(uint32_t launched, uint32_t one_each
 }
 // The same where rows are in 8 bits: a workgroup of those has more to compute for a byte, and two on a unit fill each other's waits.  One
 // on a unit all the same for planes of equal length, whose partial results count (us, one / two a unit, bfloat16: 64 of 2048 keys, 32 / 4
-// heads, 22.9 / 26.0); where two would cut the longest plane (`longest` units of keys) into more pieces than one fold takes and one would
-// not (4 of 5742-11482, 40 / 8 heads, 19.8 / 21.9; 9 of 376-18764, 32 / 4, 23.6 / 25.3); and for long shares, whose starts count for little
-// (10 of 4599-45981, 32 / 4, 47.0 / 49.5; 28 of 6377-12753, 64 / 8, 88.2 / 90.7).  Else two: 32 of 228-2279, 32 / 4, 15.7 / 14.1;
-// 7 of 2993-5985, 40 / 8, 18.9 / 18.0; 4 of 32257-35841, 32 / 4, 33.3 / 30.9; 18 of 206-10269, 64 / 8, 40.8 / 39.2.  Over 46 drawn calls
-// the choice is the better one but for ties of a per cent.
+// heads, 22.9 / 26.0); and where one cuts the longest plane (`longest` units of keys) into no more pieces than one fold takes, if two would
+// cut it into more (4 of 5742-11482, 40 / 8 heads, 19.8 / 21.9; 9 of 376-18764, 32 / 4, 23.6 / 25.3) or shares are long, so that their
+// starts count for little (28 of 6377-12753, 64 / 8, 88.2 / 90.7; 32 of 300-16000, 64 / 8, 98.5 / 99.6), but not with `new_rows` to write, which
+// a second workgroup hides (that call as a step 102.2 / 100.8; 64 of 500-9000, 32 / 4, 61.4 / 60.1).  Else two: 32 of 228-2279, 32 / 4, 15.7
+// / 14.1; 7 of 2993-5985, 40 / 8, 18.9 / 18.0; 3 of 20000-100000, 32 / 4, 49.8 / 48.0; 18 of 206-10269, 64 / 8, 40.8 / 39.2.
 ELLM_SHARES_FN uint32_t balanced_workgroups_e4m3(uint32_t launched, uint32_t one_each, uint32_t U, uint32_t umax,
-                                                 uint32_t umin, uint32_t planes, uint32_t longest) {
+                                                 uint32_t umin, uint32_t planes, uint32_t longest,
+                                                 bool new_rows) {
   if (umax == umin) return balanced_workgroups(launched, one_each, U, umax, umin, planes);
   const uint64_t fold = (uint64_t)kBalancedFan * U;
-  const bool folds = (uint64_t)longest * one_each <= fold && (uint64_t)longest * launched > fold;
-  const bool one = planes <= one_each && (folds || U >= 25u * launched);
+  const bool one = planes <= one_each && (uint64_t)longest * one_each <= fold &&
+                   ((uint64_t)longest * launched > fold || (!new_rows && U >= 25u * launched));
   return balanced_takers(one ? one_each : launched, U, balanced_min_share(umax), false, planes);
 }
 // The share workgroup `id` takes: each XCD (id % 8) one contiguous eighth when W allows.

@@ -33,12 +33,15 @@ int main() {
           }
       }
   // workgroups out of 512 and 256: equal planes; a longest plane of 22 pieces on 512 and 11 on 256, of 12 and 6, of 44 and 22; more planes
-  // than units; long shares; the largest call, whose longest plane is all of it: 254 pieces are the most that two folds take, 248 the multiple of 8
+  // than units; long shares, without and with new rows to write, and of a plane of 17 pieces on 256; the largest call, whose longest plane
+  // is all of it: 254 pieces are the most that two folds take, 248 the multiple of 8
   const uint32_t U = 512 * 9;
-  printf("shares %u %u %u %u %u %u %u\n", balanced_workgroups_e4m3(512, 256, 64 * 36, 36, 36, 64, 36),
-         balanced_workgroups_e4m3(512, 256, U, 201, 9, 40, 198), balanced_workgroups_e4m3(512, 256, U, 111, 9, 60, 108),
-         balanced_workgroups_e4m3(512, 256, U, 399, 9, 20, 396), balanced_workgroups_e4m3(512, 256, 512 * 40, 201, 9, 257, 198),
-         balanced_workgroups_e4m3(512, 256, 512 * 25, 53, 9, 256, 50), balanced_workgroups_e4m3(512, 256, 0x7fffffffu, 0x7ffffffeu, 4, 2, 0x7ffffffbu));
+  auto W = [](uint32_t U, uint32_t longest, uint32_t umin, uint32_t planes, bool rows) {
+    return balanced_workgroups_e4m3(512, 256, U, longest + 3, umin + 3, planes, longest, rows);
+  };
+  printf("shares %u %u %u %u %u %u %u %u %u\n", W(64 * 36, 36, 36, 64, false), W(U, 198, 6, 40, true), W(U, 108, 6, 60, false),
+         W(U, 396, 6, 20, false), W(512 * 40, 198, 6, 257, false), W(512 * 25, 50, 6, 256, false), W(512 * 25, 50, 6, 256, true),
+         W(512 * 25, 50 * 17, 6, 256, false), W(0x7fffffffu, 0x7ffffffbu, 1, 2, false));
   // what a plane's start is charged with: nothing for equal or long planes
   printf("charge %u %u %u %u\n", balanced_charge(10, 10, 100, 10, kBalancedChargeE4m3), balanced_charge(10, 9, 100, 10, kBalancedChargeE4m3),
          balanced_charge(900, 9, 5130, 10, kBalancedChargeE4m3), balanced_charge(10, 9, 100, 10));
@@ -79,7 +82,7 @@ def test_plans_are_well_formed_and_fit_the_workspace(lines):
 
 def test_shares_of_planes_of_different_lengths(lines):
     found = {line.split()[0]: [int(x) for x in line.split()[1:]] for line in lines if not line[0].isdigit()}
-    assert found["shares"] == [256, 256, 512, 512, 512, 256, 248]
+    assert found["shares"] == [256, 256, 512, 512, 512, 256, 512, 512, 248]
     assert found["charge"] == [0, 3, 0, 2]
 
 
