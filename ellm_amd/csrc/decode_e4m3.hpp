@@ -12,7 +12,7 @@
 // Vector instructions of a chunk (8 KB): 64 conversions, 32 permutes, some 110 for the soft-max and addresses; with the matrix
 // instructions about 1100 cycles of a SIMD, a third of the time the chunk takes to arrive at the card's rate.  A wave has one chunk
 // on its way while it computes on the one before, sent for when that one is converted and its registers are free; two or three
-// ahead measured worse.  Measured (32 / 4 heads, bfloat16): 16 x 65536 keys 155 us, 6.97 TB/s; 24 of 1000-60000 130 us, 6.25 TB/s;
+// ahead measured worse.  Measured (32 / 4 heads, bfloat16): 16 x 65536 keys 155 us, 6.97 TB/s; 24 of 1000-60000 131 us, 6.3 TB/s;
 // 16 x 8192 24.5 us, 5.5 TB/s.
 #pragma once
 
