@@ -326,3 +326,23 @@ def test_a_layer_with_projections():
             # the result rounded once, and a binary32 sum of hq * 128 products and the residual
             bound = 2.0 ** -11 * want.abs() + (hq * D + 1) * 2.0 ** -24 * (a.abs() @ w.abs().T + x[:n].reshape(-1, hidden).double().abs())
             assert ((out[:n].reshape(-1, hidden).double() - want).abs() <= bound * (1 + 2.0 ** -10)).all()
+
+
+@pytest.mark.parametrize("batch,longest", [(65, 4100), (257, 1030), (300, 900), (1024, 260)])
+def test_many_sequences_of_different_lengths(batch, longest):
+    """More sequences than a wave has lanes, up to the most that a launch deals evenly: lengths from one key on."""
+    gen = torch.Generator().manual_seed(batch)
+    lengths = torch.randint(1, longest + 1, (batch,), generator=gen).tolist()
+    lengths[0], lengths[-1], lengths[batch // 2] = longest, 1, longest
+    step, apart = (Layer(72, BF16, 2, 1, [longest] * batch, uniform=True) for _ in range(2))
+    assert step.op.ragged_path(longest - 1, batch) == 1
+    positions = [n - 1 for n in lengths]
+    at = torch.tensor(positions, dtype=torch.int32, device="cuda")
+    k, v = _new(73, batch, 1, BF16)
+    rope = rope_table(longest, BF16).cuda()
+    step.cache.append_norm_rope_with_attention(0, step.op, 0, k, v, rope, positions=at, max_position=longest - 1)
+    apart.cache.append_norm_rope(0, 0, k, v, rope, positions=at, max_position=longest - 1)
+    assert _same_bits(step, apart)
+    step.check(positions)
+    step.op.run_ragged(at, longest - 1, batch)   # the same keys, all of the cache now
+    step.check(positions)
