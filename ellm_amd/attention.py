@@ -102,6 +102,10 @@ class Attention:
         if self._e4m3:
             scales = [_device_buffer(name, t, (kv_span + 127) // 128, torch.float8_e8m0fnu)
                       for name, t in zip(("k_scale", "v_scale"), kv_scales)]
+            for name, t, codes in zip(("k_scale", "v_scale"), kv_scales, (k, v)):
+                if t.dim() == codes.dim() - 1 and any(n > 1 and s * 128 != step
+                                                      for n, s, step in zip(t.shape, t.stride(), codes.stride())):
+                    raise ValueError(f"{name} must be laid out as the rows are: strides {t.stride()} for codes of {codes.stride()}")
         d.lse = _device_buffer("lse", lse, rows, torch.float32) if lse is not None else None
         d.batch_size = batch_size
         d.attention_head_num = attention_head_num

@@ -816,7 +816,9 @@ int ellm_kv_read_e4m3(const ellm_kv_cache* c, size_t layer, size_t first_sequenc
   for (int i : axis) {
     if (extent[i] <= 1) continue;
     if (dst_strides[i] < span) return fail(ELLM_ERR_INVALID_ARGUMENT, "dst_strides[%d] = %zu puts rows onto one another", i, dst_strides[i]);
-    span += (extent[i] - 1) * dst_strides[i];
+    size_t more = 0;
+    if (__builtin_mul_overflow(extent[i] - 1, dst_strides[i], &more) || __builtin_add_overflow(span, more, &span) || span >= ((size_t)1 << 60))
+      return fail(ELLM_ERR_INVALID_ARGUMENT, "dst_strides[%d] = %zu reaches past any address", i, dst_strides[i]);
   }
   if (layer >= c->desc.layers) return fail(ELLM_ERR_OUT_OF_RANGE, "layer %zu of %zu", layer, c->desc.layers);
   if (first_sequence >= c->desc.sequences || batch_size > c->desc.sequences - first_sequence)

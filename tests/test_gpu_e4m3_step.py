@@ -1,5 +1,6 @@
 """Steps over caches in 8 bits where one launch writes the new rows and attends over them: the cache bit for bit as the write
 alone leaves it, and the attention of the cache as it then stands."""
+import ctypes
 import math
 
 import pytest
@@ -346,3 +347,24 @@ def test_many_sequences_of_different_lengths(batch, longest):
     step.check(positions)
     step.op.run_ragged(at, longest - 1, batch)   # the same keys, all of the cache now
     step.check(positions)
+
+
+def test_strides_past_any_address_are_refused():
+    cache = ellm_amd.KVCache(1, 3, 2, 8, CODE[F16], e4m3=True)
+    out = torch.zeros(64 * D, dtype=F16, device="cuda")
+    lib = ellm_amd.load_library()
+    for strides in ((1 << 62, 2 * D, D), (1 << 63, 2 * D, D), (2 * D, 1 << 61, D), ((1 << 64) - 8, 2 * D, D)):
+        steps = (ctypes.c_size_t * 3)(*strides)
+        assert lib.ellm_kv_read_e4m3(cache._handle, 0, 0, 0, 8, 3, out.data_ptr(), out.data_ptr(), steps, None) == 1
+
+
+def test_scales_laid_out_otherwise_than_their_rows_are_refused():
+    codes = torch.zeros((2, 3, 40, D), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    scales = torch.zeros((2, 3, 40), dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+    q = torch.zeros((1, 2, 3, D), dtype=F16, device="cuda")
+    out = torch.zeros_like(q)
+    turned = scales.view(torch.uint8).transpose(1, 2).contiguous().transpose(1, 2).view(torch.float8_e8m0fnu)
+    for ks, vs in ((turned, scales), (scales, turned)):
+        with pytest.raises(ValueError):
+            ellm_amd.Attention(q, codes, codes, out, 2, 3, 3, D, codes.stride(), SCALE, kv_scales=(ks, vs))
+    ellm_amd.Attention(q, codes, codes, out, 2, 3, 3, D, codes.stride(), SCALE, kv_scales=(scales, scales.flatten()))
