@@ -311,14 +311,17 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(Prefill
   // (the group comes as a compile-time constant where the caller runs behind the scalar
   // branch on the group, as the run-time value in the prologue)
   // base: step_base of this lane's place in the destination buffer
-  auto store_piece = [&](auto group, uint32_t base, int i) __attribute__((always_inline)) {
+  auto piece_at = [&](auto, uint32_t base, int i) __attribute__((always_inline)) {
     const uint32_t pitch = 2 * (uint32_t)kVsPitch;
+    return (LdsU32x4*)(base + (E4M3 ? 32 * (i >> 1) * pitch + 16 * (i & 1) : 16 * i * pitch));
+  };
+  auto store_piece = [&](auto group, uint32_t base, int i) __attribute__((always_inline)) {
     if constexpr (E4M3) {
       const u32x4& x = stg[i >> 1];
-      *(LdsU32x4*)(base + 32 * (i >> 1) * pitch + 16 * (i & 1)) =
+      *piece_at(group, base, i) =
           values8<T>(u32x2{x[2 * (i & 1)], x[2 * (i & 1) + 1]}, group ? value_scale(v_scales[i >> 1]) : key_scale(k_scales[i >> 1], v_scales[i >> 1]));
     } else {
-      *(LdsU32x4*)(base + 16 * i * pitch) = stg[i];
+      *piece_at(group, base, i) = stg[i];
     }
   };
   auto load_tile = [&](auto group, uint32_t kt) __attribute__((always_inline)) {
@@ -378,10 +381,10 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong_kernel(Prefill
     asm volatile("s_waitcnt vmcnt(8)" ::: "memory");   // 4 (kPpAhead - 1): tile 0 is there
   } else {
     auto begin = [&](auto group) __attribute__((always_inline)) {
-      if (group) {
+      if (group) {   // V(-1): zeros as they are (no scale has arrived yet)
+        const uint32_t base = store_base(group, 2);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) stg[i] = u32x4{0u, 0u, 0u, 0u};
-        store_tile(group, 2);
+        for (int i = 0; i < 4; ++i) *piece_at(group, base, i) = u32x4{0u, 0u, 0u, 0u};
       }
       load_tile(group, 0);
       store_tile(group, 0);
@@ -729,14 +732,17 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong32_kernel(Prefi
       stg[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, piece_off[i], 0, 0);
     }
   };
-  auto store_piece = [&](auto group, uint32_t base, int i) __attribute__((always_inline)) {
+  auto piece_at = [&](auto group, uint32_t base, int i) __attribute__((always_inline)) {
     const uint32_t pitch = 2 * (uint32_t)(group ? kVsPitch : kKsPitch);
+    return (LdsU32x4*)(base + (E4M3 ? 32 * (i >> 1) * pitch + 16 * (i & 1) : 16 * i * pitch));
+  };
+  auto store_piece = [&](auto group, uint32_t base, int i) __attribute__((always_inline)) {
     if constexpr (E4M3) {
       const u32x4& x = stg[i >> 1];
-      *(LdsU32x4*)(base + 32 * (i >> 1) * pitch + 16 * (i & 1)) =
+      *piece_at(group, base, i) =
           values8<T>(u32x2{x[2 * (i & 1)], x[2 * (i & 1) + 1]}, group ? value_scale(v_scales[i >> 1]) : key_scale(k_scales[i >> 1], v_scales[i >> 1]));
     } else {
-      *(LdsU32x4*)(base + 16 * i * pitch) = stg[i];
+      *piece_at(group, base, i) = stg[i];
     }
   };
   auto load_tile = [&](auto group, uint32_t kt) __attribute__((always_inline)) {
@@ -764,10 +770,10 @@ __global__ __launch_bounds__(kPpThreads, 2) void prefill_pingpong32_kernel(Prefi
   for (int cc = 0; cc < 4; ++cc) pk[cc] = u32x4{0u, 0u, 0u, 0u};  // P(-1) = 0
 
   auto begin = [&](auto group) __attribute__((always_inline)) {
-    if (group) {
+    if (group) {   // V(-1): zeros as they are (no scale has arrived yet)
+      const uint32_t base = store_base(group, 2);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) stg[i] = u32x4{0u, 0u, 0u, 0u};
-      store_tile(group, 2);
+      for (int i = 0; i < 4; ++i) *piece_at(group, base, i) = u32x4{0u, 0u, 0u, 0u};
     }
     load_tile(group, 0);
     store_tile(group, 0);
