@@ -175,7 +175,7 @@ struct Stream8 {
       u32x4 kv[2][4], value[8];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const uint32_t scale = scales[16 * b + c];
+        const uint32_t scale = key_scale(scales[16 * b + c], scales[kChunk8 + 16 * b + c]);
 #pragma unroll
         for (int s = 0; s < 4; ++s) kv[b][s] = values8<T>(u32x2{x.k[b][s >> 1][2 * (s & 1)], x.k[b][s >> 1][2 * (s & 1) + 1]}, scale);
       }

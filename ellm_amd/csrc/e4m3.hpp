@@ -51,9 +51,9 @@ __device__ __forceinline__ u32x4 values8(u32x2 codes, uint32_t scale) {
   const u32x2 lo = values4<T>(codes[0], scale_of(scale)), hi = values4<T>(codes[1], scale_of(scale));
   return u32x4{lo[0], lo[1], hi[0], hi[1]};
 }
-// The scales that a chunk's kernels take a key row and its value row with.  A value row whose scale is NaN is taken as what its codes
-// say (zeros, where the cache wrote them) and its key's scale as NaN instead: rows that see the key get weights, and so
-// results, of NaN; rows that do not see it yet give it a weight of exactly 0, and 0 x NaN would be NaN.
+// The scales that a key row and its value row are taken with.  The key of a value row whose scale is NaN has a scale of NaN too: rows
+// that see it get weights of NaN, and so both results.  A chunk's kernels take the value row itself as what its codes say (zeros,
+// where the cache wrote them): rows that do not see it yet give it a weight of exactly 0, and 0 x NaN would be NaN.
 __device__ __forceinline__ uint32_t key_scale(uint32_t k, uint32_t v) { return v == kScaleNan ? kScaleNan : k; }
 __device__ __forceinline__ uint32_t value_scale(uint32_t v) { return v == kScaleNan ? 127u : v; }
 

@@ -379,7 +379,8 @@ int ellm_kv_read_e4m3(const ellm_kv_cache* cache, size_t layer, size_t first_seq
  * with v likewise; desc->dtype is the type of q and out, in which the rows' values are taken (exact for rows that the cache
  * wrote from that type, or from binary16 under bfloat16).  head_size 128, 16-bit dtype.  Any codes and scales in that layout
  * will do, not only a cache's; codes of NaN in value rows count as infinities do in ellm_attn_run (rows that do not see
- * them yet must not meet them in a chunk), scales of NaN are seen by the rows that see the key only.
+ * them yet must not meet them in a chunk), scales of NaN are seen by the rows that see the key only: a NaN scale of a position's
+ * key or value row makes both results of those, out and lse, NaN.
  * Runs as of any handle (ellm_attn_run, ellm_attn_run_ragged, ellm_kv_append_attn_run*).  ellm_attn_set_scores, ellm_attn_set_shared_prefix and ellm_matmul3_attn_run* refuse such a handle. */
 int ellm_attn_create_e4m3(const ellm_attn_desc* desc, const uint8_t* k_scale, const uint8_t* v_scale,
                           const ellm_kv_seq_table* table, ellm_attn** out_handle);

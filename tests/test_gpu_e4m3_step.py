@@ -131,6 +131,37 @@ def test_new_rows_that_are_not_finite(batch, position):
     assert torch.equal(torch.isnan(step.out).all(dim=-1), bad) and torch.equal(torch.isnan(step.out).any(dim=-1), bad)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hq,hkv,batch,keys", [(8, 2, 2, 200), (17, 1, 3, 700), (8, 4, 8, 9000)])
+def test_what_sees_a_row_that_is_nan_has_no_log_sum(dtype, hq, hkv, batch, keys):
+    """A key or a value row whose scale is NaN: both results of single tokens that see it are NaN, as a chunk's are; and of a step
+    that writes such a row."""
+    t = Layer(59, dtype, hq, hkv, [keys] * batch, uniform=True)
+    bad, group = keys // 2 + 5, hq // hkv
+    first = [keys - 1 - 7 * i for i in range(batch)]
+    first[1] = bad - 1   # does not see it
+    at = torch.tensor(first, dtype=torch.int32, device="cuda")
+    sees = torch.zeros(t.out.shape[:3], dtype=torch.bool, device="cuda")
+    sees[0, 0, :group] = True
+    t.op.run_ragged(at, keys - 1, batch)
+    torch.cuda.synchronize()
+    out, lse = t.out.clone(), t.lse.clone()
+    t.check(first)
+    for _, byte in t.tensors():
+        was = byte[:2, 0, bad].clone()
+        byte[:2, 0, bad] = 255
+        t.op.run_ragged(at, keys - 1, batch)
+        torch.cuda.synchronize()
+        assert torch.equal(torch.isnan(t.lse), sees) and torch.equal(torch.isnan(t.out).all(dim=-1), sees)
+        assert torch.equal(t.out[~sees], out[~sees]) and torch.equal(t.lse[~sees], lse[~sees])
+        byte[:2, 0, bad] = was
+    k, v = _new(62, batch, hkv, dtype)
+    v[0, 0, 0, 77] = float("inf")
+    t.cache.append_norm_rope_with_attention(0, t.op, 0, k, v, rope_table(keys, dtype).cuda(), positions=at, max_position=keys - 1)
+    torch.cuda.synchronize()
+    assert torch.equal(torch.isnan(t.lse), sees) and torch.equal(torch.isnan(t.out).all(dim=-1), sees)
+
+
 def test_rows_behind_the_last_sequence_stay():
     step = Layer(56, F16, 8, 2, [50] * 4, uniform=True)
     before = [t.clone() for pair in step.tensors() for t in pair]
