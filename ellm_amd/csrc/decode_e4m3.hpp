@@ -26,11 +26,11 @@ constexpr int kChunk8 = 32;   // keys per wave step
 // LDS of the stream lies behind what the waves are joined in: scales of a chunk, codes of a new row.
 static_assert(kRedBytes + kDecWaves * (2 * kChunk8 + 2 * kHeadDim) <= kDecWaves * kWaveLdsHalves * 2, "LDS of the single-token kernels");
 
-// The scale of the scores in log2 units.  (A score that is hidden is an infinity times this: a scale of zero is taken as one that no
-// finite product feels.)
+// The scale of the scores in log2 units.  (A score that is hidden is an infinity times this: a scale of zero is taken as 2^-149, which
+// makes at most 2^-21 of any finite product.  Kernels keep values below 2^-126 as they are.)
 inline float scale_log2_e4m3(float scale) {
   const float x = scale * kLog2e;
-  return x >= 1e-37f || x <= -1e-37f || !(x == x) ? x : 1e-37f;
+  return x == 0.0f ? 0x1p-149f : x;
 }
 
 // Query heads of a group as the B operand that goes with the keys' own order of dims: lane (head c, group g) holds

@@ -1566,8 +1566,9 @@ hipError_t launch_chunk(const AttnArgs& a, hipStream_t stream) {
   float c = a.scale * kLog2e;
   p.negate_q = c < 0.0f ? 1u : 0u;
   c = c < 0.0f ? -c : c;
-  // scale == 0 (uniform attention): a tiny positive c keeps -inf * c == -inf for masked keys
-  p.c = c > 0.0f ? c : 1e-37f;
+  // scale == 0 (uniform attention): a c above 0 keeps -inf * c == -inf for masked keys, and 2^-149 makes at most 2^-21 of any
+  // finite product
+  p.c = c > 0.0f ? c : 0x1p-149f;
   p.part_o = a.prefill_part_o;
   p.part_ml = a.prefill_part_ml;
   p.k_scale = a.k_scale;

@@ -187,6 +187,21 @@ def test_scales_of_zero_and_below(dtype, scale, interval, batch, keys):
     t.check([first] * batch)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-42, -1e-42])
+@pytest.mark.parametrize("interval,batch,keys", [(1, 2, 100), (1, 8, 9000), (20, 2, 60), (40, 1, 2040), (96, 2, 4200), (200, 1, 2500)])
+def test_scales_that_large_products_do_not_feel(scale, interval, batch, keys):
+    """Products of up to 2^124 under a scale of (nearly) zero: every key that is seen weighs the same."""
+    t = Layer(63, BF16, 8, 4, [keys] * batch, uniform=True, scale=scale, interval=interval)
+    t.tensors()[0][1].copy_(torch.where(t.tensors()[0][1] > 119, 178, 177))   # keys 2^50 and 2^51 times their codes
+    t.q.copy_(torch.where(t.q > 0, 2.0 ** 57, -2.0 ** 57))
+    first = keys - interval - (1 if interval == 1 else 0)
+    if interval == 1:
+        t.op.run_ragged(torch.full((batch,), first, dtype=torch.int32, device="cuda"), first, batch)
+    else:
+        t.op.run(first, interval, batch)
+    t.check([first] * batch)
+
+
 def test_two_recorded_steps_of_one_handle():
     """Recorded twice with different rows to write, replayed in turn with eager runs between: each as the eager call."""
     dtype, caps = BF16, [9000] * 16
