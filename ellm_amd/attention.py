@@ -81,6 +81,9 @@ class Attention:
         different capacities (then kv_strides[0] and sequence_capacity are not used)."""
         import torch
 
+        if seq_table is not None and seq_table.table is None:
+            raise ValueError("seq_table is a view of a cache with one capacity, which has no sequence table: leave it out, "
+                             "and pass k and v from the view's first sequence on")
         self._lib = load_library()
         self._keep = (q, k, v, out, lse, seq_table, kv_scales)
         self._e4m3 = kv_scales is not None
@@ -368,7 +371,8 @@ class KVCache:
         return wrap(k), wrap(v)
 
     def layer_e4m3(self, layer, first_sequence=0):
-        """One layer of a cache in 8 bits: what Attention takes beside its tensors (seq_table, strides)."""
+        """One layer of a cache in 8 bits: what Attention takes beside its tensors: .strides, and, of a cache with a capacity
+        for each sequence, the view itself as seq_table."""
         found = [ctypes.c_void_p() for _ in range(4)]
         strides = (ctypes.c_size_t * 4)()
         table = KvSeqTable() if self.capacities is not None else None
