@@ -185,3 +185,30 @@ def test_a_walked_launch_with_charged_starts(tmp_path):
     launches, bad = (int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True,
                                                     timeout=600).stdout.split())
     assert launches == 6000 and bad == 0
+
+
+@pytest.mark.parametrize("new_rows", ["false", "true"])
+def test_a_walked_launch_over_rows_in_8_bits(tmp_path, new_rows):
+    """The same with the charge and the workgroups of planes in 8 bits, of runs and of steps that write new rows."""
+    gxx = shutil.which("g++")
+    if not gxx:
+        pytest.skip("no g++")
+    text = WALK
+    for old, new in CHARGED + (
+        ("balanced_charge(umax, umin, total, B)", "balanced_charge(umax, umin, total, B, kBalancedChargeE4m3)"),
+        ("balanced_workgroups(grid, one_each, U, umax, umin, planes)",
+         f"balanced_workgroups_e4m3(grid, one_each, U, umax, umin, planes, umax - charge, {new_rows})"),
+        ("    ++launches;", "    ++launches; taken[W <= one_each]++;"),
+        ("unsigned long long launches = 0", "unsigned long long taken[2] = {0, 0}, launches = 0"),
+        ('printf("%llu %llu\\n", launches, bad)', 'printf("%llu %llu %llu %llu\\n", launches, bad, taken[0], taken[1])'),
+    ):
+        assert text.count(old) == 1, old
+        text = text.replace(old, new)
+    src = tmp_path / "walk.cpp"
+    src.write_text(text)
+    exe = tmp_path / "walk"
+    subprocess.run([gxx, "-O2", "-std=c++17", "-Wall", "-I", CSRC, str(src), "-o", str(exe)], check=True, timeout=300)
+    launches, bad, two, one = (int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True,
+                                                              timeout=600).stdout.split())
+    assert launches == 6000 and bad == 0
+    assert two > 1000 and one > 1000   # both one and two workgroups a unit
