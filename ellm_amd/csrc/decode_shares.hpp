@@ -99,7 +99,8 @@ ELLM_SHARES_FN uint32_t balanced_workgroups(uint32_t launched, uint32_t one_each
 // heads, 22.9 / 26.0); and where one cuts the longest plane (`longest` units of keys) into no more pieces than one fold takes, if two would
 // cut it into more (4 of 5742-11482, 40 / 8 heads, 19.8 / 21.9; 9 of 376-18764, 32 / 4, 23.6 / 25.3) or shares are long, so that their
 // starts count for little (28 of 6377-12753, 64 / 8, 88.2 / 90.7; 32 of 300-16000, 64 / 8, 98.5 / 99.6), but not with `new_rows` to write, which
-// a second workgroup hides (that call as a step 102.2 / 100.8; 64 of 500-9000, 32 / 4, 61.4 / 60.1).  Else two: 32 of 228-2279, 32 / 4, 15.7
+// a second workgroup hides (that call as a step 102.2 / 100.8; 64 of 500-9000, 32 / 4, 61.4 / 60.1; these two conditions make 1 to 3 %, less
+// than where a call's memory lies can).  Else two: 32 of 228-2279, 32 / 4, 15.7
 // / 14.1; 7 of 2993-5985, 40 / 8, 18.9 / 18.0; 3 of 20000-100000, 32 / 4, 49.8 / 48.0; 18 of 206-10269, 64 / 8, 40.8 / 39.2.
 ELLM_SHARES_FN uint32_t balanced_workgroups_e4m3(uint32_t launched, uint32_t one_each, uint32_t U, uint32_t umax,
                                                  uint32_t umin, uint32_t planes, uint32_t longest,

@@ -73,8 +73,8 @@ struct PrefillKernelArgs {
 // E4M3 (the template argument of the kernels below): planes of rows in 8 bits (e4m3.hpp), strides in codes.  A lane loads sixteen
 // codes at a time and converts them between the load's registers and LDS, once for all the rows that read the tile, so that
 // nothing else of a kernel changes: half the bytes, half the loads, one for a row's scales more, sixteen conversions a lane and tile of 32
-// rows.  Measured (us, 8 / 16 bits): 8192 tokens 505 / 485, 512 on 16000, 32 / 32 heads, 133 / 142, 33 x 5 on 777 12.0 / 11.3, 4 x 24 on 8000
-// 53.6 / 67.1.
+// rows.  Measured (us, 8 / 16 bits, every call on a layer of its own, rows from memory): 8192 tokens, binary16, 484 / 469; bfloat16: 512 on
+// 16000, 32 / 32 heads, 134-140 / 134-140, 33 x 5 on 777 12.4 / 12.5, 128 on 1000 14.4 / 13.2, 4 x 24 on 8000 58.5 / 66.8.
 constexpr uint32_t kElemBytes[2] = {2, 1};   // of a plane's element: [E4M3]
 
 // ---------------------------------------------------------------------------
